@@ -54,8 +54,11 @@ KERNEL_SOURCES = [
     "finalize.hip",
     "quality.hip",
     "capi_noalloc.hip",
+    "block_tables.hip",
+    "kv4_store.hip",
+    "kv4_attend.hip",
 ]
-HOST_SOURCES = ["capi.cpp"]
+HOST_SOURCES = ["capi.cpp", "capi_kv4.cpp"]
 
 
 def _run(cmd: list[str], quiet: bool = False) -> None:

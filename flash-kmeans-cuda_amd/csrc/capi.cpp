@@ -31,6 +31,8 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+void clear_error() { g_err[0] = 0; }
+
 int check_launch(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)

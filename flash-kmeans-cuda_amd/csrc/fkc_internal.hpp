@@ -12,6 +12,8 @@ namespace fkc {
 // ---------------------------------------------------------------- errors
 // Record a printf-style message as this thread's last error; returns `code`.
 int fail(int code, const char* fmt, ...);
+// Forget this thread's last error (every entry point starts with it).
+void clear_error();
 // Map the sticky launch status after a kernel launch to an FKC status.
 int check_launch(const char* what);
 
@@ -220,6 +222,40 @@ int launch_sampled_inertia(const void* x, const void* c, const int32_t* idx,
                            int64_t S, int64_t B, int64_t N, int64_t K,
                            int64_t D, int dtype, double* inertia, void* ws,
                            size_t ws_bytes, hipStream_t s);
+
+// ---------------------------------------------------------------- kv4
+// The 4-bit key/value cache of fkc.h; arguments are checked by the callers
+// (capi_kv4.cpp).  Strides are in elements.
+int launch_block_tables(const int32_t* seq, const int32_t* nw, int R,
+                        int32_t* tables, int64_t table_stride, int max_blocks,
+                        const int32_t* free_blocks, int64_t num_free,
+                        int block_size, int64_t num_tokens, int32_t* slots,
+                        int32_t* cu_new, int32_t* taken, hipStream_t s);
+struct Kv4Rows {
+  const void* p;
+  int64_t token_stride, head_stride;
+};
+int launch_kv4_append(const fkc_kv4_cache& c, Kv4Rows k, Kv4Rows v,
+                      const int32_t* slots, int64_t T, hipStream_t s);
+int launch_kv4_read(const fkc_kv4_cache& c, const int32_t* slots, int64_t T,
+                    void* k_out, void* v_out, hipStream_t s);
+struct Kv4Attend {
+  Kv4Rows q;
+  int64_t H, T;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t* seq;
+  const int32_t* cu_q;  // null: one query per request
+  int64_t R, max_seq;   // max_seq <= table entries * block_size
+  bool causal;
+  float sm_scale;
+  void* out;
+  float* lse;  // may be null
+};
+size_t kv4_attend_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int64_t T,
+                                  int64_t R, int64_t max_seq);
+int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& a, void* ws,
+                      size_t ws_bytes, hipStream_t s);
 
 // ---------------------------------------------------------------- loop
 // The Lloyd loop behind fkc_kmeans_lloyd*; profile = false ignores the

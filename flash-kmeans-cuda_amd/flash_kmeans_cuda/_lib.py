@@ -57,6 +57,11 @@ SIGNATURES = {
     "fkc_profile_assign_ms": (_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int64)]),
     "fkc_kmeans_sort_recounts_offset": (_sz, [_i64, _i64, _i64, _i64, _int, _int]),
     "fkc_assign_plan": (_int, [_i64, _i64, _i64, _i64, _int, _int, _vp]),
+    "fkc_block_tables": (_int, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "fkc_kv4_append": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "fkc_kv4_read": (_int, [_vp, _vp, _i64, _vp, _vp, _vp]),
+    "fkc_kv4_attend_workspace_bytes": (_sz, [_vp, _i64, _i64, _i64, _i64]),
+    "fkc_kv4_attend": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -347,6 +347,112 @@ FKC_CAPI size_t fkc_kmeans_sort_recounts_offset(int64_t B, int64_t N, int64_t K,
 FKC_CAPI int fkc_assign_plan(int64_t B, int64_t N, int64_t K, int64_t D,
                              int dtype, int slices, int32_t* plan);
 
+/*
+ * A paged key/value cache held in 4 bits (no counterpart in the reference;
+ * its levels are what the Lloyd loop above learns with K = 16 and D = 1).
+ * Slot i of block b holds one key and one value vector of every head h: D
+ * codes of 4 bits (element d in byte d/2, even d in the low half) and one
+ * scale; element d stands for scale * levels[h][code].
+ *   k_codes, v_codes    (num_blocks, heads, block_size, D/2) bytes
+ *   k_scales, v_scales  (num_blocks, heads, block_size) of dtype
+ *   k_levels, v_levels  (heads, 16) of dtype, in any order, finite
+ * all dense and 16-byte aligned; dtype FKC_F16 or FKC_BF16; D 64, 128 or 256;
+ * block_size a multiple of 16; num_blocks * block_size < 2^31.  A token's
+ * slot number is block * block_size + position in the block.
+ */
+typedef struct fkc_kv4_cache {
+  void* k_codes;
+  void* v_codes;
+  void* k_scales;
+  void* v_scales;
+  const void* k_levels;
+  const void* v_levels;
+  int64_t num_blocks;
+  int64_t heads;
+  int64_t block_size;
+  int64_t D;
+  int32_t dtype;
+} fkc_kv4_cache;
+
+/*
+ * Cache slots of a step's new tokens, from the requests' lengths alone.
+ * Request r has seq_lens[r] tokens after the step, the last new_lens[r] of
+ * them new; row r of tables (R rows, table_stride apart, max_blocks entries
+ * each) names the ceil((seq - new) / block_size) blocks it holds already.
+ * Each further block it needs is the next of free_blocks, in request order,
+ * and is written into tables.  Then
+ *   slots[cu_new[r] + i] = slot of token seq - new + i of request r,
+ *   cu_new (R + 1)       = running count of new tokens,
+ *   taken (1)            = blocks needed, those that free_blocks lacked too.
+ * slots has num_tokens entries; those past the last token are -1, and so are
+ * the slots (and table entries) of a block that free_blocks does not reach,
+ * of a position past max_blocks, and of a held block whose entry is negative.
+ * Tokens past num_tokens are dropped, but the table entries of their blocks
+ * are written.  Negative lengths count as 0, new_lens past seq_lens as
+ * seq_lens; the sums of both stay below 2^31.
+ */
+FKC_CAPI int fkc_block_tables(const int32_t* seq_lens, const int32_t* new_lens,
+                              int64_t R, int32_t* tables, int64_t table_stride,
+                              int64_t max_blocks, const int32_t* free_blocks,
+                              int64_t num_free, int64_t block_size,
+                              int64_t num_tokens, int32_t* slots,
+                              int32_t* cu_new, int32_t* taken,
+                              fkc_stream_t stream);
+
+/*
+ * Store T tokens' keys and values (T, heads, D) of the cache's dtype, strides
+ * in elements, rows of D contiguous and 16-byte aligned.  Per vector x:
+ *   s = max_d |x_d|  (held as the scale; 0 below 2^-126),
+ *   y_d = x_d * (1 / s)  (fp32, both steps rounded; 0 where s = 0),
+ *   code_d = the level at the smallest fp32 distance |y_d - level|, the
+ *            lowest index of equal ones (0 where y_d is NaN).
+ * A vector with an infinity or a NaN keeps it as its scale, so what is read
+ * back is not finite either.  Tokens whose slot is outside the cache (-1) are
+ * skipped; of two tokens with one slot either stays, scale and codes apart.
+ */
+FKC_CAPI int fkc_kv4_append(const fkc_kv4_cache* cache, const void* k,
+                            int64_t k_token_stride, int64_t k_head_stride,
+                            const void* v, int64_t v_token_stride,
+                            int64_t v_head_stride, const int32_t* slots,
+                            int64_t T, fkc_stream_t stream);
+
+/* k_out, v_out (T, heads, D) of the cache's dtype, dense: the vectors that
+ * the slots hold, scale * level rounded once; zeros for a slot outside the
+ * cache.  Either output may be NULL. */
+FKC_CAPI int fkc_kv4_read(const fkc_kv4_cache* cache, const int32_t* slots,
+                          int64_t T, void* k_out, void* v_out,
+                          fkc_stream_t stream);
+
+/*
+ * Attention of T queries over the cache.  q (T, H, D) of the cache's dtype,
+ * strides in elements, rows of D contiguous and 16-byte aligned; query head h
+ * reads cache head h / (H / heads).  Request r owns the queries
+ * cu_q[r] .. cu_q[r+1] (cu_q NULL: T = R, one query each), which are its last
+ * tokens: query i of n sits at position seq_lens[r] - n + i and sees the
+ * tokens up to it (causal) or all seq_lens[r] of them.  Token t lies in block
+ * tables[r * table_stride + t / block_size]; tokens of a block outside the
+ * cache are not seen.  Over the seen tokens
+ *   z_t = sm_scale * <q, k_t>,  out = sum_t softmax(z)_t v_t  (T, H, D) dense,
+ *   lse = log sum_t exp(z_t)  (T, H) fp32, may be NULL;
+ * a query that sees nothing gets out = 0 and lse = -infinity.  Lengths past
+ * max_seq (at most max_blocks * block_size) are cut to it.  What the cache
+ * holds past a request's length is never used, whatever its bits.  Scores,
+ * maxima, sums and outputs are kept in fp32; the weights softmax * scale are
+ * rounded to dtype for the matrix cores.  H <= 16384; T * H < 2^31.
+ */
+FKC_CAPI size_t fkc_kv4_attend_workspace_bytes(const fkc_kv4_cache* cache,
+                                               int64_t H, int64_t T, int64_t R,
+                                               int64_t max_seq);
+FKC_CAPI int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
+                            int64_t q_token_stride, int64_t q_head_stride,
+                            int64_t H, int64_t T, const int32_t* tables,
+                            int64_t table_stride, int64_t max_blocks,
+                            const int32_t* seq_lens, const int32_t* cu_q,
+                            int64_t R, int64_t max_seq, int causal,
+                            float sm_scale, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes,
+                            fkc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
