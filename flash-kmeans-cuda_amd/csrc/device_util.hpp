@@ -128,19 +128,21 @@ __device__ inline void drain_before_announce() {
 
 // n / d for 0 <= n < 2^31 by one high multiply: with l = ceil(log2 d) and
 // m = floor(2^(31+l) / d) + 1 < 2^32, n / d = n * m >> (31 + l) (the excess of
-// m over 2^(31+l) / d adds less than n / 2^(31+l) < 2^-l <= 1/d).
+// m over 2^(31+l) / d adds less than n / 2^(31+l) < 2^-l <= 1/d).  d = 1 has no
+// such m and is kept as m = 0.
 struct FastDiv {
   uint32_t m;
   int sh;
   uint32_t d;
   __host__ explicit FastDiv(uint32_t div) : m(0), sh(0), d(div) {
+    if (div <= 1) return;
     int l = 1;
-    while ((1u << l) < div && l < 31) ++l;
+    while (l < 31 && (1u << l) < div) ++l;
     m = (uint32_t)((1ull << (31 + l)) / div) + 1u;
     sh = l - 1;
   }
   __device__ inline uint32_t div(uint32_t n) const {
-    return __umulhi(n, m) >> sh;
+    return m ? __umulhi(n, m) >> sh : n;
   }
 };
 
