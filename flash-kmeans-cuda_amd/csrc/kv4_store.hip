@@ -8,7 +8,8 @@
 // Bound by memory: 2 D bytes in and D / 2 + 2 out per vector, so the search
 // has to cost less than the ~25 vector-ALU operations per element that the
 // time of those bytes has room for.  Sixteen distances, compares and selects
-// are 64; the sorted levels' thresholds halved four times are 23.
+// are 64, halving the sorted levels' 15 thresholds 33; one look into a table of
+// y's CELLS cells, each with the one threshold that falls into it, is 10.
 #include <algorithm>
 #include <type_traits>
 
@@ -22,130 +23,121 @@ constexpr int LV = 16;           // levels per head
 constexpr int KT = 256;          // threads per workgroup
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 
-// Levels of one head, ready for the search.
-struct Levels {
-  float raw[LV];    // as stored
-  float uniq[LV];   // ascending, without repeats
-  int order[LV];    // index of uniq[j]: the lowest of equal levels
-  int dup[LV];      // raw[i] repeats a level of lower index
-  float thr[LV];    // smallest y that takes uniq[j + 1] before uniq[j]
-  int n;            // distinct levels
-  int plain;        // thresholds do not describe the search: compare them all
-};
-
-// Order-preserving map of finite floats to integers and back (+0 and -0
-// apart, which compare equal: no threshold is between them).
-__device__ inline int64_t float_key(float f) {
-  const int32_t b = __float_as_int(f);
-  return b < 0 ? -(int64_t)(b & 0x7fffffff) - 1 : (int64_t)b;
+// Order-preserving map of finite floats to integers and back.
+__device__ inline uint32_t float_key(float f) {
+  const uint32_t b = __float_as_uint(f);
+  return b >> 31 ? ~b : b | 0x80000000u;
 }
-__device__ inline float key_float(int64_t k) {
-  return k < 0 ? __int_as_float((int32_t)(-(k + 1)) | (int32_t)0x80000000)
-               : __int_as_float((int32_t)k);
+__device__ inline float key_float(uint32_t k) {
+  return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
-// Thresholds of the levels, by the whole workgroup.  Between neighbours a < b
-// the distances y - a and b - y, rounded, rise and fall with y, so the choice
-// "b before a" (nearer, or as near with the lower index) turns once, at an
-// exact fp32 y within a few roundings of the middle; 16 lanes look for it,
-// each round 16 places at once.  Farther levels cannot interfere while
-// neighbours are so far apart that no rounded distance (|y| <= 1 + 2^-23) can
-// make two of them equal: 2^-20 of the largest distance; levels closer than
-// that, or not finite, are compared one by one instead.
+// Cells of y, rising with y.  Quotients by the largest magnitude (|y| <= 1 +
+// 2^-23) and NaN are inside; thresholds anywhere are moved in.
+constexpr int CELLS = 1024;
+__device__ inline uint32_t cell_of(float y) {
+  return (uint32_t)(int)__builtin_fmaf(y, CELLS / 2 - 0.125f, (float)(CELLS / 2));
+}
+__device__ inline uint32_t cell_of_any(float y) { return cell_of(fminf(fmaxf(y, -1.f), 1.f)); }
+
+// Fills the table of a head's levels, by the whole workgroup: cell c holds a
+// threshold and the codes below it (4 bits) and from it on (the next 4).
+// Returns whether the table describes the choice; if not, every level has to
+// be compared.
+//
+// Between neighbours a < b the distances y - a and b - y, rounded, rise and
+// fall with y, so the choice "b before a" (nearer, or as near with the lower
+// index) turns once, at an exact fp32 threshold within a rounding of a distance
+// of the middle; the four 16-lane rows of a wave look for it, four places a
+// round, lane j of a row for the one above the j-th smallest level.  Farther
+// levels cannot interfere while neighbours are so far apart that no rounded
+// distance can make two of them equal: 2^-20 of the largest distance.  Levels
+// closer than that, not finite, or with two thresholds in one cell are left to
+// the plain comparison; equal ones count as the one of lowest index.
 template <int DT>
-__device__ void prepare_levels(Levels& L, const typename Elem<DT>::T* lv) {
+__device__ inline bool fill_cells(const typename Elem<DT>::T* lv, uint2* cells) {
 #pragma clang fp contract(off)
-  const int t = threadIdx.x;
-  if (t < LV) L.raw[t] = Elem<DT>::load(lv[t]);
-  if (t == 0) L.plain = 0;
-  __syncthreads();
-  if (t < LV) {
-    int dup = 0;
-    for (int i = 0; i < t; ++i) dup |= L.raw[i] == L.raw[t];
-    L.dup[t] = dup;
-    L.thr[t] = INFINITY;
-    L.uniq[t] = 0.f;
-    L.order[t] = 0;
+  const int lane = threadIdx.x & 63, i = lane & 15;
+  const float mine = Elem<DT>::load(lv[i]);
+  int rank = 0, same = i;
+#pragma unroll
+  for (int c = LV - 1; c >= 0; --c) {
+    const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), c));
+    const bool eq = other == mine;
+    rank += other < mine || (eq && c < i);
+    same = eq ? c : same;  // ends with the lowest
   }
-  __syncthreads();
-  if (t < LV && !L.dup[t]) {
-    int rank = 0;
-    for (int i = 0; i < LV; ++i) rank += !L.dup[i] && L.raw[i] < L.raw[t];
-    L.uniq[rank] = L.raw[t];
-    L.order[rank] = t;
-  }
-  if (t == 0) {
-    int n = 0;
-    for (int i = 0; i < LV; ++i) n += !L.dup[i];
-    L.n = n;
-  }
-  __syncthreads();
-  const int n = L.n;
-  if (t < LV) {
-    const float far = 1.f + fmaxf(fabsf(L.uniq[0]), fabsf(L.uniq[n - 1]));
-    const bool ok = t + 1 < n ? L.uniq[t + 1] - L.uniq[t] >= far * 0x1p-20f
-                              : fabsf(L.raw[t]) < INFINITY;
-    if (!ok || !(fabsf(L.raw[t]) < INFINITY)) L.plain = 1;  // every writer stores 1
-  }
-  __syncthreads();
-  const int j = t / 16, lane = t & 15;
-  if (!L.plain && j + 1 < n) {
-    const float a = L.uniq[j], b = L.uniq[j + 1];
-    const bool lower = L.order[j + 1] < L.order[j];
-    const float mid = 0.5f * a + 0.5f * b;
-    const float e = (b - a) * 0x1p-20f + fabsf(mid) * 0x1p-22f;
-    int64_t lo = float_key(fmaxf(a, mid - e)), hi = float_key(fminf(b, mid + e));
-    // lo takes a, hi takes b; at most 9 rounds from the widest interval.
-    while (hi - lo > 1) {
-      const int64_t at = lo + (hi - lo) * (lane + 1) / 17;
-      const float y = key_float(at);
-      const float da = y - a, db = b - y;
-      const bool takes_b = db < da || (db == da && lower);
-      const uint64_t m = __ballot(takes_b) >> (threadIdx.x & 48);
-      const int first = __builtin_ctz((uint32_t)m & 0xffffu | 0x10000u);
-      const int64_t w = hi - lo;
-      hi = first < 16 ? lo + w * (first + 1) / 17 : hi;
-      lo = first > 0 ? lo + w * first / 17 : lo;
+  const int to = ((lane & 48) | rank) * 4;
+  const float a = __int_as_float(__builtin_amdgcn_ds_permute(to, __float_as_int(mine)));
+  const int idx = __builtin_amdgcn_ds_permute(to, same);
+  const int next = min(lane + 1, 63) * 4;
+  const float b = __int_as_float(__builtin_amdgcn_ds_bpermute(next, __float_as_int(a)));
+  const int idx_b = __builtin_amdgcn_ds_bpermute(next, idx);
+  const float far =
+      1.f + fmaxf(fabsf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 0))),
+                  fabsf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), LV - 1))));
+  const bool pair = i + 1 < LV && b != a;  // this lane has a threshold to find
+  bool bad = !(fabsf(mine) < INFINITY) || (pair && !(b - a >= far * 0x1p-20f));
+  if (__any(bad)) return false;  // the same for every wave
+  const float mid = 0.5f * a + 0.5f * b;
+  const float e = (b - a) * 0x1p-22f + fabsf(mid) * 0x1p-22f;
+  uint32_t lo = pair ? float_key(fmaxf(a, mid - e)) : 0;  // takes a
+  uint32_t hi = pair ? float_key(fminf(b, mid + e)) : 1;  // takes b
+  while (__any(hi - lo > 1)) {  // at most a fifth and four are left each round
+    const uint32_t step = max((hi - lo) / 5, 1u);
+    const float y = key_float(min(lo + step * (lane / 16 + 1), hi));
+    const float da = y - a, db = b - y;
+    const uint64_t m = __ballot(db < da || (db == da && idx_b < idx)) >> i;
+    const uint32_t first =
+        (m & 1) ? 0 : (m >> 16 & 1) ? 1 : (m >> 32 & 1) ? 2 : (m >> 48 & 1) ? 3 : 4;
+    if (hi - lo > 1) {
+      if (first < 4) hi = min(lo + step * (first + 1), hi);
+      lo += step * first;
     }
-    if (lane == 0) L.thr[j] = key_float(hi);
+  }
+  const float thr = pair ? key_float(hi) : INFINITY;
+  const uint32_t cell = pair ? cell_of_any(thr) : CELLS;
+  // Codes below the cells' thresholds: those from the last threshold of the
+  // cells before on.
+  uint32_t code[CELLS / KT], prev = CELLS;
+#pragma unroll
+  for (int c = 0; c < CELLS / KT; ++c) code[c] = __builtin_amdgcn_readlane(idx, 0);
+#pragma unroll
+  for (int j = 0; j < LV - 1; ++j) {
+    const uint32_t at = __builtin_amdgcn_readlane((int)cell, j);
+    const uint32_t id = __builtin_amdgcn_readlane(idx, j + 1);
+    bad |= at < CELLS && at == prev;
+    prev = at < CELLS ? at : prev;
+#pragma unroll
+    for (int c = 0; c < CELLS / KT; ++c)
+      code[c] = at < threadIdx.x + c * KT ? id : code[c];
+  }
+  if (__any(bad)) return false;
+#pragma unroll
+  for (int c = 0; c < CELLS / KT; ++c)
+    cells[threadIdx.x + c * KT] = uint2{__float_as_uint(INFINITY), code[c]};
+  __syncthreads();
+  if (threadIdx.x < LV && cell < CELLS) {
+    // equal levels in a row: the first of them is what lies below
+    cells[cell] = uint2{__float_as_uint(thr), (uint32_t)idx | (uint32_t)idx_b << 4};
   }
   __syncthreads();
+  return true;
 }
 
-// The rows of one head that a workgroup stores: D / 8 lanes per vector.
-template <int DT, int D>
-__global__ void __launch_bounds__(KT)
-kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
-                  int T, int per_wg, uint32_t* __restrict__ k_codes,
-                  uint32_t* __restrict__ v_codes, uint16_t* __restrict__ k_scales,
-                  uint16_t* __restrict__ v_scales, const uint16_t* __restrict__ k_levels,
-                  const uint16_t* __restrict__ v_levels, int heads, FastDiv bs,
-                  uint32_t num_slots) {
+// The rows of one head that a workgroup stores, D / 8 lanes per vector, NB
+// passes of the workgroup at a time.
+template <int DT, int D, int NB, bool PLAIN>
+__device__ inline void store_rows(const uint2* cells, const typename Elem<DT>::T* __restrict__ levels,
+                                  const uint16_t* __restrict__ base, int64_t token_stride,
+                                  const int32_t* __restrict__ slots, int t0, int t1,
+                                  uint32_t* __restrict__ codes, uint16_t* __restrict__ scales,
+                                  int heads, int h, FastDiv bs, uint32_t num_slots) {
 #pragma clang fp contract(off)
   using E = Elem<DT>;
   using T16 = typename E::T;
-  constexpr int LPV = D / 8;        // lanes per vector, 8 elements each
-  constexpr int VP = KT / LPV;      // vectors per pass of the workgroup
-  constexpr int NB = 4;             // passes in flight
-  __shared__ Levels L;
-  const int h = blockIdx.y;
-  const bool isv = blockIdx.z != 0;
-  const Kv4Rows src = isv ? vr : kr;
-  uint32_t* codes = isv ? v_codes : k_codes;
-  uint16_t* scales = isv ? v_scales : k_scales;
-  prepare_levels<DT>(L, reinterpret_cast<const T16*>(isv ? v_levels : k_levels) + h * LV);
-  float thr[LV - 1];
-#pragma unroll
-  for (int i = 0; i < LV - 1; ++i) thr[i] = L.thr[i];
-  uint64_t order = 0;
-  for (int i = 0; i < LV; ++i) order |= (uint64_t)L.order[i] << (4 * i);
-  const bool plain = L.plain != 0;
-
+  constexpr int LPV = D / 8, VP = KT / LPV;
   const int sub = threadIdx.x % LPV, vec = threadIdx.x / LPV;
-  const uint16_t* base = static_cast<const uint16_t*>(src.p) +
-                         (int64_t)h * src.head_stride + sub * 8;
-  const int t0 = blockIdx.x * per_wg;
-  const int t1 = min(T, t0 + per_wg);
   for (int tb = t0; tb < t1; tb += NB * VP) {
     uint4 x[NB];
     uint32_t slot[NB];
@@ -153,9 +145,13 @@ kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
     for (int i = 0; i < NB; ++i) {
       const int tok = tb + i * VP + vec;
       slot[i] = tok < t1 ? (uint32_t)slots[tok] : 0xffffffffu;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
       // a token that is not stored is not read either
+      const int tok = tb + i * VP + vec;
       x[i] = slot[i] < num_slots
-                 ? *reinterpret_cast<const uint4*>(base + (int64_t)tok * src.token_stride)
+                 ? *reinterpret_cast<const uint4*>(base + (int64_t)tok * token_stride)
                  : uint4{0, 0, 0, 0};
     }
 #pragma unroll
@@ -175,38 +171,41 @@ kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
         top = 0;
       }
       const float inv = s > 0.f ? 1.f / s : 0.f;
-      const bool finite = s < INFINITY;
-      uint32_t word = 0;
+      float y[8];
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
         const uint16_t bits = (uint16_t)(w[d / 2] >> (16 * (d & 1)));
-        const float y = E::load(__builtin_bit_cast(T16, bits)) * inv;
-        uint32_t code;
-        if (!plain && finite) {
-          // Thresholds below y: halve 15, 7, 3, 1 of them.
-          float u[7], v[3];
-          const bool c3 = y >= thr[7];
+        y[d] = E::load(__builtin_bit_cast(T16, bits)) * inv;
+      }
+      uint32_t word = 0;
+      if constexpr (PLAIN) {
+        float best[8];
 #pragma unroll
-          for (int q = 0; q < 7; ++q) u[q] = c3 ? thr[8 + q] : thr[q];
-          const bool c2 = y >= u[3];
+        for (int d = 0; d < 8; ++d) best[d] = fabsf(y[d] - E::load(levels[0]));
+#pragma unroll 1
+        for (int c = 1; c < LV; ++c) {
+          const float lv = E::load(levels[c]);
 #pragma unroll
-          for (int q = 0; q < 3; ++q) v[q] = c2 ? u[4 + q] : u[q];
-          const bool c1 = y >= v[1];
-          const bool c0 = y >= (c1 ? v[2] : v[0]);
-          const uint32_t rank = (c3 ? 8 : 0) + (c2 ? 4 : 0) + (c1 ? 2 : 0) + (c0 ? 1 : 0);
-          code = (uint32_t)(order >> (4 * rank)) & 15u;
-        } else {
-          code = 0;
-          float best = fabsf(y - L.raw[0]);
-          for (int c = 1; c < LV; ++c) {
-            const float dist = fabsf(y - L.raw[c]);
-            if (dist < best) {
-              best = dist;
-              code = c;
+          for (int d = 0; d < 8; ++d) {
+            const float dist = fabsf(y[d] - lv);
+            if (dist < best[d]) {
+              best[d] = dist;
+              word = (word & ~(15u << (4 * d))) | (uint32_t)c << (4 * d);
             }
           }
         }
-        word |= code << (4 * d);
+      } else {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const uint2 e = cells[cell_of(y[d])];
+          word |= (e.y >> (y[d] >= __uint_as_float(e.x) ? 4 : 0) & 15u) << (4 * d);
+        }
+      }
+      // An element over an infinity or a NaN that is neither 0 takes level 0.
+      if (!PLAIN && !(s < INFINITY)) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+          if (y[d] != y[d]) word &= ~(15u << (4 * d));
       }
       if (slot[i] < num_slots) {
         const uint32_t blk = bs.div(slot[i]);
@@ -216,6 +215,35 @@ kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
       }
     }
   }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(KT)
+kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
+                  int T, int per_wg, uint32_t* __restrict__ k_codes,
+                  uint32_t* __restrict__ v_codes, uint16_t* __restrict__ k_scales,
+                  uint16_t* __restrict__ v_scales, const uint16_t* __restrict__ k_levels,
+                  const uint16_t* __restrict__ v_levels, int heads, FastDiv bs,
+                  uint32_t num_slots) {
+  using T16 = typename Elem<DT>::T;
+  const int h = blockIdx.y;
+  const bool isv = blockIdx.z != 0;
+  const Kv4Rows src = isv ? vr : kr;
+  const T16* levels = reinterpret_cast<const T16*>(isv ? v_levels : k_levels) + h * LV;
+  __shared__ uint2 cells[CELLS];
+  const bool table = fill_cells<DT>(levels, cells);
+  const uint16_t* base = static_cast<const uint16_t*>(src.p) + (int64_t)h * src.head_stride +
+                         threadIdx.x % (D / 8) * 8;
+  const int t0 = blockIdx.x * per_wg;
+  const int t1 = min(T, t0 + per_wg);
+  uint32_t* codes = isv ? v_codes : k_codes;
+  uint16_t* scales = isv ? v_scales : k_scales;
+  if (table)
+    store_rows<DT, D, 4, false>(cells, levels, base, src.token_stride, slots, t0, t1, codes,
+                                scales, heads, h, bs, num_slots);
+  else
+    store_rows<DT, D, 1, true>(cells, levels, base, src.token_stride, slots, t0, t1, codes,
+                               scales, heads, h, bs, num_slots);
 }
 
 // The reverse: eight elements per lane, levels in LDS once per bank so that
