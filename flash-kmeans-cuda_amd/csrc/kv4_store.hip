@@ -20,7 +20,7 @@ namespace fkc {
 namespace {
 
 constexpr int LV = 16;           // levels per head
-constexpr int KT = 256;          // threads per workgroup
+constexpr int KT = 512;          // threads per workgroup
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126
 
 // Order-preserving map of finite floats to integers and back.
@@ -32,11 +32,13 @@ __device__ inline float key_float(uint32_t k) {
   return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
-// Cells of y, rising with y.  Quotients by the largest magnitude (|y| <= 1 +
-// 2^-23) and NaN are inside; thresholds anywhere are moved in.
+// Cells of y, rising with y, as the byte offset of their entry: in the sum with
+// 2^20 the last bit counts eighths of a cell.  Any y has one (NaN the first);
+// quotients by the largest magnitude (|y| <= 1 + 2^-23) have their own.
 constexpr int CELLS = 1024;
 __device__ inline uint32_t cell_of(float y) {
-  return (uint32_t)(int)__builtin_fmaf(y, CELLS / 2 - 0.125f, (float)(CELLS / 2));
+  const float f = __builtin_fmaf(y, CELLS / 2 - 0.25f, 0x1p20f + CELLS / 2);
+  return __float_as_uint(f) & (CELLS - 1) * 8u;
 }
 __device__ inline uint32_t cell_of_any(float y) { return cell_of(fminf(fmaxf(y, -1.f), 1.f)); }
 
@@ -48,177 +50,215 @@ __device__ inline uint32_t cell_of_any(float y) { return cell_of(fminf(fmaxf(y, 
 // Between neighbours a < b the distances y - a and b - y, rounded, rise and
 // fall with y, so the choice "b before a" (nearer, or as near with the lower
 // index) turns once, at an exact fp32 threshold within a rounding of a distance
-// of the middle; the four 16-lane rows of a wave look for it, four places a
-// round, lane j of a row for the one above the j-th smallest level.  Farther
-// levels cannot interfere while neighbours are so far apart that no rounded
-// distance can make two of them equal: 2^-20 of the largest distance.  Levels
-// closer than that, not finite, or with two thresholds in one cell are left to
-// the plain comparison; equal ones count as the one of lowest index.
+// of the middle; the four 16-lane rows of the first wave look for it, four
+// places a round, lane j of a row for the one above the j-th smallest level.
+// Farther levels cannot interfere while neighbours are so far apart that no
+// rounded distance can make two of them equal: 2^-20 of the largest distance.
+// Levels closer than that, not finite, or with two thresholds in one cell are
+// left to the plain comparison; equal ones count as the one of lowest index.
+struct Cells {
+  uint2 at[CELLS];
+  uint32_t cell[LV], code[LV];  // of threshold j; of the j-th smallest level
+  int bad;
+};
+
 template <int DT>
-__device__ inline bool fill_cells(const typename Elem<DT>::T* lv, uint2* cells) {
+__device__ inline bool fill_cells(const typename Elem<DT>::T* lv, Cells& t) {
 #pragma clang fp contract(off)
-  const int lane = threadIdx.x & 63, i = lane & 15;
-  const float mine = Elem<DT>::load(lv[i]);
-  int rank = 0, same = i;
+  float thr = INFINITY;
+  uint32_t cell = CELLS * 8, codes = 0;
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x, i = lane & 15;
+    const float mine = Elem<DT>::load(lv[i]);
+    int rank = 0, same = i;
 #pragma unroll
-  for (int c = LV - 1; c >= 0; --c) {
-    const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), c));
-    const bool eq = other == mine;
-    rank += other < mine || (eq && c < i);
-    same = eq ? c : same;  // ends with the lowest
-  }
-  const int to = ((lane & 48) | rank) * 4;
-  const float a = __int_as_float(__builtin_amdgcn_ds_permute(to, __float_as_int(mine)));
-  const int idx = __builtin_amdgcn_ds_permute(to, same);
-  const int next = min(lane + 1, 63) * 4;
-  const float b = __int_as_float(__builtin_amdgcn_ds_bpermute(next, __float_as_int(a)));
-  const int idx_b = __builtin_amdgcn_ds_bpermute(next, idx);
-  const float far =
-      1.f + fmaxf(fabsf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 0))),
-                  fabsf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), LV - 1))));
-  const bool pair = i + 1 < LV && b != a;  // this lane has a threshold to find
-  bool bad = !(fabsf(mine) < INFINITY) || (pair && !(b - a >= far * 0x1p-20f));
-  if (__any(bad)) return false;  // the same for every wave
-  const float mid = 0.5f * a + 0.5f * b;
-  const float e = (b - a) * 0x1p-22f + fabsf(mid) * 0x1p-22f;
-  uint32_t lo = pair ? float_key(fmaxf(a, mid - e)) : 0;  // takes a
-  uint32_t hi = pair ? float_key(fminf(b, mid + e)) : 1;  // takes b
-  while (__any(hi - lo > 1)) {  // at most a fifth and four are left each round
-    const uint32_t step = max((hi - lo) / 5, 1u);
-    const float y = key_float(min(lo + step * (lane / 16 + 1), hi));
-    const float da = y - a, db = b - y;
-    const uint64_t m = __ballot(db < da || (db == da && idx_b < idx)) >> i;
-    const uint32_t first =
-        (m & 1) ? 0 : (m >> 16 & 1) ? 1 : (m >> 32 & 1) ? 2 : (m >> 48 & 1) ? 3 : 4;
-    if (hi - lo > 1) {
-      if (first < 4) hi = min(lo + step * (first + 1), hi);
-      lo += step * first;
+    for (int c = LV - 1; c >= 0; --c) {
+      const float other = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), c));
+      const bool eq = other == mine;
+      rank += other < mine || (eq && c < i);
+      same = eq ? c : same;  // ends with the lowest
     }
+    // (NaN, which ranks below nothing, sends several lanes to one place: bad.)
+    const int to = ((lane & 48) | rank) * 4;
+    const float a = __int_as_float(__builtin_amdgcn_ds_permute(to, __float_as_int(mine)));
+    const int idx = __builtin_amdgcn_ds_permute(to, same);
+    const int next = min(lane + 1, 63) * 4;
+    const float b = __int_as_float(__builtin_amdgcn_ds_bpermute(next, __float_as_int(a)));
+    const int idx_b = __builtin_amdgcn_ds_bpermute(next, idx);
+    const float far =
+        1.f + fmaxf(fabsf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), 0))),
+                    fabsf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(a), LV - 1))));
+    const bool pair = i + 1 < LV && b != a;  // this lane has a threshold to find
+    bool bad = __any(!(fabsf(mine) < INFINITY) || (pair && !(b - a >= far * 0x1p-20f)));
+    const float mid = 0.5f * a + 0.5f * b;
+    const float e = (b - a) * 0x1p-22f + fabsf(mid) * 0x1p-22f;
+    uint32_t lo = pair && !bad ? float_key(fmaxf(a, mid - e)) : 0;  // takes a
+    uint32_t hi = pair && !bad ? float_key(fminf(b, mid + e)) : 1;  // takes b
+    while (__any(hi - lo > 1)) {  // at most a fifth and four are left each round
+      const uint32_t step = max((hi - lo) / 5, 1u);
+      const float y = key_float(min(lo + step * (lane / 16 + 1), hi));
+      const float da = y - a, db = b - y;
+      const uint64_t m = __ballot(db < da || (db == da && idx_b < idx)) >> i;
+      const uint32_t first =
+          (m & 1) ? 0 : (m >> 16 & 1) ? 1 : (m >> 32 & 1) ? 2 : (m >> 48 & 1) ? 3 : 4;
+      if (hi - lo > 1) {
+        if (first < 4) hi = min(lo + step * (first + 1), hi);
+        lo += step * first;
+      }
+    }
+    if (pair && !bad) {
+      thr = key_float(hi);
+      cell = cell_of_any(thr);
+    }
+    codes = (uint32_t)idx | (uint32_t)idx_b << 4;
+    uint32_t prev = CELLS * 8;
+#pragma unroll
+    for (int j = 0; j < LV - 1; ++j) {
+      const uint32_t at = __builtin_amdgcn_readlane((int)cell, j);
+      bad |= at < CELLS * 8 && at == prev;
+      prev = at < CELLS * 8 ? at : prev;
+    }
+    if (lane < LV) {
+      t.cell[lane] = cell / 8;
+      t.code[lane] = (uint32_t)idx;
+    }
+    if (lane == 0) t.bad = bad;
   }
-  const float thr = pair ? key_float(hi) : INFINITY;
-  const uint32_t cell = pair ? cell_of_any(thr) : CELLS;
+  __syncthreads();
+  if (t.bad) return false;
   // Codes below the cells' thresholds: those from the last threshold of the
   // cells before on.
-  uint32_t code[CELLS / KT], prev = CELLS;
+  uint32_t code[CELLS / KT];
 #pragma unroll
-  for (int c = 0; c < CELLS / KT; ++c) code[c] = __builtin_amdgcn_readlane(idx, 0);
+  for (int c = 0; c < CELLS / KT; ++c) code[c] = t.code[0];
 #pragma unroll
   for (int j = 0; j < LV - 1; ++j) {
-    const uint32_t at = __builtin_amdgcn_readlane((int)cell, j);
-    const uint32_t id = __builtin_amdgcn_readlane(idx, j + 1);
-    bad |= at < CELLS && at == prev;
-    prev = at < CELLS ? at : prev;
+    const uint32_t at = t.cell[j], id = t.code[j + 1];
 #pragma unroll
     for (int c = 0; c < CELLS / KT; ++c)
       code[c] = at < threadIdx.x + c * KT ? id : code[c];
   }
-  if (__any(bad)) return false;
 #pragma unroll
   for (int c = 0; c < CELLS / KT; ++c)
-    cells[threadIdx.x + c * KT] = uint2{__float_as_uint(INFINITY), code[c]};
+    t.at[threadIdx.x + c * KT] = uint2{__float_as_uint(INFINITY), code[c]};
   __syncthreads();
-  if (threadIdx.x < LV && cell < CELLS) {
-    // equal levels in a row: the first of them is what lies below
-    cells[cell] = uint2{__float_as_uint(thr), (uint32_t)idx | (uint32_t)idx_b << 4};
-  }
+  if (threadIdx.x < LV && cell < CELLS * 8)
+    t.at[cell / 8] = uint2{__float_as_uint(thr), codes};
   __syncthreads();
   return true;
 }
 
-// The rows of one head that a workgroup stores, D / 8 lanes per vector, NB
-// passes of the workgroup at a time.
-template <int DT, int D, int NB, bool PLAIN>
-__device__ inline void store_rows(const uint2* cells, const typename Elem<DT>::T* __restrict__ levels,
-                                  const uint16_t* __restrict__ base, int64_t token_stride,
-                                  const int32_t* __restrict__ slots, int t0, int t1,
-                                  uint32_t* __restrict__ codes, uint16_t* __restrict__ scales,
-                                  int heads, int h, FastDiv bs, uint32_t num_slots) {
-#pragma clang fp contract(off)
-  using E = Elem<DT>;
-  using T16 = typename E::T;
-  constexpr int LPV = D / 8, VP = KT / LPV;
-  const int sub = threadIdx.x % LPV, vec = threadIdx.x / LPV;
-  for (int tb = t0; tb < t1; tb += NB * VP) {
-    uint4 x[NB];
-    uint32_t slot[NB];
+// NB passes of a workgroup over the rows of one head, D / 8 lanes per vector.
+template <int D, int NB>
+struct Batch {
+  static constexpr int LPV = D / 8, VP = KT / LPV;
+  uint4 x[NB];
+  uint32_t slot[NB];
+  __device__ inline void load(const uint16_t* base, int64_t token_stride,
+                              const int32_t* slots, int tb, int t1, uint32_t num_slots) {
+    const int first = tb + threadIdx.x / LPV;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int tok = tb + i * VP + vec;
+      const int tok = first + i * VP;
       slot[i] = tok < t1 ? (uint32_t)slots[tok] : 0xffffffffu;
     }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      // a token that is not stored is not read either
-      const int tok = tb + i * VP + vec;
-      x[i] = slot[i] < num_slots
-                 ? *reinterpret_cast<const uint4*>(base + (int64_t)tok * token_stride)
-                 : uint4{0, 0, 0, 0};
+    for (int i = 0; i < NB; ++i)  // a token that is not stored is not read either
+      x[i] = slot[i] < num_slots ? *reinterpret_cast<const uint4*>(
+                                       base + (int64_t)(first + i * VP) * token_stride)
+                                 : uint4{0, 0, 0, 0};
+  }
+};
+
+// The largest of v over the LPV lanes of a vector.
+template <int LPV>
+__device__ inline uint32_t vector_max(uint32_t v) {
+#define FKC_DPP_MAX(CTRL) \
+  v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true))
+  FKC_DPP_MAX(0xB1);   // quad_perm [1,0,3,2]
+  FKC_DPP_MAX(0x4E);   // quad_perm [2,3,0,1]
+  FKC_DPP_MAX(0x141);  // row_half_mirror: 8 lanes
+  if (LPV > 8) FKC_DPP_MAX(0x140);  // row_mirror: 16 lanes
+#undef FKC_DPP_MAX
+  if (LPV > 16) v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+  return v;
+}
+
+template <int DT, int D, bool PLAIN, int NB>
+__device__ inline void store_batch(const Batch<D, NB>& in, const Cells& t,
+                                   const typename Elem<DT>::T* levels, uint32_t* codes,
+                                   uint16_t* scales, int heads, int h, FastDiv bs,
+                                   uint32_t num_slots) {
+#pragma clang fp contract(off)
+  using E = Elem<DT>;
+  using T16 = typename E::T;
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  constexpr int LPV = D / 8;
+  const int sub = threadIdx.x % LPV;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) {
+    const uint32_t w[4] = {in.x[i].x, in.x[i].y, in.x[i].z, in.x[i].w};
+    // Magnitudes of 16-bit floats order as their bits do, NaN on top.
+    u16x2 two = {0, 0};
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      two = __builtin_elementwise_max(two, __builtin_bit_cast(u16x2, w[d] & 0x7fff7fffu));
+    uint32_t top = vector_max<LPV>(max((uint32_t)two[0], (uint32_t)two[1]));
+    float s = E::load(__builtin_bit_cast(T16, (uint16_t)top));
+    if (s < kMinScale) {
+      s = 0.f;
+      top = 0;
     }
+    const float inv = s > 0.f ? 1.f / s : 0.f;
+    float y[8];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      // Magnitudes of 16-bit floats order as their bits do, NaN on top.
-      uint32_t top = 0;
+    for (int d = 0; d < 8; ++d) {
+      const uint16_t bits = (uint16_t)(w[d / 2] >> (16 * (d & 1)));
+      y[d] = E::load(__builtin_bit_cast(T16, bits)) * inv;
+    }
+    uint32_t word = 0;
+    if constexpr (PLAIN) {
+      float best[8];
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-        top = max(top, max(w[d] & 0x7fffu, (w[d] >> 16) & 0x7fffu));
-#pragma unroll
-      for (int off = 1; off < LPV; off <<= 1)
-        top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-      float s = E::load(__builtin_bit_cast(T16, (uint16_t)top));
-      if (s < kMinScale) {
-        s = 0.f;
-        top = 0;
-      }
-      const float inv = s > 0.f ? 1.f / s : 0.f;
-      float y[8];
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const uint16_t bits = (uint16_t)(w[d / 2] >> (16 * (d & 1)));
-        y[d] = E::load(__builtin_bit_cast(T16, bits)) * inv;
-      }
-      uint32_t word = 0;
-      if constexpr (PLAIN) {
-        float best[8];
-#pragma unroll
-        for (int d = 0; d < 8; ++d) best[d] = fabsf(y[d] - E::load(levels[0]));
+      for (int d = 0; d < 8; ++d) best[d] = fabsf(y[d] - E::load(levels[0]));
 #pragma unroll 1
-        for (int c = 1; c < LV; ++c) {
-          const float lv = E::load(levels[c]);
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const float dist = fabsf(y[d] - lv);
-            if (dist < best[d]) {
-              best[d] = dist;
-              word = (word & ~(15u << (4 * d))) | (uint32_t)c << (4 * d);
-            }
-          }
-        }
-      } else {
+      for (int c = 1; c < LV; ++c) {
+        const float lv = E::load(levels[c]);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          const uint2 e = cells[cell_of(y[d])];
-          word |= (e.y >> (y[d] >= __uint_as_float(e.x) ? 4 : 0) & 15u) << (4 * d);
+          const float dist = fabsf(y[d] - lv);
+          if (dist < best[d]) {
+            best[d] = dist;
+            word = (word & ~(15u << (4 * d))) | (uint32_t)c << (4 * d);
+          }
         }
       }
+    } else {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        const uint2 e = *reinterpret_cast<const uint2*>(
+            reinterpret_cast<const char*>(t.at) + cell_of(y[d]));
+        // the low four bits, on top of the word shifted down by four
+        word = __builtin_amdgcn_alignbit(e.y >> (y[d] >= __uint_as_float(e.x) ? 4 : 0), word, 4);
+      }
       // An element over an infinity or a NaN that is neither 0 takes level 0.
-      if (!PLAIN && !(s < INFINITY)) {
+      if (__any(!(s < INFINITY))) {
 #pragma unroll
         for (int d = 0; d < 8; ++d)
           if (y[d] != y[d]) word &= ~(15u << (4 * d));
       }
-      if (slot[i] < num_slots) {
-        const uint32_t blk = bs.div(slot[i]);
-        const int64_t row = ((int64_t)blk * heads + h) * bs.d + (slot[i] - blk * bs.d);
-        codes[row * LPV + sub] = word;
-        if (sub == 0) scales[row] = (uint16_t)top;
-      }
+    }
+    if (in.slot[i] < num_slots) {
+      const uint32_t blk = bs.div(in.slot[i]);
+      const int64_t row = ((int64_t)blk * heads + h) * bs.d + (in.slot[i] - blk * bs.d);
+      codes[row * LPV + sub] = word;
+      if (sub == 0) scales[row] = (uint16_t)top;
     }
   }
 }
 
 template <int DT, int D>
-__global__ void __launch_bounds__(KT)
+__global__ void __launch_bounds__(KT, 8)
 kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
                   int T, int per_wg, uint32_t* __restrict__ k_codes,
                   uint32_t* __restrict__ v_codes, uint16_t* __restrict__ k_scales,
@@ -226,24 +266,31 @@ kv4_append_kernel(Kv4Rows kr, Kv4Rows vr, const int32_t* __restrict__ slots,
                   const uint16_t* __restrict__ v_levels, int heads, FastDiv bs,
                   uint32_t num_slots) {
   using T16 = typename Elem<DT>::T;
+  constexpr int NB = 2;
+  using B = Batch<D, NB>;
+  __shared__ Cells t;
   const int h = blockIdx.y;
   const bool isv = blockIdx.z != 0;
   const Kv4Rows src = isv ? vr : kr;
   const T16* levels = reinterpret_cast<const T16*>(isv ? v_levels : k_levels) + h * LV;
-  __shared__ uint2 cells[CELLS];
-  const bool table = fill_cells<DT>(levels, cells);
-  const uint16_t* base = static_cast<const uint16_t*>(src.p) + (int64_t)h * src.head_stride +
-                         threadIdx.x % (D / 8) * 8;
-  const int t0 = blockIdx.x * per_wg;
-  const int t1 = min(T, t0 + per_wg);
   uint32_t* codes = isv ? v_codes : k_codes;
   uint16_t* scales = isv ? v_scales : k_scales;
-  if (table)
-    store_rows<DT, D, 4, false>(cells, levels, base, src.token_stride, slots, t0, t1, codes,
-                                scales, heads, h, bs, num_slots);
-  else
-    store_rows<DT, D, 1, true>(cells, levels, base, src.token_stride, slots, t0, t1, codes,
-                               scales, heads, h, bs, num_slots);
+  const uint16_t* base = static_cast<const uint16_t*>(src.p) + (int64_t)h * src.head_stride +
+                         threadIdx.x % B::LPV * 8;
+  const int t0 = blockIdx.x * per_wg;
+  const int t1 = min(T, t0 + per_wg);
+  // Rows are on their way while the table is made.
+  B cur, nxt;
+  cur.load(base, src.token_stride, slots, t0, t1, num_slots);
+  const bool table = fill_cells<DT>(levels, t);
+  for (int tb = t0; tb < t1; tb += NB * B::VP) {
+    nxt.load(base, src.token_stride, slots, tb + NB * B::VP, t1, num_slots);
+    if (table)
+      store_batch<DT, D, false>(cur, t, levels, codes, scales, heads, h, bs, num_slots);
+    else
+      store_batch<DT, D, true>(cur, t, levels, codes, scales, heads, h, bs, num_slots);
+    cur = nxt;
+  }
 }
 
 // The reverse: eight elements per lane, levels in LDS once per bank so that
@@ -305,12 +352,12 @@ kv4_read_kernel(const int32_t* __restrict__ slots, int T, int per_wg,
   }
 }
 
-// Tokens per workgroup: about eight workgroups per CU over all heads, keys
-// and values, in whole passes.
+// Tokens per workgroup: about four workgroups (all that fit) per CU over all
+// heads, keys and values, in whole passes.
 int tokens_per_wg(int64_t T, int64_t heads, int D) {
   const int64_t vp = KT / (D / 8);
   const int64_t passes = (T + vp - 1) / vp * heads * 2;
-  const int64_t want = 8 * (int64_t)device_shape().cus;
+  const int64_t want = 4 * (int64_t)device_shape().cus;
   return (int)(vp * std::max<int64_t>(1, (passes + want - 1) / want));
 }
 
