@@ -207,9 +207,13 @@ __device__ inline void load_codes(const Args& a, const int (&base)[2], int n, in
 }
 
 // Entry of byte b of w in the table: `off` is the lane's offset in an entry.
-__device__ inline uint32_t lookup(const char* lds, uint32_t w, int b, uint32_t off) {
-  const uint32_t at = __builtin_amdgcn_perm(w, off, 0x0c0c0000u | (uint32_t)(4 + b) << 8);
-  return *reinterpret_cast<const uint32_t*>(lds + at);
+// The table is the start of the workgroup's LDS (its kernels have dynamic LDS
+// only), so the v_perm is the whole address; through the pointer to the table
+// every look-up would cost an addition of that 0.
+__device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
+  typedef const uint32_t __attribute__((address_space(3))) * LdsPtr;
+  return *(LdsPtr)(uintptr_t)__builtin_amdgcn_perm(w, off,
+                                                   0x0c0c0000u | (uint32_t)(4 + b) << 8);
 }
 
 // The split form: the WAVES waves of a workgroup share NT tiles of 16 columns
@@ -227,9 +231,11 @@ kv4_split_kernel(const Args a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  int idx = blockIdx.x;
-  const int c = idx % a.chunks;
-  idx /= a.chunks;
+  // Heads first, chunks last: consecutive workgroups go to the eight XCDs in
+  // turn, and every head has as much to do as the next, while later chunks
+  // are those of the longest requests only.
+  const int items = gridDim.x / a.chunks;
+  const int c = blockIdx.x / items, idx = blockIdx.x - c * items;
   const int hc = idx % a.heads;
   Tile t;
   if (!find_tile<COLS>(a, idx / a.heads, t)) return;
@@ -311,7 +317,7 @@ kv4_split_kernel(const Args a) {
       for (int k = 0; k < KS; ++k) {
         u32x4 kf;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) kf[b] = lookup(lds, cur.k[j][k], b, koff);
+        for (int b = 0; b < 4; ++b) kf[b] = lookup(cur.k[j][k], b, koff);
 #pragma unroll
         for (int x = 0; x < NT; ++x)
           s[x][j] = mfma<DT>(kf, qf[x][k], k ? s[x][j] : f32x4{0.f, 0.f, 0.f, 0.f});
@@ -396,7 +402,7 @@ kv4_split_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[j][i] = lookup(lds, cur.v[j][i][b / 4], b % 4, voff);
+        for (int i = 0; i < 4; ++i) e[j][i] = lookup(cur.v[j][i][b / 4], b % 4, voff);
       u32x4 lo, hi;  // features 2 b and 2 b + 1 of the lane's row, by token
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
