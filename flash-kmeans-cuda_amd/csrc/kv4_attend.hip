@@ -69,6 +69,10 @@ constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
                                            // a difference of two is no NaN
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
+constexpr int kJoin = 8 / 2 * 32 * 4;      // maxima and sums of half the waves
+
+// Read by scalar loads: nothing writes it while the kernel runs.
+typedef const int32_t __attribute__((address_space(4))) * Const32;
 
 struct Args {
   const uint16_t* q;
@@ -85,12 +89,14 @@ struct Args {
   const int32_t* cu_q;
   uint16_t* out;
   float* lse;
-  float* part;     // (T, H, chunks, D) unnormalised outputs
-  float* part_ml;  // (T, H, chunks, 2) maximum (base 2), sum
+  float* part;     // two partial results of COLS columns per workgroup:
+  float* part_ml;  // unnormalised outputs; maximum (base 2) and sum
+  int4* desc;      // per workgroup: what is to be joined from it on
   FastDiv bs, gdiv;
   uint32_t num_blocks;
   int heads, H, G, T, R, max_seq, causal;
-  int chunk, chunks;  // tokens per workgroup, workgroups along the context
+  int whole;          // one item per workgroup, else equal shares
+  int min_share;      // units a share has at least
   int tiles_per_req;  // without cu_q
   float zscale;       // sm_scale * log2(e)
 };
@@ -146,12 +152,12 @@ __device__ inline int sees(const Args& a, const Tile& t, int i) {
 
 // Tables of a head's level pairs, by the whole workgroup.
 template <int THREADS>
-__device__ inline void fill_table(const Args& a, int hc, char* lds) {
+__device__ inline void fill_table(const Args& a, int hc, char* lds, int tid) {
   const uint16_t* kl = a.k_levels + hc * 16;
   const uint16_t* vl = a.v_levels + hc * 16;
 #pragma unroll
   for (int r = 0; r < kTable / 16 / THREADS; ++r) {
-    const int i = r * THREADS + threadIdx.x;
+    const int i = r * THREADS + tid;
     const int e = i / (kEntry / 16);
     const uint16_t* lv = (i & 8) ? vl : kl;
     const uint32_t w = lv[e & 15] | (uint32_t)lv[e >> 4] << 16;
@@ -216,345 +222,473 @@ __device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
                                                    0x0c0c0000u | (uint32_t)(4 + b) << 8);
 }
 
+// Work of a launch, counted in units of UNIT tokens (one turn of all waves).
+// An item is a tile of a request under one cache head; each of a request's
+// tiles counts ceil(tokens / UNIT) units, at least one.  The items in order
+// (head, request, tile) are cut into equal shares, one per workgroup, wherever
+// the cuts fall: lengths of any mixture fill the chip evenly, a workgroup
+// meets few heads (whose tables it has to fill), and an item that is cut is
+// joined afterwards.
+struct Item {
+  int hc;
+  Tile t;
+  int n;     // units
+  int unit;  // first unit of the share in it
+};
+
+template <int COLS>
+__device__ inline void request(const Args& a, int r, Tile& t, int& n, int& tiles) {
+  t.req = r;
+  if (a.cu_q == nullptr) {
+    t.row0 = r;
+    t.nq = r < a.R ? 1 : 0;
+  } else {
+    t.row0 = min(max(a.cu_q[min(r, a.R)], 0), a.T);
+    const int next = r < a.R ? min(max(a.cu_q[r + 1], 0), a.T) : a.T;
+    t.nq = r <= a.R ? max(next - t.row0, 0) : 0;
+  }
+  t.end = tokens_of(a, r);
+  tiles = (int)(((int64_t)t.nq * a.G + COLS - 1) / COLS);
+}
+
+// Running sums of the requests' units, THREADS slices of `per` requests.
+template <int COLS, int THREADS, int UNIT>
+struct Shares {
+  int* s_pre;  // LDS, THREADS + THREADS / 64
+  int per, total;
+  __device__ inline int units(const Args& a, int r) const {
+    Tile t;
+    int n, tiles;
+    request<COLS>(a, r, t, n, tiles);
+    return tiles * max((t.end + UNIT - 1) / UNIT, 1);
+  }
+  __device__ inline Shares(int* lds, int p, int n) : s_pre(lds), per(p), total(n) {}
+  __device__ inline Shares(const Args& a, int* lds) : s_pre(lds) {
+    const int rt = a.R + (a.cu_q != nullptr ? 1 : 0);
+    per = (rt + THREADS - 1) / THREADS;
+    int sum = 0;
+    for (int i = 0; i < per; ++i) {
+      const int r = threadIdx.x * per + i;
+      if (r < rt) sum += units(a, r);
+    }
+    const int incl = wave_incl_scan(sum);
+    int* s_wave = s_pre + THREADS;
+    if ((threadIdx.x & 63) == 63) s_wave[threadIdx.x >> 6] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      before += w < (int)(threadIdx.x >> 6) ? s_wave[w] : 0;
+      total += s_wave[w];
+    }
+    s_pre[threadIdx.x] = before + incl - sum;
+    __syncthreads();
+    total = __builtin_amdgcn_readfirstlane(total);
+  }
+  // The item that unit u (below total) of a head's falls into.
+  __device__ inline Item find(const Args& a, int hc, int u) const {
+    int j = -1;
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i)
+      j += __builtin_popcountll(__ballot(s_pre[i * 64 + (threadIdx.x & 63)] <= u));
+    u -= __builtin_amdgcn_readfirstlane(s_pre[j]);
+    Item x;
+    x.hc = hc;
+    int r = j * per, tiles = 0;
+    for (;; ++r) {
+      request<COLS>(a, r, x.t, x.n, tiles);
+      x.n = max((x.t.end + UNIT - 1) / UNIT, 1);
+      if (u < tiles * x.n || r >= a.R) break;
+      u -= tiles * x.n;
+    }
+    const int tile = u / x.n;
+    x.unit = u - tile * x.n;
+    x.t.col0 = tile * COLS;
+    return x;
+  }
+};
+
 // The split form: the WAVES waves of a workgroup share NT tiles of 16 columns
-// and take 32 tokens of its chunk in turn, each with its own running maximum
-// and sum; they are joined in LDS at the end, chunks by a second kernel.
+// and take 32 tokens in turn, each with its own running maximum and sum; they
+// are joined in LDS at the end of an item, cut items by a second kernel.
 template <int DT, int D, int NT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, WAVES * (NT * D > 256 ? 1 : 2) / 4)
 kv4_split_kernel(const Args a) {
-  constexpr int COLS = 16 * NT;
+  constexpr int COLS = 16 * NT, THREADS = WAVES * 64, UNIT = WAVES * 32;
   constexpr int KS = D / 32;  // steps of the first product
   constexpr int ND = D / 16;  // feature tiles of the second
   extern __shared__ __align__(16) char lds[];
-  int* s_base = reinterpret_cast<int*>(lds + kTable);
+  float* sml = reinterpret_cast<float*>(lds + kTable);
+  int* s_pre = reinterpret_cast<int*>(lds + kTable + kJoin);
 
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15, g = lane >> 4;
-  // Heads first, chunks last: consecutive workgroups go to the eight XCDs in
-  // turn, and every head has as much to do as the next, while later chunks
-  // are those of the longest requests only.
-  const int items = gridDim.x / a.chunks;
-  const int c = blockIdx.x / items, idx = blockIdx.x - c * items;
-  const int hc = idx % a.heads;
-  Tile t;
-  if (!find_tile<COLS>(a, idx / a.heads, t)) return;
-  const int ncols = t.nq * a.G;
-  const int last = min(t.col0 + COLS, ncols) - 1;
-  const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0));
-  const int lim_max = sees(a, t, (int)a.gdiv.div(last));
-  const int t0 = c * a.chunk;
-  if (t0 >= lim_max && c != 0) return;
-  const int t1 = min(t0 + a.chunk, lim_max);
-
-  // 16-token groups of the chunk: their place in the cache, -1 where there
-  // is no block.
-  for (int i = threadIdx.x; i < (t1 - t0 + 31) / 32 * 2; i += WAVES * 64) {
-    const int tok = t0 + i * 16;
-    int base = -1;
-    if (tok < t1) {
-      const uint32_t b = a.bs.div(tok);
-      const uint32_t blk = (uint32_t)a.tables[(int64_t)t.req * a.table_stride + b];
-      if (blk < a.num_blocks)
-        base = (int)((blk * (uint32_t)a.heads + hc) * (a.bs.d / 16) + (tok - b * a.bs.d) / 16);
+  int64_t u = blockIdx.x, u_end = u + 1;  // of all heads' units
+  int64_t share = 1;
+  int per_head = 1, table = -1;  // units of a head; head whose table is in LDS
+  if (!a.whole) {
+    const Shares<COLS, THREADS, UNIT> sh(a, s_pre);
+    per_head = sh.total;
+    const int64_t all = (int64_t)per_head * a.heads;
+    share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)a.min_share);
+    u = blockIdx.x * share;
+    u_end = min(u + share, all);
+    if (threadIdx.x == 0) a.desc[blockIdx.x].x = 0;
+  }
+  for (; u < u_end;) {
+    // Opaque, so that what derives from it is computed per item, not kept in
+    // registers over the whole share.
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const uint32_t koff = (uint32_t)(lane & 31) * 4, voff = koff + 128;
+    Item x;
+    int ub;
+    if (a.whole) {
+      // Heads first: consecutive workgroups go to the eight XCDs in turn, and
+      // every head has as much to do as the next.
+      const int tile = blockIdx.x / a.heads;
+      x.hc = blockIdx.x - tile * a.heads;
+      if (!find_tile<COLS>(a, tile, x.t)) return;
+      x.unit = 0;
+      x.n = ub = max((x.t.end + UNIT - 1) / UNIT, 1);
+      u = u_end;
+    } else {
+      Shares<COLS, THREADS, UNIT> sh(s_pre, (a.R + (a.cu_q != nullptr) + THREADS - 1) / THREADS,
+                                     per_head);
+      const int hc = (int)(u / per_head);
+      x = sh.find(a, hc, (int)(u - (int64_t)hc * per_head));
+      ub = (int)min((int64_t)x.n, x.unit + (u_end - u));
+      u += ub - x.unit;
     }
-    s_base[i] = base;
-  }
-  fill_table<WAVES * 64>(a, hc, lds);
+    // The same in every lane, which the compiler cannot see of loaded values.
+    auto scalar = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
+    Tile& t = x.t;
+    scalar(t.req), scalar(t.row0), scalar(t.nq), scalar(t.col0), scalar(t.end);
+    scalar(x.hc), scalar(x.n), scalar(x.unit), scalar(ub);
+    const int ncols = t.nq * a.G;
+    const int last = min(t.col0 + COLS, ncols) - 1;
+    const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0));
+    const int lim_max = sees(a, t, (int)a.gdiv.div(last));
+    const int t0 = x.unit * UNIT;
+    const int t1 = min(ub * UNIT, lim_max);
+    const int ntile = max(t1 - t0 + 31, 0) / 32;
+    const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
 
-  int lim[NT], row[NT], head[NT];
-  u32x4 qf[NT][KS];
+    // Cache blocks of a tile's two halves, and from them their 16-slot group
+    // over all heads: -1 where there is no block.
+    auto load_blocks = [&](int it, int (&blk)[2]) {
 #pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    const int col = t.col0 + 16 * x + n;
-    const bool ok = col < ncols;
-    const int i = (int)a.gdiv.div(ok ? col : 0);
-    row[x] = t.row0 + i;
-    head[x] = hc * a.G + (ok ? col - i * a.G : 0);
-    lim[x] = ok ? sees(a, t, i) : 0;
-    const uint16_t* qp = a.q + row[x] * a.q_ts + head[x] * a.q_hs + g * (D / 4);
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-      qf[x][s] = ok ? *reinterpret_cast<const u32x4*>(qp + s * 8) : u32x4{0, 0, 0, 0};
-    if (!ok) row[x] = -1;
-  }
-  __syncthreads();
-
-  float m[NT], l[NT];
-  f32x4 o[NT][ND];
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    m[x] = kLowest;
-    l[x] = 0.f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) o[x][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  // fp16 weights are kept within the type's range whatever the scales are:
-  // times 2^14 over a power of two that no scale so far exceeds.
-  float vref = 0.f, vmul = 1.f;
-  const uint32_t koff = (uint32_t)(lane & 31) * 4, voff = koff + 128;
-  const int ntile = (t1 - t0 + 31) / 32;
-
-  auto bases = [&](int it, int (&base)[2]) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      base[j] = __builtin_amdgcn_readfirstlane(s_base[min(it, ntile - 1) * 2 + j]);
-  };
-  int base[2], nbase[2];
-  Codes<D> cur, nxt;
-  if (wave < ntile) {
-    bases(wave, base);
-    load_codes<D>(a, base, n, g, cur);
-  }
-  for (int it = wave; it < ntile; it += WAVES) {
-    bases(it + WAVES, nbase);
-    load_codes<D>(a, nbase, n, g, nxt);
-
-    f32x4 s[NT][2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        u32x4 kf;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) kf[b] = lookup(cur.k[j][k], b, koff);
-#pragma unroll
-        for (int x = 0; x < NT; ++x)
-          s[x][j] = mfma<DT>(kf, qf[x][k], k ? s[x][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int j = 0; j < 2; ++j) {
+        const int tok = t0 + it * 32 + 16 * j;
+        blk[j] = tok < t1 ? blocks[a.bs.div(tok)] : -1;
       }
-    const int tok = t0 + it * 32 + 4 * g;  // token (j, i): tok + 16 j + i
-    const bool masked = t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0;
-    float ks[2][4], vs[2][4];
+    };
+    auto groups = [&](int it, const int (&blk)[2], int (&base)[2]) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t kw = i < 2 ? cur.ks[j].x : cur.ks[j].y;
-        const uint32_t vw = i < 2 ? cur.vs[j].x : cur.vs[j].y;
-        ks[j][i] = from16<DT>((i & 1) ? kw >> 16 : kw & 0xffffu) * a.zscale;
-        vs[j][i] = from16<DT>((i & 1) ? vw >> 16 : vw & 0xffffu);
-        // What lies past the requests' tokens is anything.
-        if (masked && (base[j] < 0 || tok + 16 * j + i >= lim_max)) vs[j][i] = 0.f;
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t b = (uint32_t)blk[j];
+        const uint32_t tok = t0 + it * 32 + 16 * j;
+        const uint32_t in = (tok - a.bs.div(tok) * a.bs.d) / 16;
+        base[j] = b < a.num_blocks ? (int)((b * (uint32_t)a.heads + x.hc) * (a.bs.d / 16) + in)
+                                   : -1;
       }
-    if constexpr (DT == FKC_F16) {
-      float top = 0.f;
+    };
+    int blk[2], base[2], nbase[2];
+    load_blocks(wave, blk);
+
+    int lim[NT], row[NT], head[NT];
+    u32x4 qf[NT][KS];
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      const int col = t.col0 + 16 * y + n;
+      const bool ok = col < ncols;
+      const int i = (int)a.gdiv.div(ok ? col : 0);
+      row[y] = t.row0 + i;
+      head[y] = x.hc * a.G + (ok ? col - i * a.G : 0);
+      lim[y] = ok ? sees(a, t, i) : 0;
+      const uint16_t* qp = a.q + row[y] * a.q_ts + head[y] * a.q_hs + g * (D / 4);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        qf[y][s] = ok ? *reinterpret_cast<const u32x4*>(qp + s * 8) : u32x4{0, 0, 0, 0};
+      if (!ok) row[y] = -1;
+    }
+    Codes<D> cur, nxt;
+    groups(wave, blk, base);
+    if (a.num_blocks != 0) load_codes<D>(a, base, n, g, cur);
+    load_blocks(wave + WAVES, blk);
+    if (table != x.hc) {
+      table = x.hc;
+      fill_table<THREADS>(a, x.hc, lds, tid);
+    }
+    __syncthreads();
+
+    float m[NT], l[NT];
+    f32x4 o[NT][ND];
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      m[y] = kLowest;
+      l[y] = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[y][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // fp16 weights are kept within the type's range whatever the scales are:
+    // times 2^14 over a power of two that no scale so far exceeds.
+    float vref = 0.f, vmul = 1.f;
+
+    for (int it = wave; it < ntile; it += WAVES) {
+      groups(it + WAVES, blk, nbase);
+      load_codes<D>(a, nbase, n, g, nxt);
+      load_blocks(it + 2 * WAVES, blk);
+
+      f32x4 s[NT][2];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(vs[j][i]) < INFINITY ? fabsf(vs[j][i]) : 0.f);
-      if (__any(top > vref)) {
+        for (int k = 0; k < KS; ++k) {
+          u32x4 kf;
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        // next power of two: times 2^14 over it stays in range
-        const float ref = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
-        const float mul = 16384.f / ref;
-        const float f = vref > 0.f ? mul / vmul : 0.f;  // nothing yet: o is 0
-        vref = ref;
-        vmul = mul;
+          for (int b = 0; b < 4; ++b) kf[b] = lookup(cur.k[j][k], b, koff);
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[x][d] *= f;
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vs[j][i] *= vmul;
-    }
-    u32x4 pf[NT];
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      float z[2][4], top = kLowest;
+          for (int y = 0; y < NT; ++y)
+            s[y][j] = mfma<DT>(kf, qf[y][k], k ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+        }
+      const int tok = t0 + it * 32 + 4 * g;  // token (j, i): tok + 16 j + i
+      const bool masked = t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0;
+      float ks[2][4], vs[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          z[j][i] = s[x][j][i] * ks[j][i];
-          if (masked && (base[j] < 0 || tok + 16 * j + i >= lim[x])) z[j][i] = -INFINITY;
-          top = fmaxf(top, z[j][i]);
+          const uint32_t kw = i < 2 ? cur.ks[j].x : cur.ks[j].y;
+          const uint32_t vw = i < 2 ? cur.vs[j].x : cur.vs[j].y;
+          ks[j][i] = from16<DT>((i & 1) ? kw >> 16 : kw & 0xffffu) * a.zscale;
+          vs[j][i] = from16<DT>((i & 1) ? vw >> 16 : vw & 0xffffu);
+          // What lies past the requests' tokens is anything.
+          if (masked && (base[j] < 0 || tok + 16 * j + i >= lim_max)) vs[j][i] = 0.f;
         }
-      if (__any(top > m[x])) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float nm = fmaxf(m[x], top);
-        const float f = __builtin_amdgcn_exp2f(m[x] - nm);
-        m[x] = nm;
-        l[x] *= f;
+      if constexpr (DT == FKC_F16) {
+        float top = 0.f;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[x][d] *= f;
-      }
-      float w[2][4];
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+          for (int i = 0; i < 4; ++i)
+            top = fmaxf(top, fabsf(vs[j][i]) < INFINITY ? fabsf(vs[j][i]) : 0.f);
+        if (__any(top > vref)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(z[j][i] - m[x]);
-          l[x] += p;
-          w[j][i] = masked && z[j][i] == -INFINITY ? 0.f : p * vs[j][i];
+          for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+          // next power of two: times 2^14 over it stays in range
+          const float ref = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
+          const float mul = 16384.f / ref;
+          const float f = vref > 0.f ? mul / vmul : 0.f;  // nothing yet: o is 0
+          vref = ref;
+          vmul = mul;
+#pragma unroll
+          for (int y = 0; y < NT; ++y)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) o[y][d] *= f;
         }
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        pf[x][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
-    }
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-    for (int b = 0; b < ND / 2; ++b) {
-      uint32_t e[2][4];
+          for (int i = 0; i < 4; ++i) vs[j][i] *= vmul;
+      }
+      u32x4 pf[NT];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int y = 0; y < NT; ++y) {
+        float z[2][4], top = kLowest;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[j][i] = lookup(cur.v[j][i][b / 4], b % 4, voff);
-      u32x4 lo, hi;  // features 2 b and 2 b + 1 of the lane's row, by token
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t x0 = e[k >> 1][2 * (k & 1)], x1 = e[k >> 1][2 * (k & 1) + 1];
-        lo[k] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
-        hi[k] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+          for (int i = 0; i < 4; ++i) {
+            z[j][i] = s[y][j][i] * ks[j][i];
+            if (masked && (base[j] < 0 || tok + 16 * j + i >= lim[y])) z[j][i] = -INFINITY;
+            top = fmaxf(top, z[j][i]);
+          }
+        if (__any(top > m[y])) {
+          top = fmaxf(top, __shfl_xor(top, 16, 64));
+          top = fmaxf(top, __shfl_xor(top, 32, 64));
+          const float nm = fmaxf(m[y], top);
+          const float f = __builtin_amdgcn_exp2f(m[y] - nm);
+          m[y] = nm;
+          l[y] *= f;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[y][d] *= f;
+        }
+        float w[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = __builtin_amdgcn_exp2f(z[j][i] - m[y]);
+            l[y] += p;
+            w[j][i] = masked && z[j][i] == -INFINITY ? 0.f : p * vs[j][i];
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          pf[y][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
       }
 #pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        o[x][2 * b] = mfma<DT>(lo, pf[x], o[x][2 * b]);
-        o[x][2 * b + 1] = mfma<DT>(hi, pf[x], o[x][2 * b + 1]);
+      for (int b = 0; b < ND / 2; ++b) {
+        uint32_t e[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) e[j][i] = lookup(cur.v[j][i][b / 4], b % 4, voff);
+        u32x4 lo, hi;  // features 2 b and 2 b + 1 of the lane's row, by token
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t x0 = e[k >> 1][2 * (k & 1)], x1 = e[k >> 1][2 * (k & 1) + 1];
+          lo[k] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
+          hi[k] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
+        }
+#pragma unroll
+        for (int y = 0; y < NT; ++y) {
+          o[y][2 * b] = mfma<DT>(lo, pf[y], o[y][2 * b]);
+          o[y][2 * b + 1] = mfma<DT>(hi, pf[y], o[y][2 * b + 1]);
+        }
       }
+      cur = nxt;
+      base[0] = nbase[0];
+      base[1] = nbase[1];
     }
-    cur = nxt;
-    base[0] = nbase[0];
-    base[1] = nbase[1];
-  }
 
-  // Join the lanes of a column (they share m), then the waves, half of them
-  // at a time, the later one into the earlier.
+    // Join the lanes of a column (they share m), then the waves that had
+    // tokens, half of them at a time, the later one into the earlier.
 #pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    l[x] += __shfl_xor(l[x], 16, 64);
-    l[x] += __shfl_xor(l[x], 32, 64);
-    if constexpr (DT == FKC_F16)
+    for (int y = 0; y < NT; ++y) {
+      l[y] += __shfl_xor(l[y], 16, 64);
+      l[y] += __shfl_xor(l[y], 32, 64);
+      if constexpr (DT == FKC_F16)
 #pragma unroll
-      for (int d = 0; d < ND; ++d) o[x][d] *= 1.f / vmul;
-  }
+        for (int d = 0; d < ND; ++d) o[y][d] *= 1.f / vmul;
+    }
+    if (ntile > 1) table = -1;  // the table's place is used
 #pragma unroll
-  for (int half = WAVES / 2; half > 0; half /= 2) {
+    for (int half = WAVES / 2; half > 0; half /= 2) {
+      if (ntile <= half) continue;
 #pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      f32x4* so = reinterpret_cast<f32x4*>(lds);
-      float* sml = reinterpret_cast<float*>(lds + kTable);
-      __syncthreads();
-      if (wave >= half && wave < 2 * half) {
+      for (int y = 0; y < NT; ++y) {
+        f32x4* so = reinterpret_cast<f32x4*>(lds);
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) so[((wave - half) * ND + d) * 64 + lane] = o[x][d];
-        if (g == 0) {
-          sml[(wave - half) * 32 + n] = m[x];
-          sml[(wave - half) * 32 + 16 + n] = l[x];
+          for (int d = 0; d < ND; ++d) so[((wave - half) * ND + d) * 64 + lane] = o[y][d];
+          if (g == 0) {
+            sml[(wave - half) * 32 + n] = m[y];
+            sml[(wave - half) * 32 + 16 + n] = l[y];
+          }
+        }
+        __syncthreads();
+        if (wave < half) {
+          const float m2 = sml[wave * 32 + n], l2 = sml[wave * 32 + 16 + n];
+          const float nm = fmaxf(m[y], m2);
+          const float f1 = __builtin_amdgcn_exp2f(m[y] - nm);
+          const float f2 = __builtin_amdgcn_exp2f(m2 - nm);
+          m[y] = nm;
+          l[y] = l[y] * f1 + l2 * f2;
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+            o[y][d] = o[y][d] * f1 + so[(wave * ND + d) * 64 + lane] * f2;
         }
       }
-      __syncthreads();
-      if (wave < half) {
-        const float m2 = sml[wave * 32 + n], l2 = sml[wave * 32 + 16 + n];
-        const float nm = fmaxf(m[x], m2);
-        const float f1 = __builtin_amdgcn_exp2f(m[x] - nm);
-        const float f2 = __builtin_amdgcn_exp2f(m2 - nm);
-        m[x] = nm;
-        l[x] = l[x] * f1 + l2 * f2;
+    }
+    const bool cut = x.unit > 0 || ub < x.n;
+    if (wave == 0) {
+      // A share cuts the item before it and the one after it at most.
+      const int64_t slot = (int64_t)blockIdx.x * 2 + (x.unit > 0 ? 0 : 1);
 #pragma unroll
-        for (int d = 0; d < ND; ++d) o[x][d] = o[x][d] * f1 + so[(wave * ND + d) * 64 + lane] * f2;
+      for (int y = 0; y < NT; ++y) {
+        if (row[y] < 0) continue;
+        const int64_t at = (int64_t)row[y] * a.H + head[y];
+        if (!cut) {
+          const float f = l[y] > 0.f ? 1.f / l[y] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[ND / 2];
+#pragma unroll
+            for (int d = 0; d < ND / 2; ++d)
+              w[d] = pack2<DT>(o[y][2 * d][i] * f, o[y][2 * d + 1][i] * f);
+            uint32_t* op = reinterpret_cast<uint32_t*>(a.out + at * D + (4 * g + i) * ND);
+#pragma unroll
+            for (int d = 0; d < ND / 2; ++d) op[d] = w[d];
+          }
+          if (g == 0 && a.lse != nullptr)
+            a.lse[at] = l[y] > 0.f ? m[y] * kLn2 + __logf(l[y]) : -INFINITY;
+        } else {
+          float* op = a.part + (slot * COLS + 16 * y + n) * D;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < ND; ++d) op[(4 * g + i) * ND + d] = o[y][d][i];
+          if (g == 0) {
+            a.part_ml[(slot * COLS + 16 * y + n) * 2] = m[y];
+            a.part_ml[(slot * COLS + 16 * y + n) * 2 + 1] = l[y];
+          }
+        }
+      }
+      if (cut && x.unit == 0 && lane == 0) {
+        // u is the share's end: the item's other units are the next ones'.
+        const int more = (int)((x.n - ub + share - 1) / share);
+        a.desc[blockIdx.x] = int4{more + 1, t.row0, t.col0, (last - t.col0 + 1) << 16 | x.hc};
       }
     }
-  }
-  if (wave != 0) return;
-#pragma unroll
-  for (int x = 0; x < NT; ++x) {
-    if (row[x] < 0) continue;
-    const int64_t at = (int64_t)row[x] * a.H + head[x];
-    if (lim[x] <= a.chunk) {  // all of the row is here
-      if (c != 0) continue;
-      const float f = l[x] > 0.f ? 1.f / l[x] : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[ND / 2];
-#pragma unroll
-        for (int d = 0; d < ND / 2; ++d)
-          w[d] = pack2<DT>(o[x][2 * d][i] * f, o[x][2 * d + 1][i] * f);
-        uint32_t* op = reinterpret_cast<uint32_t*>(a.out + at * D + (4 * g + i) * ND);
-#pragma unroll
-        for (int d = 0; d < ND / 2; ++d) op[d] = w[d];
-      }
-      if (g == 0 && a.lse != nullptr)
-        a.lse[at] = l[x] > 0.f ? m[x] * kLn2 + __logf(l[x]) : -INFINITY;
-    } else if (t0 < lim[x]) {
-      float* op = a.part + (at * a.chunks + c) * D;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) op[(4 * g + i) * ND + d] = o[x][d][i];
-      if (g == 0) {
-        a.part_ml[(at * a.chunks + c) * 2] = m[x];
-        a.part_ml[(at * a.chunks + c) * 2 + 1] = l[x];
-      }
-    }
+    if (u < u_end) __syncthreads();  // the next item fills the table again
   }
 }
 
-// Joins the chunks of a row that needed more than one: a workgroup per query
-// and head, D / 4 lanes per chunk.
-template <int DT, int D>
+// Joins the parts of a cut item: the workgroup's that its first unit was in
+// (its second slot) and the following ones' (their first).  A workgroup per
+// four columns, D / 4 lanes per part.
+template <int DT, int D, int COLS>
 __global__ void __launch_bounds__(256)
 kv4_join_kernel(const Args a) {
   constexpr int LPC = D / 4, CP = 256 / LPC;
   __shared__ f32x4 so[256];
   __shared__ float sm[CP], sl[CP];
-  const int64_t at = (int64_t)blockIdx.x * a.H + blockIdx.y;
-  const int row = blockIdx.x;
-  Tile t{row, 1, 0, 0, row};
-  if (a.cu_q != nullptr) {
-    int lo = 0, len = a.R + 1;
-    while (len > 1) {
-      const int half = len >> 1;
-      if (a.cu_q[lo + half] <= row) lo += half;
-      len -= half;
-    }
-    if (lo >= a.R) return;
-    t.req = lo;
-    t.row0 = a.cu_q[lo];
-    t.nq = a.cu_q[lo + 1] - t.row0;
-  }
-  t.end = tokens_of(a, t.req);
-  const int lim = sees(a, t, row - t.row0);
-  if (lim <= a.chunk) return;
-  const int nc = (lim + a.chunk - 1) / a.chunk;
+  const int4 item = a.desc[blockIdx.x];
+  const int ncols = item.w >> 16, hc = item.w & 0xffff;
   const int sub = threadIdx.x % LPC, part = threadIdx.x / LPC;
-  const float* ml = a.part_ml + at * a.chunks * 2;
-  float m = kLowest, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int c = part; c < nc; c += CP) {
-    const float m2 = ml[2 * c], l2 = ml[2 * c + 1];
-    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (at * a.chunks + c) * D + 4 * sub);
-    const float nm = fmaxf(m, m2);
-    const float f1 = __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(m2 - nm);
-    m = nm;
-    l = l * f1 + l2 * f2;
-    o = o * f1 + x * f2;
-  }
-  so[threadIdx.x] = o;
-  if (sub == 0) {
-    sm[part] = m;
-    sl[part] = l;
-  }
-  __syncthreads();
-  if (threadIdx.x >= LPC) return;
+  for (int col = blockIdx.y * 4; item.x > 0 && col < min(ncols, (int)blockIdx.y * 4 + 4); ++col) {
+    float m = kLowest, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int c = part; c < item.x; c += CP) {
+      const int64_t at = (((int64_t)blockIdx.x + c) * 2 + (c ? 0 : 1)) * COLS + col;
+      const float m2 = a.part_ml[2 * at], l2 = a.part_ml[2 * at + 1];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * sub);
+      const float nm = fmaxf(m, m2);
+      const float f1 = __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(m2 - nm);
+      m = nm;
+      l = l * f1 + l2 * f2;
+      o = o * f1 + x * f2;
+    }
+    __syncthreads();
+    so[threadIdx.x] = o;
+    if (sub == 0) {
+      sm[part] = m;
+      sl[part] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= LPC) continue;
 #pragma unroll
-  for (int c = 1; c < CP; ++c) {
-    const float nm = fmaxf(m, sm[c]);
-    const float f1 = __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(sm[c] - nm);
-    m = nm;
-    l = l * f1 + sl[c] * f2;
-    o = o * f1 + so[c * LPC + sub] * f2;
+    for (int c = 1; c < CP; ++c) {
+      const float nm = fmaxf(m, sm[c]);
+      const float f1 = __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(sm[c] - nm);
+      m = nm;
+      l = l * f1 + sl[c] * f2;
+      o = o * f1 + so[c * LPC + sub] * f2;
+    }
+    const int i = (int)a.gdiv.div(item.z + col);
+    const int64_t at =
+        (int64_t)(item.y + i) * a.H + hc * a.G + (item.z + col - i * a.G);
+    const float f = l > 0.f ? 1.f / l : 0.f;
+    uint2 w;
+    w.x = pack2<DT>(o[0] * f, o[1] * f);
+    w.y = pack2<DT>(o[2] * f, o[3] * f);
+    *reinterpret_cast<uint2*>(a.out + at * D + 4 * sub) = w;
+    if (sub == 0 && a.lse != nullptr)
+      a.lse[at] = l > 0.f ? m * kLn2 + __logf(l) : -INFINITY;
   }
-  const float f = l > 0.f ? 1.f / l : 0.f;
-  uint2 w;
-  w.x = pack2<DT>(o[0] * f, o[1] * f);
-  w.y = pack2<DT>(o[2] * f, o[3] * f);
-  *reinterpret_cast<uint2*>(a.out + at * D + 4 * sub) = w;
-  if (sub == 0 && a.lse != nullptr)
-    a.lse[at] = l > 0.f ? m * kLn2 + __logf(l) : -INFINITY;
 }
 
 template <typename F>
@@ -568,12 +702,17 @@ int by_shape(int dtype, int64_t D, F&& f) {
                           : with(std::integral_constant<int, FKC_BF16>{});
 }
 
+// Units of a share at least, times two: where no context is longer, every item
+// goes to a workgroup of its own and nothing has to be joined.
+constexpr int kMinShare = 4;
+
 struct Plan {
-  int nt;           // column tiles per workgroup
-  int chunk;        // tokens per workgroup
-  int chunks;
+  int nt;             // column tiles per workgroup
+  int waves;
+  bool whole;         // one item per workgroup
+  int64_t wgs;
   int tiles_per_req;  // without cu_q
-  int64_t tiles;      // of nt * 16 columns, over all requests (an upper bound)
+  size_t part_rows() const { return (size_t)wgs * 2 * 16 * nt; }
 };
 
 Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t max_seq,
@@ -582,33 +721,30 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
   const int64_t G = H / c.heads;
   // Column tiles: as many as an average request fills, up to two.
   p.nt = R > 0 && T * G > 16 * R ? 2 : 1;
+  p.waves = p.nt == 2 || c.D == 256 ? 4 : 8;
   const int64_t cols = 16 * p.nt;
   p.tiles_per_req = (int)((G + cols - 1) / cols);
-  p.tiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
-  // Chunks: about four workgroups for each of the two places per CU.
-  const int64_t want = 8 * (int64_t)device_shape().cus;
-  const int64_t s = std::max<int64_t>(1, want / std::max<int64_t>(1, R * c.heads));
-  int64_t chunk = (max_seq + s - 1) / s;
-  chunk = std::min<int64_t>(std::max<int64_t>(chunk, 1024), 4096);
-  p.chunk = (int)((chunk + 255) / 256 * 256);
-  p.chunks = (int)std::max<int64_t>(1, (max_seq + p.chunk - 1) / p.chunk);
+  const int64_t tiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
+  // Contexts that no share would be smaller than are not cut.
+  p.whole = max_seq <= kMinShare * 32 * p.waves;
+  p.wgs = p.whole ? tiles * c.heads : 2 * (int64_t)device_shape().cus;
   return p;
 }
 
 template <int DT, int D, int NT, int WAVES>
 int launch_split(const Args& a, const Plan& p, hipStream_t s) {
-  const int bytes = kTable + std::max(WAVES / 2 * 32 * 4, p.chunk / 16 * 4);
+  const int bytes = kTable + kJoin + (WAVES * 64 + WAVES) * 4;
   auto* kernel = &kv4_split_kernel<DT, D, NT, WAVES>;
   if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
     return fail(FKC_ERR_LAUNCH, "kv4_attend: %d bytes of LDS refused", bytes);
-  hipLaunchKernelGGL((kv4_split_kernel<DT, D, NT, WAVES>),
-                     dim3((uint32_t)(p.tiles * a.heads * p.chunks)), dim3(WAVES * 64), bytes, s,
-                     a);
+  hipLaunchKernelGGL((kv4_split_kernel<DT, D, NT, WAVES>), dim3((uint32_t)p.wgs),
+                     dim3(WAVES * 64), bytes, s, a);
   if (int rc = check_launch("kv4_attend")) return rc;
-  if (p.chunks == 1) return FKC_OK;
-  hipLaunchKernelGGL((kv4_join_kernel<DT, D>), dim3((uint32_t)a.T, (uint32_t)a.H), dim3(256), 0,
-                     s, a);
+  if (p.whole) return FKC_OK;
+  const int64_t cols = std::min<int64_t>(16 * NT, a.cu_q ? 16 * NT : a.G);
+  hipLaunchKernelGGL((kv4_join_kernel<DT, D, 16 * NT>),
+                     dim3((uint32_t)p.wgs, (uint32_t)((cols + 3) / 4)), dim3(256), 0, s, a);
   return check_launch("kv4_attend (join)");
 }
 
@@ -617,31 +753,34 @@ int launch_split(const Args& a, const Plan& p, hipStream_t s) {
 size_t kv4_attend_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R,
                                   int64_t max_seq) {
   const Plan p = make_plan(c, H, T, R, max_seq, true);
-  if (p.chunks == 1) return 0;
+  if (p.whole) return 0;
   Carve w(nullptr);
-  w.take<float>((size_t)T * H * p.chunks * c.D);
-  w.take<float>((size_t)T * H * p.chunks * 2);
+  w.take<float>(p.part_rows() * c.D);
+  w.take<float>(p.part_rows() * 2);
+  w.take<int4>((size_t)p.wgs);
   return w.used;
 }
 
 int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size_t,
                       hipStream_t s) {
   const Plan p = make_plan(c, x.H, x.T, x.R, x.max_seq, x.cu_q != nullptr);
-  if (p.tiles * c.heads > INT32_MAX / p.chunks)
-    return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times chunks");
   const int G = (int)(x.H / c.heads);
+  const int64_t units = x.max_seq / (32 * p.waves) + 1;
+  if (p.wgs > INT32_MAX || x.T * G / 16 + x.R + 1 > INT32_MAX / units)
+    return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   Args a{(const uint16_t*)x.q.p, x.q.token_stride, x.q.head_stride,
          (const uint8_t*)c.k_codes, (const uint8_t*)c.v_codes,
          (const uint16_t*)c.k_scales, (const uint16_t*)c.v_scales,
          (const uint16_t*)c.k_levels, (const uint16_t*)c.v_levels,
          x.tables, x.table_stride, x.seq, x.cu_q, (uint16_t*)x.out, x.lse, nullptr, nullptr,
-         FastDiv((uint32_t)c.block_size), FastDiv((uint32_t)G), (uint32_t)c.num_blocks,
+         nullptr, FastDiv((uint32_t)c.block_size), FastDiv((uint32_t)G), (uint32_t)c.num_blocks,
          (int)c.heads, (int)x.H, G, (int)x.T, (int)x.R, (int)x.max_seq, (int)x.causal,
-         p.chunk, p.chunks, p.tiles_per_req, x.sm_scale * kLog2e};
-  if (p.chunks > 1) {
+         (int)p.whole, kMinShare / 2, p.tiles_per_req, x.sm_scale * kLog2e};
+  if (!p.whole) {
     Carve w(ws);
-    a.part = w.take<float>((size_t)x.T * x.H * p.chunks * c.D);
-    a.part_ml = w.take<float>((size_t)x.T * x.H * p.chunks * 2);
+    a.part = w.take<float>(p.part_rows() * c.D);
+    a.part_ml = w.take<float>(p.part_rows() * 2);
+    a.desc = w.take<int4>((size_t)p.wgs);
   }
   return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     constexpr int DT = dt.value, DD = d.value;
