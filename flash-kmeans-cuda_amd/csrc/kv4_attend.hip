@@ -21,6 +21,7 @@
 // The products are then of levels, exact in 16 bits.  A token's scales stay
 // outside: the key's multiplies the score, the value's the weight.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "device_util.hpp"
@@ -98,7 +99,8 @@ struct Args {
   int whole;          // one item per workgroup, else equal shares
   int min_share;      // units a share has at least
   int tiles_per_req;  // without cu_q
-  float zscale;       // sm_scale * log2(e)
+  float zscale;       // |sm_scale| * log2(e), above 0
+  uint32_t qsign;     // flips the queries' signs where sm_scale is negative
 };
 
 // What a tile of COLS columns is.  With cu_q the tiles of request r are
@@ -175,51 +177,91 @@ struct Codes {
   uint2 ks[2], vs[2];                        // their scales, 16 bits each
 };
 
+// A lane's byte offsets into a 16-slot group: keys and values (token 4 g).
 template <int D>
-__device__ inline void load_codes(const Args& a, const int (&base)[2], int n, int g,
-                                  Codes<D>& c) {
+struct Lane {
+  uint32_t k, v, s;
+  __device__ inline Lane(int n, int g)
+      : k(n * (D / 2) + g * (D / 8)), v(4 * g * (D / 2) + n * (D / 32)), s(8 * g) {}
+};
+
+template <typename T>
+__device__ inline T at(const void* base, uint32_t off) {
+  return *reinterpret_cast<const T*>(static_cast<const char*>(base) + off);
+}
+
+template <int D>
+__device__ inline void load_keys(const Args& a, const int (&base)[2], const Lane<D>& p,
+                                 Codes<D>& c) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const int64_t row = (int64_t)max(base[j], 0) * 16;  // a missing half reads slot 0
-    const uint8_t* kp = a.k_codes + row * (D / 2) + (uint32_t)(n * (D / 2) + g * (D / 8));
+    // a missing half reads slot 0
+    const uint8_t* kp = a.k_codes + (int64_t)max(base[j], 0) * (16 * D / 2);
+    if constexpr (D == 64) {
+      const uint2 x = at<uint2>(kp, p.k);
+      c.k[j][0] = x.x;
+      c.k[j][1] = x.y;
+    } else {
 #pragma unroll
-    for (int w = 0; w < Codes<D>::KD; w += 4) {
-      if constexpr (D == 64) {
-        const uint2 x = *reinterpret_cast<const uint2*>(kp);
-        c.k[j][0] = x.x;
-        c.k[j][1] = x.y;
-      } else {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(kp + w * 4);
+      for (int w = 0; w < Codes<D>::KD; w += 4) {
+        const u32x4 x = at<u32x4>(kp, p.k + w * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) c.k[j][w + e] = x[e];
       }
     }
-    const uint8_t* vp = a.v_codes + row * (D / 2) + (uint32_t)(4 * g * (D / 2) + n * (D / 32));
+  }
+}
+
+template <int D>
+__device__ inline void load_values(const Args& a, const int (&base)[2], const Lane<D>& p,
+                                   Codes<D>& c) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const uint8_t* vp = a.v_codes + (int64_t)max(base[j], 0) * (16 * D / 2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (D == 64) {
-        c.v[j][i][0] = *reinterpret_cast<const uint16_t*>(vp + i * (D / 2));
+        c.v[j][i][0] = at<uint16_t>(vp, p.v + i * (D / 2));
       } else if constexpr (D == 128) {
-        c.v[j][i][0] = *reinterpret_cast<const uint32_t*>(vp + i * (D / 2));
+        c.v[j][i][0] = at<uint32_t>(vp, p.v + i * (D / 2));
       } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(vp + i * (D / 2));
+        const uint2 x = at<uint2>(vp, p.v + i * (D / 2));
         c.v[j][i][0] = x.x;
         c.v[j][i][1] = x.y;
       }
     }
-    c.ks[j] = *reinterpret_cast<const uint2*>(a.k_scales + row + 4 * g);
-    c.vs[j] = *reinterpret_cast<const uint2*>(a.v_scales + row + 4 * g);
   }
+}
+
+template <int D>
+__device__ inline void load_scales(const Args& a, const int (&base)[2], const Lane<D>& p,
+                                   Codes<D>& c) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t row = (int64_t)max(base[j], 0) * 16;
+    c.ks[j] = at<uint2>(a.k_scales + row, p.s);
+    c.vs[j] = at<uint2>(a.v_scales + row, p.s);
+  }
+}
+
+// Codes of two tokens, eight features each, as pairs of one feature: byte f of
+// even holds feature 2 f of both, of odd feature 2 f + 1.
+__device__ inline void pair_tokens(uint32_t t0, uint32_t t1, uint32_t& even, uint32_t& odd) {
+  constexpr uint32_t lo = 0x0f0f0f0fu;
+  even = (t0 & lo) | (t1 << 4 & ~lo);
+  odd = (t0 >> 4 & lo) | (t1 & ~lo);
 }
 
 // Entry of byte b of w in the table: `off` is the lane's offset in an entry.
 // The table is the start of the workgroup's LDS (its kernels have dynamic LDS
 // only), so the v_perm is the whole address; through the pointer to the table
 // every look-up would cost an addition of that 0.
+template <int PART>  // 0: keys, 128: values
 __device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
-  typedef const uint32_t __attribute__((address_space(3))) * LdsPtr;
-  return *(LdsPtr)(uintptr_t)__builtin_amdgcn_perm(w, off,
-                                                   0x0c0c0000u | (uint32_t)(4 + b) << 8);
+  typedef const char __attribute__((address_space(3))) * LdsPtr;
+  typedef const uint32_t __attribute__((address_space(3))) * LdsWord;
+  const uint32_t at = __builtin_amdgcn_perm(w, off, 0x0c0c0000u | (uint32_t)(4 + b) << 8);
+  return *(LdsWord)((LdsPtr)(uintptr_t)at + PART);
 }
 
 // Work of a launch, counted in units of UNIT tokens (one turn of all waves).
@@ -309,12 +351,24 @@ struct Shares {
   }
 };
 
+// Keeps what a rarely taken branch computes inside it (selects in its place
+// would run for every tile).
+__device__ inline void rare(float& v) { asm volatile("" : "+v"(v)); }
+
 // The split form: the WAVES waves of a workgroup share NT tiles of 16 columns
 // and take 32 tokens in turn, each with its own running maximum and sum; they
 // are joined in LDS at the end of an item, cut items by a second kernel.
+// The kernel's (only) argument, read again from where it lies: what is not used
+// between two such places takes no registers there.
+__device__ inline const Args& arguments() {
+  auto p = (const Args __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
 template <int DT, int D, int NT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, WAVES * (NT * D > 256 ? 1 : 2) / 4)
-kv4_split_kernel(const Args a) {
+kv4_split_kernel(const Args args) {
   constexpr int COLS = 16 * NT, THREADS = WAVES * 64, UNIT = WAVES * 32;
   constexpr int KS = D / 32;  // steps of the first product
   constexpr int ND = D / 16;  // feature tiles of the second
@@ -326,7 +380,8 @@ kv4_split_kernel(const Args a) {
   int64_t u = blockIdx.x, u_end = u + 1;  // of all heads' units
   int64_t share = 1;
   int per_head = 1, table = -1;  // units of a head; head whose table is in LDS
-  if (!a.whole) {
+  if (!args.whole) {
+    const Args& a = arguments();
     const Shares<COLS, THREADS, UNIT> sh(a, s_pre);
     per_head = sh.total;
     const int64_t all = (int64_t)per_head * a.heads;
@@ -340,8 +395,9 @@ kv4_split_kernel(const Args a) {
     // registers over the whole share.
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
+    const Args& a = arguments();
     const int lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const uint32_t koff = (uint32_t)(lane & 31) * 4, voff = koff + 128;
+    const uint32_t loff = (uint32_t)(lane & 31) * 4;
     Item x;
     int ub;
     if (a.whole) {
@@ -397,25 +453,35 @@ kv4_split_kernel(const Args a) {
     int blk[2], base[2], nbase[2];
     load_blocks(wave, blk);
 
-    int lim[NT], row[NT], head[NT];
+    // Query and head of this lane's column of tile y; row -1 past the last.
+    auto column = [&](const Args& a, int y, int& row, int& head, int& i) {
+      const int col = t.col0 + 16 * y + n;
+      i = (int)a.gdiv.div(min(col, ncols - 1));
+      row = col < ncols ? t.row0 + i : -1;
+      head = x.hc * a.G + (min(col, ncols - 1) - i * a.G);
+    };
+    int lim[NT];
     u32x4 qf[NT][KS];
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
-      const int col = t.col0 + 16 * y + n;
-      const bool ok = col < ncols;
-      const int i = (int)a.gdiv.div(ok ? col : 0);
-      row[y] = t.row0 + i;
-      head[y] = x.hc * a.G + (ok ? col - i * a.G : 0);
+      int row, head, i;
+      column(a, y, row, head, i);
+      const bool ok = row >= 0;
       lim[y] = ok ? sees(a, t, i) : 0;
-      const uint16_t* qp = a.q + row[y] * a.q_ts + head[y] * a.q_hs + g * (D / 4);
+      const uint16_t* qp = a.q + max(row, t.row0) * a.q_ts + head * a.q_hs + g * (D / 4);
 #pragma unroll
       for (int s = 0; s < KS; ++s)
-        qf[y][s] = ok ? *reinterpret_cast<const u32x4*>(qp + s * 8) : u32x4{0, 0, 0, 0};
-      if (!ok) row[y] = -1;
+        qf[y][s] = (ok ? *reinterpret_cast<const u32x4*>(qp + s * 8) : u32x4{0, 0, 0, 0}) ^
+                   a.qsign;
     }
-    Codes<D> cur, nxt;
+    const Lane<D> lanes(n, g);
+    Codes<D> cur;
     groups(wave, blk, base);
-    if (a.num_blocks != 0) load_codes<D>(a, base, n, g, cur);
+    if (a.num_blocks != 0) {
+      load_keys<D>(a, base, lanes, cur);
+      load_scales<D>(a, base, lanes, cur);
+      load_values<D>(a, base, lanes, cur);
+    }
     load_blocks(wave + WAVES, blk);
     if (table != x.hc) {
       table = x.hc;
@@ -423,6 +489,7 @@ kv4_split_kernel(const Args a) {
     }
     __syncthreads();
 
+    // Maxima are of q k before the (positive) score scale.
     float m[NT], l[NT];
     f32x4 o[NT][ND];
 #pragma unroll
@@ -436,9 +503,11 @@ kv4_split_kernel(const Args a) {
     // times 2^14 over a power of two that no scale so far exceeds.
     float vref = 0.f, vmul = 1.f;
 
+    // What a tile has used up is fetched for the next one at once, into the
+    // same registers: with a second set of them four waves a SIMD do not fit,
+    // and it is they that hide the loads' latency.
     for (int it = wave; it < ntile; it += WAVES) {
       groups(it + WAVES, blk, nbase);
-      load_codes<D>(a, nbase, n, g, nxt);
       load_blocks(it + 2 * WAVES, blk);
 
       f32x4 s[NT][2];
@@ -448,11 +517,12 @@ kv4_split_kernel(const Args a) {
         for (int k = 0; k < KS; ++k) {
           u32x4 kf;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) kf[b] = lookup(cur.k[j][k], b, koff);
+          for (int b = 0; b < 4; ++b) kf[b] = lookup<0>(cur.k[j][k], b, loff);
 #pragma unroll
           for (int y = 0; y < NT; ++y)
             s[y][j] = mfma<DT>(kf, qf[y][k], k ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
+      load_keys<D>(a, nbase, lanes, cur);
       const int tok = t0 + it * 32 + 4 * g;  // token (j, i): tok + 16 j + i
       const bool masked = t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0;
       float ks[2][4], vs[2][4];
@@ -462,31 +532,46 @@ kv4_split_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) {
           const uint32_t kw = i < 2 ? cur.ks[j].x : cur.ks[j].y;
           const uint32_t vw = i < 2 ? cur.vs[j].x : cur.vs[j].y;
-          ks[j][i] = from16<DT>((i & 1) ? kw >> 16 : kw & 0xffffu) * a.zscale;
+          ks[j][i] = from16<DT>((i & 1) ? kw >> 16 : kw & 0xffffu);
           vs[j][i] = from16<DT>((i & 1) ? vw >> 16 : vw & 0xffffu);
-          // What lies past the requests' tokens is anything.
-          if (masked && (base[j] < 0 || tok + 16 * j + i >= lim_max)) vs[j][i] = 0.f;
         }
+      load_scales<D>(a, nbase, lanes, cur);
+      if (masked) {  // what lies past the requests' tokens is anything
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (base[j] < 0 || tok + 16 * j + i >= lim_max) vs[j][i] = 0.f;
+            rare(vs[j][i]);
+          }
+      }
       if constexpr (DT == FKC_F16) {
         float top = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            top = fmaxf(top, fabsf(vs[j][i]) < INFINITY ? fabsf(vs[j][i]) : 0.f);
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(vs[j][i]));
         if (__any(top > vref)) {
+          top = 0.f;  // of the finite ones; the others are what they are
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              top = fmaxf(top, fabsf(vs[j][i]) < INFINITY ? fabsf(vs[j][i]) : 0.f);
 #pragma unroll
           for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-          // next power of two: times 2^14 over it stays in range
-          const float ref = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
-          const float mul = 16384.f / ref;
-          const float f = vref > 0.f ? mul / vmul : 0.f;  // nothing yet: o is 0
-          vref = ref;
-          vmul = mul;
+          if (top > vref) {
+            // next power of two: times 2^14 over it stays in range
+            const float ref = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
+            const float mul = 16384.f / ref;
+            const float f = vref > 0.f ? mul / vmul : 0.f;  // nothing yet: o is 0
+            vref = ref;
+            vmul = mul;
 #pragma unroll
-          for (int y = 0; y < NT; ++y)
+            for (int y = 0; y < NT; ++y)
 #pragma unroll
-            for (int d = 0; d < ND; ++d) o[y][d] *= f;
+              for (int d = 0; d < ND; ++d) o[y][d] *= f;
+          }
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -500,55 +585,77 @@ kv4_split_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            z[j][i] = s[y][j][i] * ks[j][i];
-            if (masked && (base[j] < 0 || tok + 16 * j + i >= lim[y])) z[j][i] = -INFINITY;
-            top = fmaxf(top, z[j][i]);
-          }
+          for (int i = 0; i < 4; ++i) z[j][i] = s[y][j][i] * ks[j][i];
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (base[j] < 0 || tok + 16 * j + i >= lim[y]) z[j][i] = -INFINITY;
+              rare(z[j][i]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, z[j][i]);
         if (__any(top > m[y])) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           const float nm = fmaxf(m[y], top);
-          const float f = __builtin_amdgcn_exp2f(m[y] - nm);
+          const float f = __builtin_amdgcn_exp2f((m[y] - nm) * a.zscale);
           m[y] = nm;
           l[y] *= f;
 #pragma unroll
           for (int d = 0; d < ND; ++d) o[y][d] *= f;
         }
+        const float mz = m[y] * a.zscale;
         float w[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(z[j][i] - m[y]);
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][i], a.zscale, -mz));
             l[y] += p;
-            w[j][i] = masked && z[j][i] == -INFINITY ? 0.f : p * vs[j][i];
+            w[j][i] = p * vs[j][i];
           }
+        if (masked) {  // a scale that is not finite counts where it is seen
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              w[j][i] = z[j][i] == -INFINITY ? 0.f : w[j][i];
+              rare(w[j][i]);
+            }
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           pf[y][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
       }
+      // Features 2 b and 2 b + 1 of the lane's row, two tokens a dword.
 #pragma unroll
-      for (int b = 0; b < ND / 2; ++b) {
-        uint32_t e[2][4];
+      for (int v = 0; v < (ND + 7) / 8; ++v) {
+        uint32_t even[4], odd[4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int k = 0; k < 4; ++k)
+          pair_tokens(cur.v[k >> 1][2 * (k & 1)][v], cur.v[k >> 1][2 * (k & 1) + 1][v], even[k],
+                      odd[k]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e[j][i] = lookup(cur.v[j][i][b / 4], b % 4, voff);
-        u32x4 lo, hi;  // features 2 b and 2 b + 1 of the lane's row, by token
+        for (int b = 0; b < (ND < 8 ? ND / 2 : 4); ++b) {
+          u32x4 lo, hi;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t x0 = e[k >> 1][2 * (k & 1)], x1 = e[k >> 1][2 * (k & 1) + 1];
-          lo[k] = __builtin_amdgcn_perm(x1, x0, 0x05040100u);
-          hi[k] = __builtin_amdgcn_perm(x1, x0, 0x07060302u);
-        }
+          for (int k = 0; k < 4; ++k) {
+            lo[k] = lookup<128>(even[k], b, loff);
+            hi[k] = lookup<128>(odd[k], b, loff);
+          }
 #pragma unroll
-        for (int y = 0; y < NT; ++y) {
-          o[y][2 * b] = mfma<DT>(lo, pf[y], o[y][2 * b]);
-          o[y][2 * b + 1] = mfma<DT>(hi, pf[y], o[y][2 * b + 1]);
+          for (int y = 0; y < NT; ++y) {
+            o[y][8 * v + 2 * b] = mfma<DT>(lo, pf[y], o[y][8 * v + 2 * b]);
+            o[y][8 * v + 2 * b + 1] = mfma<DT>(hi, pf[y], o[y][8 * v + 2 * b + 1]);
+          }
         }
       }
-      cur = nxt;
+      load_values<D>(a, nbase, lanes, cur);
       base[0] = nbase[0];
       base[1] = nbase[1];
     }
@@ -583,8 +690,8 @@ kv4_split_kernel(const Args a) {
         if (wave < half) {
           const float m2 = sml[wave * 32 + n], l2 = sml[wave * 32 + 16 + n];
           const float nm = fmaxf(m[y], m2);
-          const float f1 = __builtin_amdgcn_exp2f(m[y] - nm);
-          const float f2 = __builtin_amdgcn_exp2f(m2 - nm);
+          const float f1 = __builtin_amdgcn_exp2f((m[y] - nm) * a.zscale);
+          const float f2 = __builtin_amdgcn_exp2f((m2 - nm) * a.zscale);
           m[y] = nm;
           l[y] = l[y] * f1 + l2 * f2;
 #pragma unroll
@@ -595,12 +702,15 @@ kv4_split_kernel(const Args a) {
     }
     const bool cut = x.unit > 0 || ub < x.n;
     if (wave == 0) {
+      const Args& a = arguments();
       // A share cuts the item before it and the one after it at most.
       const int64_t slot = (int64_t)blockIdx.x * 2 + (x.unit > 0 ? 0 : 1);
 #pragma unroll
       for (int y = 0; y < NT; ++y) {
-        if (row[y] < 0) continue;
-        const int64_t at = (int64_t)row[y] * a.H + head[y];
+        int row, head, i;
+        column(a, y, row, head, i);
+        if (row < 0) continue;
+        const int64_t at = (int64_t)row * a.H + head;
         if (!cut) {
           const float f = l[y] > 0.f ? 1.f / l[y] : 0.f;
 #pragma unroll
@@ -614,7 +724,7 @@ kv4_split_kernel(const Args a) {
             for (int d = 0; d < ND / 2; ++d) op[d] = w[d];
           }
           if (g == 0 && a.lse != nullptr)
-            a.lse[at] = l[y] > 0.f ? m[y] * kLn2 + __logf(l[y]) : -INFINITY;
+            a.lse[at] = l[y] > 0.f ? m[y] * a.zscale * kLn2 + __logf(l[y]) : -INFINITY;
         } else {
           float* op = a.part + (slot * COLS + 16 * y + n) * D;
 #pragma unroll
@@ -622,7 +732,7 @@ kv4_split_kernel(const Args a) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) op[(4 * g + i) * ND + d] = o[y][d][i];
           if (g == 0) {
-            a.part_ml[(slot * COLS + 16 * y + n) * 2] = m[y];
+            a.part_ml[(slot * COLS + 16 * y + n) * 2] = m[y] * a.zscale;
             a.part_ml[(slot * COLS + 16 * y + n) * 2 + 1] = l[y];
           }
         }
@@ -639,55 +749,89 @@ kv4_split_kernel(const Args a) {
 
 // Joins the parts of a cut item: the workgroup's that its first unit was in
 // (its second slot) and the following ones' (their first).  A workgroup per
-// four columns, D / 4 lanes per part.
+// four columns: their weights into LDS, PARTS parts at a time, then D / 4
+// lanes per part, every load independent of the others.
 template <int DT, int D, int COLS>
 __global__ void __launch_bounds__(256)
 kv4_join_kernel(const Args a) {
-  constexpr int LPC = D / 4, CP = 256 / LPC;
+  constexpr int LPC = D / 4, CP = 256 / LPC, JC = 4, PARTS = 64;
   __shared__ f32x4 so[256];
-  __shared__ float sm[CP], sl[CP];
+  __shared__ float sw[JC][PARTS];
   const int4 item = a.desc[blockIdx.x];
-  const int ncols = item.w >> 16, hc = item.w & 0xffff;
+  if (item.x == 0) return;
+  const int ncols = item.w >> 16, hc = item.w & 0xffff, col0 = blockIdx.y * JC;
+  if (col0 >= ncols) return;
   const int sub = threadIdx.x % LPC, part = threadIdx.x / LPC;
-  for (int col = blockIdx.y * 4; item.x > 0 && col < min(ncols, (int)blockIdx.y * 4 + 4); ++col) {
-    float m = kLowest, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int c = part; c < item.x; c += CP) {
-      const int64_t at = (((int64_t)blockIdx.x + c) * 2 + (c ? 0 : 1)) * COLS + col;
-      const float m2 = a.part_ml[2 * at], l2 = a.part_ml[2 * at + 1];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * sub);
-      const float nm = fmaxf(m, m2);
-      const float f1 = __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(m2 - nm);
-      m = nm;
-      l = l * f1 + l2 * f2;
-      o = o * f1 + x * f2;
-    }
-    __syncthreads();
-    so[threadIdx.x] = o;
-    if (sub == 0) {
-      sm[part] = m;
-      sl[part] = l;
-    }
-    __syncthreads();
-    if (threadIdx.x >= LPC) continue;
+  // row of part c, column col0 + j in part and part_ml
+  auto place = [&](int c, int j) {
+    return (((int64_t)blockIdx.x + c) * 2 + (c ? 0 : 1)) * COLS + min(col0 + j, COLS - 1);
+  };
+  // One wave per column: a lane per part.
+  const int j = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float m = kLowest, l = 0.f;
+  f32x4 o[JC];
 #pragma unroll
-    for (int c = 1; c < CP; ++c) {
-      const float nm = fmaxf(m, sm[c]);
-      const float f1 = __builtin_amdgcn_exp2f(m - nm), f2 = __builtin_amdgcn_exp2f(sm[c] - nm);
-      m = nm;
-      l = l * f1 + sl[c] * f2;
-      o = o * f1 + so[c * LPC + sub] * f2;
+  for (int x = 0; x < JC; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; c0 < item.x; c0 += PARTS) {
+    f32x4 v[JC][PARTS / CP];
+#pragma unroll
+    for (int i = 0; i < PARTS / CP; ++i)
+#pragma unroll
+      for (int x = 0; x < JC; ++x) {
+        const int c = min(c0 + i * CP + part, item.x - 1);
+        v[x][i] = *reinterpret_cast<const f32x4*>(a.part + place(c, x) * D + 4 * sub);
+      }
+    float m2 = kLowest, l2 = 0.f;
+    if (c0 + lane < item.x) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * place(c0 + lane, j));
+      m2 = ml.x;
+      l2 = ml.y;
     }
+    float nm = fmaxf(m, m2);
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) nm = fmaxf(nm, __shfl_xor(nm, off, 64));
+    const float f = __builtin_amdgcn_exp2f(m - nm), w = __builtin_amdgcn_exp2f(m2 - nm);
+    m = nm;
+    l = l * f + wave_sum(l2 * w);
+    __syncthreads();  // sw is read
+    sw[j][lane] = c0 + lane < item.x ? w : 0.f;
+    if (lane == 0) reinterpret_cast<float*>(so)[j] = f;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < JC; ++x) {
+      o[x] *= reinterpret_cast<const float*>(so)[x];
+#pragma unroll
+      for (int i = 0; i < PARTS / CP; ++i) {
+        const float wt = sw[x][i * CP + part];
+        // (the column or part may not exist; what stands there may be NaN)
+        o[x] += wt != 0.f ? v[x][i] * wt : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  }
+  __syncthreads();
+  if (lane == 0) {
+    sw[j][0] = l;
+    sw[j][1] = m;
+  }
+#pragma unroll
+  for (int x = 0; x < JC; ++x) {
+    __syncthreads();
+    so[threadIdx.x] = o[x];
+    __syncthreads();
+    const int col = col0 + x;
+    if (threadIdx.x >= LPC || col >= ncols) continue;
+    f32x4 sum = so[sub];
+#pragma unroll
+    for (int c = 1; c < CP; ++c) sum += so[c * LPC + sub];
     const int i = (int)a.gdiv.div(item.z + col);
-    const int64_t at =
-        (int64_t)(item.y + i) * a.H + hc * a.G + (item.z + col - i * a.G);
-    const float f = l > 0.f ? 1.f / l : 0.f;
+    const int64_t at = (int64_t)(item.y + i) * a.H + hc * a.G + (item.z + col - i * a.G);
+    const float den = sw[x][0], f = den > 0.f ? 1.f / den : 0.f;
     uint2 w;
-    w.x = pack2<DT>(o[0] * f, o[1] * f);
-    w.y = pack2<DT>(o[2] * f, o[3] * f);
+    w.x = pack2<DT>(sum[0] * f, sum[1] * f);
+    w.y = pack2<DT>(sum[2] * f, sum[3] * f);
     *reinterpret_cast<uint2*>(a.out + at * D + 4 * sub) = w;
     if (sub == 0 && a.lse != nullptr)
-      a.lse[at] = l > 0.f ? m * kLn2 + __logf(l) : -INFINITY;
+      a.lse[at] = den > 0.f ? sw[x][1] * kLn2 + __logf(den) : -INFINITY;
   }
 }
 
@@ -775,7 +919,10 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
          x.tables, x.table_stride, x.seq, x.cu_q, (uint16_t*)x.out, x.lse, nullptr, nullptr,
          nullptr, FastDiv((uint32_t)c.block_size), FastDiv((uint32_t)G), (uint32_t)c.num_blocks,
          (int)c.heads, (int)x.H, G, (int)x.T, (int)x.R, (int)x.max_seq, (int)x.causal,
-         (int)p.whole, kMinShare / 2, p.tiles_per_req, x.sm_scale * kLog2e};
+         (int)p.whole, kMinShare / 2, p.tiles_per_req,
+         // (of scores times 0 the masked ones would be NaN)
+         std::max(std::fabs(x.sm_scale) * kLog2e, 1e-30f),
+         std::signbit(x.sm_scale) ? 0x80008000u : 0u};
   if (!p.whole) {
     Carve w(ws);
     a.part = w.take<float>(p.part_rows() * c.D);
