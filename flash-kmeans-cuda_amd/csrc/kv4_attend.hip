@@ -70,7 +70,7 @@ constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
                                            // a difference of two is no NaN
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
-constexpr int kJoin = 8 / 2 * 32 * 4;      // maxima and sums of half the waves
+constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
 // Read by scalar loads: nothing writes it while the kernel runs.
 typedef const int32_t __attribute__((address_space(4))) * Const32;
@@ -152,18 +152,24 @@ __device__ inline int sees(const Args& a, const Tile& t, int i) {
   return a.causal ? max(0, t.end - t.nq + 1 + i) : t.end;
 }
 
-// Tables of a head's level pairs, by the whole workgroup.
+// Tables of a head's level pairs, by the whole workgroup: thread tid writes
+// entries of low level tid / 16 % 16 only, so it needs that one and, of the
+// high ones, those its turns r come to.
 template <int THREADS>
 __device__ inline void fill_table(const Args& a, int hc, char* lds, int tid) {
-  const uint16_t* kl = a.k_levels + hc * 16;
-  const uint16_t* vl = a.v_levels + hc * 16;
+  constexpr int TURNS = kTable / 16 / THREADS, PER = 16 / TURNS;  // high levels per turn
+  const uint16_t* lv = ((tid & 8) ? a.v_levels : a.k_levels) + hc * 16;
+  const uint32_t low = lv[tid / 16 % 16];
+  u32x4 high[2];
+  high[0] = reinterpret_cast<const u32x4*>(lv)[0];
+  high[1] = reinterpret_cast<const u32x4*>(lv)[1];
+  const bool odd = tid / 256;  // with two high levels per turn: the second
 #pragma unroll
-  for (int r = 0; r < kTable / 16 / THREADS; ++r) {
-    const int i = r * THREADS + tid;
-    const int e = i / (kEntry / 16);
-    const uint16_t* lv = (i & 8) ? vl : kl;
-    const uint32_t w = lv[e & 15] | (uint32_t)lv[e >> 4] << 16;
-    *reinterpret_cast<u32x4*>(lds + i * 16) = u32x4{w, w, w, w};
+  for (int r = 0; r < TURNS; ++r) {
+    const int h = r * PER;
+    const uint32_t two = high[h / 8][h / 2 % 4];
+    const uint32_t w = ((PER == 2 ? odd : h & 1) ? two & 0xffff0000u : two << 16) | low;
+    *reinterpret_cast<u32x4*>(lds + (r * THREADS + tid) * 16) = u32x4{w, w, w, w};
   }
 }
 
@@ -279,7 +285,7 @@ struct Item {
 };
 
 template <int COLS>
-__device__ inline void request(const Args& a, int r, Tile& t, int& n, int& tiles) {
+__device__ inline void request(const Args& a, int r, Tile& t, int& tiles) {
   t.req = r;
   if (a.cu_q == nullptr) {
     t.row0 = r;
@@ -296,13 +302,12 @@ __device__ inline void request(const Args& a, int r, Tile& t, int& n, int& tiles
 // Running sums of the requests' units, THREADS slices of `per` requests.
 template <int COLS, int THREADS, int UNIT>
 struct Shares {
-  int* s_pre;  // LDS, THREADS + THREADS / 64
+  int* s_pre;  // LDS: THREADS + THREADS / 64 rounded to a multiple of 4, then
+               // four numbers of each request where every thread has one
   int per, total;
-  __device__ inline int units(const Args& a, int r) const {
-    Tile t;
-    int n, tiles;
-    request<COLS>(a, r, t, n, tiles);
-    return tiles * max((t.end + UNIT - 1) / UNIT, 1);
+  static constexpr int kInts = THREADS + (THREADS / 64 + 3) / 4 * 4 + THREADS * 4;
+  __device__ inline int4* s_req() const {
+    return reinterpret_cast<int4*>(s_pre + THREADS + (THREADS / 64 + 3) / 4 * 4);
   }
   __device__ inline Shares(int* lds, int p, int n) : s_pre(lds), per(p), total(n) {}
   __device__ inline Shares(const Args& a, int* lds) : s_pre(lds) {
@@ -311,7 +316,12 @@ struct Shares {
     int sum = 0;
     for (int i = 0; i < per; ++i) {
       const int r = threadIdx.x * per + i;
-      if (r < rt) sum += units(a, r);
+      if (r >= rt) break;
+      Tile t;
+      int tiles;
+      request<COLS>(a, r, t, tiles);
+      sum += tiles * max((t.end + UNIT - 1) / UNIT, 1);
+      if (per == 1) s_req()[r] = int4{t.row0, t.nq, t.end, 0};
     }
     const int incl = wave_incl_scan(sum);
     int* s_wave = s_pre + THREADS;
@@ -337,12 +347,21 @@ struct Shares {
     u -= __builtin_amdgcn_readfirstlane(s_pre[j]);
     Item x;
     x.hc = hc;
-    int r = j * per, tiles = 0;
-    for (;; ++r) {
-      request<COLS>(a, r, x.t, x.n, tiles);
+    if (per == 1) {
+      const int4 q = s_req()[j];
+      x.t.req = j;
+      x.t.row0 = q.x;
+      x.t.nq = q.y;
+      x.t.end = q.z;
       x.n = max((x.t.end + UNIT - 1) / UNIT, 1);
-      if (u < tiles * x.n || r >= a.R) break;
-      u -= tiles * x.n;
+    } else {
+      for (int r = j * per;; ++r) {
+        int tiles;
+        request<COLS>(a, r, x.t, tiles);
+        x.n = max((x.t.end + UNIT - 1) / UNIT, 1);
+        if (u < tiles * x.n || r >= a.R) break;
+        u -= tiles * x.n;
+      }
     }
     const int tile = u / x.n;
     x.unit = u - tile * x.n;
@@ -373,7 +392,7 @@ kv4_split_kernel(const Args args) {
   constexpr int KS = D / 32;  // steps of the first product
   constexpr int ND = D / 16;  // feature tiles of the second
   extern __shared__ __align__(16) char lds[];
-  float* sml = reinterpret_cast<float*>(lds + kTable);
+  float2* sml = reinterpret_cast<float2*>(lds + kTable);
   int* s_pre = reinterpret_cast<int*>(lds + kTable + kJoin);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -453,9 +472,9 @@ kv4_split_kernel(const Args args) {
     int blk[2], base[2], nbase[2];
     load_blocks(wave, blk);
 
-    // Query and head of this lane's column of tile y; row -1 past the last.
-    auto column = [&](const Args& a, int y, int& row, int& head, int& i) {
-      const int col = t.col0 + 16 * y + n;
+    // Query and head of a column of the tile; row -1 past the last.
+    auto column = [&](const Args& a, int col, int& row, int& head, int& i) {
+      col += t.col0;
       i = (int)a.gdiv.div(min(col, ncols - 1));
       row = col < ncols ? t.row0 + i : -1;
       head = x.hc * a.G + (min(col, ncols - 1) - i * a.G);
@@ -465,7 +484,7 @@ kv4_split_kernel(const Args args) {
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
       int row, head, i;
-      column(a, y, row, head, i);
+      column(a, 16 * y + n, row, head, i);
       const bool ok = row >= 0;
       lim[y] = ok ? sees(a, t, i) : 0;
       const uint16_t* qp = a.q + max(row, t.row0) * a.q_ts + head * a.q_hs + g * (D / 4);
@@ -661,83 +680,70 @@ kv4_split_kernel(const Args args) {
     }
 
     // Join the lanes of a column (they share m), then the waves that had
-    // tokens, half of them at a time, the later one into the earlier.
+    // tokens: their outputs, relative to the largest maximum, go to LDS as
+    // rows of features (over the table, 16-byte pieces turned by the column
+    // so that no two lanes meet in a bank) and are summed as they are written.
+    const int waves = min(ntile, WAVES);
+    table = -1;
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
       l[y] += __shfl_xor(l[y], 16, 64);
       l[y] += __shfl_xor(l[y], 32, 64);
-      if constexpr (DT == FKC_F16)
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[y][d] *= 1.f / vmul;
-    }
-    if (ntile > 1) table = -1;  // the table's place is used
-#pragma unroll
-    for (int half = WAVES / 2; half > 0; half /= 2) {
-      if (ntile <= half) continue;
-#pragma unroll
-      for (int y = 0; y < NT; ++y) {
-        f32x4* so = reinterpret_cast<f32x4*>(lds);
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-          for (int d = 0; d < ND; ++d) so[((wave - half) * ND + d) * 64 + lane] = o[y][d];
-          if (g == 0) {
-            sml[(wave - half) * 32 + n] = m[y];
-            sml[(wave - half) * 32 + 16 + n] = l[y];
-          }
-        }
-        __syncthreads();
-        if (wave < half) {
-          const float m2 = sml[wave * 32 + n], l2 = sml[wave * 32 + 16 + n];
-          const float nm = fmaxf(m[y], m2);
-          const float f1 = __builtin_amdgcn_exp2f((m[y] - nm) * a.zscale);
-          const float f2 = __builtin_amdgcn_exp2f((m2 - nm) * a.zscale);
-          m[y] = nm;
-          l[y] = l[y] * f1 + l2 * f2;
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-            o[y][d] = o[y][d] * f1 + so[(wave * ND + d) * 64 + lane] * f2;
-        }
-      }
-    }
-    const bool cut = x.unit > 0 || ub < x.n;
-    if (wave == 0) {
+      if (y) __syncthreads();  // the last tile's pieces are read
+      if (g == 0) sml[wave * 16 + n] = float2{m[y], l[y]};
+      __syncthreads();
       const Args& a = arguments();
+      float top = kLowest;
+      for (int w = 0; w < waves; ++w) top = fmaxf(top, sml[w * 16 + n].x);
+      const float f = __builtin_amdgcn_exp2f((m[y] - top) * a.zscale) *
+                      (DT == FKC_F16 ? 1.f / vmul : 1.f);
+      f32x4* so = reinterpret_cast<f32x4*>(lds);
+      if (wave < waves) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int d = 0; d < ND / 4; ++d) {
+            const int piece = (4 * g + i) * (ND / 4) + d;
+            so[(wave * 16 + n) * (D / 4) + (piece ^ n)] =
+                f32x4{o[y][4 * d][i], o[y][4 * d + 1][i], o[y][4 * d + 2][i],
+                      o[y][4 * d + 3][i]} * f;
+          }
+      }
+      __syncthreads();
+      const bool cut = x.unit > 0 || ub < x.n;
       // A share cuts the item before it and the one after it at most.
       const int64_t slot = (int64_t)blockIdx.x * 2 + (x.unit > 0 ? 0 : 1);
-#pragma unroll
-      for (int y = 0; y < NT; ++y) {
+#pragma unroll 1
+      for (int e = tid; e < 16 * D / 4; e += THREADS) {
+        const int col = e / (D / 4), piece = e % (D / 4);
         int row, head, i;
-        column(a, y, row, head, i);
+        column(a, 16 * y + col, row, head, i);
         if (row < 0) continue;
+        float top = kLowest, sum = 0.f;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < waves; ++w) top = fmaxf(top, sml[w * 16 + col].x);
+        for (int w = 0; w < waves; ++w) {
+          const float2 ml = sml[w * 16 + col];
+          sum += ml.y * __builtin_amdgcn_exp2f((ml.x - top) * a.zscale);
+          v += so[(w * 16 + col) * (D / 4) + (piece ^ col)];
+        }
         const int64_t at = (int64_t)row * a.H + head;
         if (!cut) {
-          const float f = l[y] > 0.f ? 1.f / l[y] : 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[ND / 2];
-#pragma unroll
-            for (int d = 0; d < ND / 2; ++d)
-              w[d] = pack2<DT>(o[y][2 * d][i] * f, o[y][2 * d + 1][i] * f);
-            uint32_t* op = reinterpret_cast<uint32_t*>(a.out + at * D + (4 * g + i) * ND);
-#pragma unroll
-            for (int d = 0; d < ND / 2; ++d) op[d] = w[d];
-          }
-          if (g == 0 && a.lse != nullptr)
-            a.lse[at] = l[y] > 0.f ? m[y] * a.zscale * kLn2 + __logf(l[y]) : -INFINITY;
+          const float f = sum > 0.f ? 1.f / sum : 0.f;
+          uint2 w;
+          w.x = pack2<DT>(v[0] * f, v[1] * f);
+          w.y = pack2<DT>(v[2] * f, v[3] * f);
+          *reinterpret_cast<uint2*>(a.out + at * D + 4 * piece) = w;
+          if (piece == 0 && a.lse != nullptr)
+            a.lse[at] = sum > 0.f ? top * a.zscale * kLn2 + __logf(sum) : -INFINITY;
         } else {
-          float* op = a.part + (slot * COLS + 16 * y + n) * D;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) op[(4 * g + i) * ND + d] = o[y][d][i];
-          if (g == 0) {
-            a.part_ml[(slot * COLS + 16 * y + n) * 2] = m[y] * a.zscale;
-            a.part_ml[(slot * COLS + 16 * y + n) * 2 + 1] = l[y];
-          }
+          const int64_t at = slot * COLS + 16 * y + col;
+          *reinterpret_cast<f32x4*>(a.part + at * D + 4 * piece) = v;
+          if (piece == 0)
+            *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top * a.zscale, sum};
         }
       }
-      if (cut && x.unit == 0 && lane == 0) {
+      if (cut && x.unit == 0 && tid == 0 && y == 0) {
         // u is the share's end: the item's other units are the next ones'.
         const int more = (int)((x.n - ub + share - 1) / share);
         a.desc[blockIdx.x] = int4{more + 1, t.row0, t.col0, (last - t.col0 + 1) << 16 | x.hc};
@@ -877,7 +883,7 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
 
 template <int DT, int D, int NT, int WAVES>
 int launch_split(const Args& a, const Plan& p, hipStream_t s) {
-  const int bytes = kTable + kJoin + (WAVES * 64 + WAVES) * 4;
+  const int bytes = kTable + kJoin + Shares<16 * NT, WAVES * 64, WAVES * 32>::kInts * 4;
   auto* kernel = &kv4_split_kernel<DT, D, NT, WAVES>;
   if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
