@@ -58,6 +58,13 @@ __device__ inline uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
+// A barrier for what is passed through LDS.  (__syncthreads also waits for every
+// global load and store that is on its way: those prefetched for the next tile
+// and the results of the last item.)
+__device__ inline void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 template <int DT>
 __device__ inline float from16(uint32_t bits) {
   using E = Elem<DT>;
@@ -70,6 +77,7 @@ constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
                                            // a difference of two is no NaN
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
+constexpr int kItem = 3;                   // units that an item costs by itself
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
 // Read by scalar loads: nothing writes it while the kernel runs.
@@ -272,7 +280,8 @@ __device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
 
 // Work of a launch, counted in units of UNIT tokens (one turn of all waves).
 // An item is a tile of a request under one cache head; each of a request's
-// tiles counts ceil(tokens / UNIT) units, at least one.  The items in order
+// tiles counts ceil(tokens / UNIT) units, at least one, and kItem more in
+// front of them for what an item costs by itself.  The items in order
 // (head, request, tile) are cut into equal shares, one per workgroup, wherever
 // the cuts fall: lengths of any mixture fill the chip evenly, a workgroup
 // meets few heads (whose tables it has to fill), and an item that is cut is
@@ -280,8 +289,8 @@ __device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
 struct Item {
   int hc;
   Tile t;
-  int n;     // units
-  int unit;  // first unit of the share in it
+  int n;   // units, with the kItem first ones
+  int at;  // first of them that is the share's
 };
 
 template <int COLS>
@@ -320,13 +329,13 @@ struct Shares {
       Tile t;
       int tiles;
       request<COLS>(a, r, t, tiles);
-      sum += tiles * max((t.end + UNIT - 1) / UNIT, 1);
+      sum += tiles * (max((t.end + UNIT - 1) / UNIT, 1) + kItem);
       if (per == 1) s_req()[r] = int4{t.row0, t.nq, t.end, 0};
     }
     const int incl = wave_incl_scan(sum);
     int* s_wave = s_pre + THREADS;
     if ((threadIdx.x & 63) == 63) s_wave[threadIdx.x >> 6] = incl;
-    __syncthreads();
+    lds_barrier();
     int before = 0;
     total = 0;
 #pragma unroll
@@ -335,7 +344,7 @@ struct Shares {
       total += s_wave[w];
     }
     s_pre[threadIdx.x] = before + incl - sum;
-    __syncthreads();
+    lds_barrier();
     total = __builtin_amdgcn_readfirstlane(total);
   }
   // The item that unit u (below total) of a head's falls into.
@@ -353,18 +362,18 @@ struct Shares {
       x.t.row0 = q.x;
       x.t.nq = q.y;
       x.t.end = q.z;
-      x.n = max((x.t.end + UNIT - 1) / UNIT, 1);
+      x.n = max((x.t.end + UNIT - 1) / UNIT, 1) + kItem;
     } else {
       for (int r = j * per;; ++r) {
         int tiles;
         request<COLS>(a, r, x.t, tiles);
-        x.n = max((x.t.end + UNIT - 1) / UNIT, 1);
+        x.n = max((x.t.end + UNIT - 1) / UNIT, 1) + kItem;
         if (u < tiles * x.n || r >= a.R) break;
         u -= tiles * x.n;
       }
     }
     const int tile = u / x.n;
-    x.unit = u - tile * x.n;
+    x.at = u - tile * x.n;
     x.t.col0 = tile * COLS;
     return x;
   }
@@ -409,7 +418,7 @@ kv4_split_kernel(const Args args) {
     u_end = min(u + share, all);
     if (threadIdx.x == 0) a.desc[blockIdx.x].x = 0;
   }
-  for (; u < u_end;) {
+  while (u < u_end) {
     // Opaque, so that what derives from it is computed per item, not kept in
     // registers over the whole share.
     int tid = threadIdx.x;
@@ -418,35 +427,39 @@ kv4_split_kernel(const Args args) {
     const int lane = tid & 63, n = lane & 15, g = lane >> 4;
     const uint32_t loff = (uint32_t)(lane & 31) * 4;
     Item x;
-    int ub;
+    int units, from, to;  // of the item, and the share's of them
     if (a.whole) {
       // Heads first: consecutive workgroups go to the eight XCDs in turn, and
       // every head has as much to do as the next.
       const int tile = blockIdx.x / a.heads;
       x.hc = blockIdx.x - tile * a.heads;
       if (!find_tile<COLS>(a, tile, x.t)) return;
-      x.unit = 0;
-      x.n = ub = max((x.t.end + UNIT - 1) / UNIT, 1);
+      from = 0;
+      units = to = max((x.t.end + UNIT - 1) / UNIT, 1);
       u = u_end;
     } else {
       Shares<COLS, THREADS, UNIT> sh(s_pre, (a.R + (a.cu_q != nullptr) + THREADS - 1) / THREADS,
                                      per_head);
       const int hc = (int)(u / per_head);
       x = sh.find(a, hc, (int)(u - (int64_t)hc * per_head));
-      ub = (int)min((int64_t)x.n, x.unit + (u_end - u));
-      u += ub - x.unit;
+      const int end = (int)min((int64_t)x.n, x.at + (u_end - u));
+      u += end - x.at;
+      from = max(x.at - kItem, 0);
+      to = max(end - kItem, 0);
+      units = x.n - kItem;
+      if (to == 0) break;  // the share ends before the item's units
     }
     // The same in every lane, which the compiler cannot see of loaded values.
     auto scalar = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
     Tile& t = x.t;
     scalar(t.req), scalar(t.row0), scalar(t.nq), scalar(t.col0), scalar(t.end);
-    scalar(x.hc), scalar(x.n), scalar(x.unit), scalar(ub);
+    scalar(x.hc), scalar(units), scalar(from), scalar(to);
     const int ncols = t.nq * a.G;
     const int last = min(t.col0 + COLS, ncols) - 1;
     const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0));
     const int lim_max = sees(a, t, (int)a.gdiv.div(last));
-    const int t0 = x.unit * UNIT;
-    const int t1 = min(ub * UNIT, lim_max);
+    const int t0 = from * UNIT;
+    const int t1 = min(to * UNIT, lim_max);
     const int ntile = max(t1 - t0 + 31, 0) / 32;
     const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
 
@@ -496,7 +509,7 @@ kv4_split_kernel(const Args args) {
     const Lane<D> lanes(n, g);
     Codes<D> cur;
     groups(wave, blk, base);
-    if (a.num_blocks != 0) {
+    if (wave < ntile) {
       load_keys<D>(a, base, lanes, cur);
       load_scales<D>(a, base, lanes, cur);
       load_values<D>(a, base, lanes, cur);
@@ -506,7 +519,7 @@ kv4_split_kernel(const Args args) {
       table = x.hc;
       fill_table<THREADS>(a, x.hc, lds, tid);
     }
-    __syncthreads();
+    lds_barrier();
 
     // Maxima are of q k before the (positive) score scale.
     float m[NT], l[NT];
@@ -526,6 +539,7 @@ kv4_split_kernel(const Args args) {
     // same registers: with a second set of them four waves a SIMD do not fit,
     // and it is they that hide the loads' latency.
     for (int it = wave; it < ntile; it += WAVES) {
+      const bool more = it + WAVES < ntile;
       groups(it + WAVES, blk, nbase);
       load_blocks(it + 2 * WAVES, blk);
 
@@ -541,7 +555,7 @@ kv4_split_kernel(const Args args) {
           for (int y = 0; y < NT; ++y)
             s[y][j] = mfma<DT>(kf, qf[y][k], k ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
-      load_keys<D>(a, nbase, lanes, cur);
+      if (more) load_keys<D>(a, nbase, lanes, cur);
       const int tok = t0 + it * 32 + 4 * g;  // token (j, i): tok + 16 j + i
       const bool masked = t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0;
       float ks[2][4], vs[2][4];
@@ -554,7 +568,7 @@ kv4_split_kernel(const Args args) {
           ks[j][i] = from16<DT>((i & 1) ? kw >> 16 : kw & 0xffffu);
           vs[j][i] = from16<DT>((i & 1) ? vw >> 16 : vw & 0xffffu);
         }
-      load_scales<D>(a, nbase, lanes, cur);
+      if (more) load_scales<D>(a, nbase, lanes, cur);
       if (masked) {  // what lies past the requests' tokens is anything
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -674,7 +688,7 @@ kv4_split_kernel(const Args args) {
           }
         }
       }
-      load_values<D>(a, nbase, lanes, cur);
+      if (more) load_values<D>(a, nbase, lanes, cur);
       base[0] = nbase[0];
       base[1] = nbase[1];
     }
@@ -689,9 +703,9 @@ kv4_split_kernel(const Args args) {
     for (int y = 0; y < NT; ++y) {
       l[y] += __shfl_xor(l[y], 16, 64);
       l[y] += __shfl_xor(l[y], 32, 64);
-      if (y) __syncthreads();  // the last tile's pieces are read
+      if (y) lds_barrier();  // the last tile's pieces are read
       if (g == 0) sml[wave * 16 + n] = float2{m[y], l[y]};
-      __syncthreads();
+      lds_barrier();
       const Args& a = arguments();
       float top = kLowest;
       for (int w = 0; w < waves; ++w) top = fmaxf(top, sml[w * 16 + n].x);
@@ -709,10 +723,10 @@ kv4_split_kernel(const Args args) {
                       o[y][4 * d + 3][i]} * f;
           }
       }
-      __syncthreads();
-      const bool cut = x.unit > 0 || ub < x.n;
+      lds_barrier();
+      const bool cut = from > 0 || to < units;
       // A share cuts the item before it and the one after it at most.
-      const int64_t slot = (int64_t)blockIdx.x * 2 + (x.unit > 0 ? 0 : 1);
+      const int64_t slot = (int64_t)blockIdx.x * 2 + (from > 0 ? 0 : 1);
 #pragma unroll 1
       for (int e = tid; e < 16 * D / 4; e += THREADS) {
         const int col = e / (D / 4), piece = e % (D / 4);
@@ -743,13 +757,13 @@ kv4_split_kernel(const Args args) {
             *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top * a.zscale, sum};
         }
       }
-      if (cut && x.unit == 0 && tid == 0 && y == 0) {
+      if (cut && from == 0 && tid == 0 && y == 0) {
         // u is the share's end: the item's other units are the next ones'.
-        const int more = (int)((x.n - ub + share - 1) / share);
+        const int more = (int)((units - to + share - 1) / share);
         a.desc[blockIdx.x] = int4{more + 1, t.row0, t.col0, (last - t.col0 + 1) << 16 | x.hc};
       }
     }
-    if (u < u_end) __syncthreads();  // the next item fills the table again
+    if (u < u_end) lds_barrier();  // the next item fills the table again
   }
 }
 
@@ -915,7 +929,7 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
                       hipStream_t s) {
   const Plan p = make_plan(c, x.H, x.T, x.R, x.max_seq, x.cu_q != nullptr);
   const int G = (int)(x.H / c.heads);
-  const int64_t units = x.max_seq / (32 * p.waves) + 1;
+  const int64_t units = x.max_seq / (32 * p.waves) + 1 + kItem;
   if (p.wgs > INT32_MAX || x.T * G / 16 + x.R + 1 > INT32_MAX / units)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   Args a{(const uint16_t*)x.q.p, x.q.token_stride, x.q.head_stride,
