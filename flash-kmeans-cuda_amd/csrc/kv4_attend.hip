@@ -77,7 +77,7 @@ constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
                                            // a difference of two is no NaN
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
-constexpr int kItem = 3;                   // units that an item costs by itself
+constexpr int kItem = 3;                   // granules that an item costs by itself
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
 // Read by scalar loads: nothing writes it while the kernel runs.
@@ -105,7 +105,7 @@ struct Args {
   uint32_t num_blocks;
   int heads, H, G, T, R, max_seq, causal;
   int whole;          // one item per workgroup, else equal shares
-  int min_share;      // units a share has at least
+  int min_share;      // granules a share has at least
   int tiles_per_req;  // without cu_q
   float zscale;       // |sm_scale| * log2(e), above 0
   uint32_t qsign;     // flips the queries' signs where sm_scale is negative
@@ -157,7 +157,7 @@ __device__ inline bool find_tile(const Args& a, int tile, Tile& t) {
 
 // Tokens that query i of a request sees.
 __device__ inline int sees(const Args& a, const Tile& t, int i) {
-  return a.causal ? max(0, t.end - t.nq + 1 + i) : t.end;
+  return a.causal ? min(max(0, t.end - t.nq + 1 + i), t.end) : t.end;
 }
 
 // Tables of a head's level pairs, by the whole workgroup: thread tid writes
@@ -278,19 +278,22 @@ __device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
   return *(LdsWord)((LdsPtr)(uintptr_t)at + PART);
 }
 
-// Work of a launch, counted in units of UNIT tokens (one turn of all waves).
-// An item is a tile of a request under one cache head; each of a request's
-// tiles counts ceil(tokens / UNIT) units, at least one, and kItem more in
-// front of them for what an item costs by itself.  The items in order
-// (head, request, tile) are cut into equal shares, one per workgroup, wherever
-// the cuts fall: lengths of any mixture fill the chip evenly, a workgroup
-// meets few heads (whose tables it has to fill), and an item that is cut is
-// joined afterwards.
+// Work of a launch.  An item is a tile of a request under one cache head; it
+// weighs the tokens it sees, in granules of GR, and kItem granules more in
+// front for what an item costs by itself.  The items in order (head, request,
+// tile) are cut into equal shares, one per workgroup, wherever the cuts fall:
+// lengths of any mixture fill the chip evenly, a workgroup meets few heads
+// (whose tables it has to fill), and an item that is cut is joined afterwards.
+//
+// Tile j of a causal request sees about A + (j + 1) COLS / G tokens, A those in
+// front of its queries, so j tiles weigh a sum in closed form, from which a
+// tile is found again without a list of them.  (A weight only has to be the
+// same for everyone; what a share takes is in tokens.)
 struct Item {
   int hc;
   Tile t;
-  int n;   // units, with the kItem first ones
-  int at;  // first of them that is the share's
+  int n;   // its weight
+  int at;  // where the share begins in it
 };
 
 template <int COLS>
@@ -308,8 +311,16 @@ __device__ inline void request(const Args& a, int r, Tile& t, int& tiles) {
   tiles = (int)(((int64_t)t.nq * a.G + COLS - 1) / COLS);
 }
 
-// Running sums of the requests' units, THREADS slices of `per` requests.
-template <int COLS, int THREADS, int UNIT>
+// Weight of the first j tiles.
+template <int COLS, int GR>
+__device__ inline int weight(const Args& a, const Tile& t, int j) {
+  const int own = (a.causal ? max(t.end - t.nq, 0) : t.end) / GR + 1 + kItem;
+  if (!a.causal || j <= 1) return j * own;
+  return j * own + (int)((int64_t)COLS * j * (j + 1) / 2 / (a.G * GR));
+}
+
+// Running sums of the requests' weights, THREADS slices of `per` requests.
+template <int COLS, int THREADS, int GR>
 struct Shares {
   int* s_pre;  // LDS: THREADS + THREADS / 64 rounded to a multiple of 4, then
                // four numbers of each request where every thread has one
@@ -329,8 +340,8 @@ struct Shares {
       Tile t;
       int tiles;
       request<COLS>(a, r, t, tiles);
-      sum += tiles * (max((t.end + UNIT - 1) / UNIT, 1) + kItem);
-      if (per == 1) s_req()[r] = int4{t.row0, t.nq, t.end, 0};
+      sum += weight<COLS, GR>(a, t, tiles);
+      if (per == 1) s_req()[r] = int4{t.row0, t.nq, t.end, tiles};
     }
     const int incl = wave_incl_scan(sum);
     int* s_wave = s_pre + THREADS;
@@ -347,7 +358,7 @@ struct Shares {
     lds_barrier();
     total = __builtin_amdgcn_readfirstlane(total);
   }
-  // The item that unit u (below total) of a head's falls into.
+  // The item that place u (below total) of a head's falls into.
   __device__ inline Item find(const Args& a, int hc, int u) const {
     int j = -1;
 #pragma unroll
@@ -356,27 +367,115 @@ struct Shares {
     u -= __builtin_amdgcn_readfirstlane(s_pre[j]);
     Item x;
     x.hc = hc;
+    int tiles;
     if (per == 1) {
       const int4 q = s_req()[j];
       x.t.req = j;
-      x.t.row0 = q.x;
-      x.t.nq = q.y;
-      x.t.end = q.z;
-      x.n = max((x.t.end + UNIT - 1) / UNIT, 1) + kItem;
+      x.t.row0 = __builtin_amdgcn_readfirstlane(q.x);
+      x.t.nq = __builtin_amdgcn_readfirstlane(q.y);
+      x.t.end = __builtin_amdgcn_readfirstlane(q.z);
+      tiles = __builtin_amdgcn_readfirstlane(q.w);
     } else {
       for (int r = j * per;; ++r) {
-        int tiles;
         request<COLS>(a, r, x.t, tiles);
-        x.n = max((x.t.end + UNIT - 1) / UNIT, 1) + kItem;
-        if (u < tiles * x.n || r >= a.R) break;
-        u -= tiles * x.n;
+        const int w = weight<COLS, GR>(a, x.t, tiles);
+        if (u < w || r >= a.R) break;
+        u -= w;
       }
     }
-    const int tile = u / x.n;
-    x.at = u - tile * x.n;
+    int tile = 0;  // the last whose weights before it are u at most
+    for (int len = tiles; len > 1;) {
+      const int half = len >> 1;
+      if (weight<COLS, GR>(a, x.t, tile + half) <= u) tile += half;
+      len -= half;
+    }
+    const int w = weight<COLS, GR>(a, x.t, tile);
+    x.n = weight<COLS, GR>(a, x.t, tile + 1) - w;
+    x.at = u - w;
     x.t.col0 = tile * COLS;
     return x;
   }
+};
+
+__device__ inline int64_t scalar64(int64_t v) {
+  return (int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
+// A share as a workgroup walks through it, item by item.
+template <int COLS, int THREADS, int GR>
+struct Walk {
+  int64_t u = 0, u_end = 0, share = 1;  // places over all heads
+  int per_head = 1;
+  int* s_pre;
+  // The item at hand: its tokens from .. to of the lim that its last column
+  // sees are the share's; more: shares after this one that hold some of it.
+  Item x;
+  int from, to, lim, more;
+  __device__ inline Walk(const Args& a, int* lds) : s_pre(lds) {
+    const Shares<COLS, THREADS, GR> sh(a, lds);
+    per_head = sh.total;
+    const int64_t all = (int64_t)per_head * a.heads;
+    share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)a.min_share);
+    share = scalar64(share);
+    u = blockIdx.x * share;
+    u_end = scalar64(min(u + share, all));
+    if (threadIdx.x == 0) a.desc[blockIdx.x].x = 0;
+  }
+  __device__ inline bool next(const Args& a) {
+    while (u < u_end) {
+      const Shares<COLS, THREADS, GR> sh(
+          s_pre, (a.R + (a.cu_q != nullptr) + THREADS - 1) / THREADS, per_head);
+      const int hc = (int)(u / per_head);
+      x = sh.find(a, hc, (int)(u - (int64_t)hc * per_head));
+      // The same in every lane, which the compiler cannot see of loaded values.
+      auto scalar = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
+      scalar(x.t.req), scalar(x.t.row0), scalar(x.t.nq), scalar(x.t.end), scalar(x.t.col0);
+      scalar(x.n), scalar(x.at);
+      const int end = (int)min((int64_t)x.n, x.at + (u_end - u));
+      u += end - x.at;
+      const int last = min(x.t.col0 + COLS, x.t.nq * a.G) - 1;
+      lim = sees(a, x.t, (int)a.gdiv.div(last));
+      auto tokens = [&](int place) {
+        return place == x.n ? lim : (int)min((int64_t)max(place - kItem, 0) * GR, (int64_t)lim);
+      };
+      from = tokens(x.at);
+      to = tokens(end);
+      const int full = min(x.n, kItem + (lim + GR - 1) / GR);  // place where to is lim
+      more = (int)((max(full - end, 0) + share - 1) / share);
+      scalar(from), scalar(to), scalar(lim), scalar(more);
+      u = scalar64(u);
+      // The share may hold none of the item's tokens; of an item without any
+      // the last place stands for it.
+      if (from < to || (lim == 0 && end == x.n)) return true;
+    }
+    return false;
+  }
+  __device__ inline bool cut() const { return from > 0 || to < lim; }
+  // A share cuts the item before it and the one after it at most.
+  __device__ inline int64_t slot() const { return (int64_t)blockIdx.x * 2 + (from > 0 ? 0 : 1); }
+  // For the join, by one thread: a cut item that begins here.
+  __device__ inline void announce(const Args& a) const {
+    if (!cut() || from > 0) return;
+    const int cols = min(COLS, x.t.nq * a.G - x.t.col0);
+    a.desc[blockIdx.x] = int4{more + 1, x.t.row0, x.t.col0, cols << 16 | x.hc};
+  }
+  // One item per workgroup, no cuts, without the sums.
+  __device__ inline bool whole(const Args& a) {
+    // Heads first: consecutive workgroups go to the eight XCDs in turn, and
+    // every head has as much to do as the next.
+    const int tile = blockIdx.x / a.heads;
+    x.hc = blockIdx.x - tile * a.heads;
+    if (!find_tile<COLS>(a, tile, x.t)) return false;
+    auto scalar = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
+    scalar(x.t.req), scalar(x.t.row0), scalar(x.t.nq), scalar(x.t.end), scalar(x.t.col0);
+    const int last = min(x.t.col0 + COLS, x.t.nq * a.G) - 1;
+    from = 0;
+    to = lim = __builtin_amdgcn_readfirstlane(sees(a, x.t, (int)a.gdiv.div(last)));
+    more = 0;
+    return true;
+  }
+  __device__ inline explicit Walk(int* lds) : s_pre(lds) {}
 };
 
 // Keeps what a rarely taken branch computes inside it (selects in its place
@@ -405,20 +504,11 @@ kv4_split_kernel(const Args args) {
   int* s_pre = reinterpret_cast<int*>(lds + kTable + kJoin);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int64_t u = blockIdx.x, u_end = u + 1;  // of all heads' units
-  int64_t share = 1;
-  int per_head = 1, table = -1;  // units of a head; head whose table is in LDS
-  if (!args.whole) {
-    const Args& a = arguments();
-    const Shares<COLS, THREADS, UNIT> sh(a, s_pre);
-    per_head = sh.total;
-    const int64_t all = (int64_t)per_head * a.heads;
-    share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)a.min_share);
-    u = blockIdx.x * share;
-    u_end = min(u + share, all);
-    if (threadIdx.x == 0) a.desc[blockIdx.x].x = 0;
-  }
-  while (u < u_end) {
+  int table = -1;  // head whose table is in LDS
+  typedef Walk<COLS, THREADS, UNIT> W;
+  W k = args.whole ? W(s_pre) : W(arguments(), s_pre);
+  if (!(args.whole ? k.whole(arguments()) : k.next(arguments()))) return;
+  for (;;) {
     // Opaque, so that what derives from it is computed per item, not kept in
     // registers over the whole share.
     int tid = threadIdx.x;
@@ -426,40 +516,11 @@ kv4_split_kernel(const Args args) {
     const Args& a = arguments();
     const int lane = tid & 63, n = lane & 15, g = lane >> 4;
     const uint32_t loff = (uint32_t)(lane & 31) * 4;
-    Item x;
-    int units, from, to;  // of the item, and the share's of them
-    if (a.whole) {
-      // Heads first: consecutive workgroups go to the eight XCDs in turn, and
-      // every head has as much to do as the next.
-      const int tile = blockIdx.x / a.heads;
-      x.hc = blockIdx.x - tile * a.heads;
-      if (!find_tile<COLS>(a, tile, x.t)) return;
-      from = 0;
-      units = to = max((x.t.end + UNIT - 1) / UNIT, 1);
-      u = u_end;
-    } else {
-      Shares<COLS, THREADS, UNIT> sh(s_pre, (a.R + (a.cu_q != nullptr) + THREADS - 1) / THREADS,
-                                     per_head);
-      const int hc = (int)(u / per_head);
-      x = sh.find(a, hc, (int)(u - (int64_t)hc * per_head));
-      const int end = (int)min((int64_t)x.n, x.at + (u_end - u));
-      u += end - x.at;
-      from = max(x.at - kItem, 0);
-      to = max(end - kItem, 0);
-      units = x.n - kItem;
-      if (to == 0) break;  // the share ends before the item's units
-    }
-    // The same in every lane, which the compiler cannot see of loaded values.
-    auto scalar = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
-    Tile& t = x.t;
-    scalar(t.req), scalar(t.row0), scalar(t.nq), scalar(t.col0), scalar(t.end);
-    scalar(x.hc), scalar(units), scalar(from), scalar(to);
+    const Item& x = k.x;
+    const Tile& t = x.t;
     const int ncols = t.nq * a.G;
-    const int last = min(t.col0 + COLS, ncols) - 1;
-    const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0));
-    const int lim_max = sees(a, t, (int)a.gdiv.div(last));
-    const int t0 = from * UNIT;
-    const int t1 = min(to * UNIT, lim_max);
+    const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0)), lim_max = k.lim;
+    const int t0 = k.from, t1 = k.to;
     const int ntile = max(t1 - t0 + 31, 0) / 32;
     const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
 
@@ -547,13 +608,13 @@ kv4_split_kernel(const Args args) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
+        for (int c = 0; c < KS; ++c) {
           u32x4 kf;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) kf[b] = lookup<0>(cur.k[j][k], b, loff);
+          for (int b = 0; b < 4; ++b) kf[b] = lookup<0>(cur.k[j][c], b, loff);
 #pragma unroll
           for (int y = 0; y < NT; ++y)
-            s[y][j] = mfma<DT>(kf, qf[y][k], k ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+            s[y][j] = mfma<DT>(kf, qf[y][c], c ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
       if (more) load_keys<D>(a, nbase, lanes, cur);
       const int tok = t0 + it * 32 + 4 * g;  // token (j, i): tok + 16 j + i
@@ -724,9 +785,8 @@ kv4_split_kernel(const Args args) {
           }
       }
       lds_barrier();
-      const bool cut = from > 0 || to < units;
-      // A share cuts the item before it and the one after it at most.
-      const int64_t slot = (int64_t)blockIdx.x * 2 + (from > 0 ? 0 : 1);
+      const bool cut = k.cut();
+      const int64_t slot = k.slot();
 #pragma unroll 1
       for (int e = tid; e < 16 * D / 4; e += THREADS) {
         const int col = e / (D / 4), piece = e % (D / 4);
@@ -757,13 +817,11 @@ kv4_split_kernel(const Args args) {
             *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top * a.zscale, sum};
         }
       }
-      if (cut && from == 0 && tid == 0 && y == 0) {
-        // u is the share's end: the item's other units are the next ones'.
-        const int more = (int)((units - to + share - 1) / share);
-        a.desc[blockIdx.x] = int4{more + 1, t.row0, t.col0, (last - t.col0 + 1) << 16 | x.hc};
-      }
     }
-    if (u < u_end) lds_barrier();  // the next item fills the table again
+    if (args.whole) return;
+    if (tid == 0) k.announce(arguments());
+    if (!k.next(arguments())) return;
+    lds_barrier();  // the next item fills the table again
   }
 }
 
