@@ -80,6 +80,12 @@ constexpr int kTable = 256 * kEntry;
 constexpr int kItem = 3;                   // granules that an item costs by itself
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
+// log(2^m l): the exponents of both are added before anything is rounded.
+__device__ inline float log_sum(float m, float l) {
+  const int e = (int)(__float_as_uint(l) >> 23) - 127;
+  return l > 0.f ? (m + e) * kLn2 + __logf(ldexpf(l, -e)) : -INFINITY;
+}
+
 // Read by scalar loads: nothing writes it while the kernel runs.
 typedef const int32_t __attribute__((address_space(4))) * Const32;
 
@@ -482,9 +488,6 @@ struct Walk {
 // would run for every tile).
 __device__ inline void rare(float& v) { asm volatile("" : "+v"(v)); }
 
-// The split form: the WAVES waves of a workgroup share NT tiles of 16 columns
-// and take 32 tokens in turn, each with its own running maximum and sum; they
-// are joined in LDS at the end of an item, cut items by a second kernel.
 // The kernel's (only) argument, read again from where it lies: what is not used
 // between two such places takes no registers there.
 __device__ inline const Args& arguments() {
@@ -493,10 +496,18 @@ __device__ inline const Args& arguments() {
   return *(const Args*)p;
 }
 
-template <int DT, int D, int NT, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, WAVES * (NT * D > 256 ? 1 : 2) / 4)
-kv4_split_kernel(const Args args) {
-  constexpr int COLS = 16 * NT, THREADS = WAVES * 64, UNIT = WAVES * 32;
+// Two forms, over 32 tokens and NT column tiles per wave at a time, each wave
+// with its own running maxima and sums:
+//   split  the waves of a workgroup share the tiles and take the tokens in
+//          turn; they are joined in LDS at the end of an item
+//   wide   (prompts) every wave has tiles of its own and goes over all tokens
+// Items that the shares cut are joined by a second kernel.
+template <int DT, int D, int NT, int WAVES, bool WIDE>
+__global__ void __launch_bounds__(WAVES * 64, WIDE ? WAVES / 4
+                                                   : WAVES * (NT * D > 256 ? 1 : 2) / 4)
+kv4_attend_kernel(const Args args) {
+  constexpr int COLS = 16 * NT * (WIDE ? WAVES : 1), THREADS = WAVES * 64;
+  constexpr int STRIDE = WIDE ? 1 : WAVES, UNIT = STRIDE * 32;
   constexpr int KS = D / 32;  // steps of the first product
   constexpr int ND = D / 16;  // feature tiles of the second
   extern __shared__ __align__(16) char lds[];
@@ -519,8 +530,14 @@ kv4_split_kernel(const Args args) {
     const Item& x = k.x;
     const Tile& t = x.t;
     const int ncols = t.nq * a.G;
-    const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0)), lim_max = k.lim;
-    const int t0 = k.from, t1 = k.to;
+    // The wave's columns, counted in the request, and what the first and the
+    // last of them see.
+    const int col0 = t.col0 + (WIDE ? wave * 16 * NT : 0);
+    const int lim_min = sees(a, t, (int)a.gdiv.div(min(col0, ncols - 1)));
+    const int lim_max =
+        !WIDE ? k.lim
+              : col0 < ncols ? sees(a, t, (int)a.gdiv.div(min(col0 + 16 * NT, ncols) - 1)) : 0;
+    const int t0 = k.from, t1 = WIDE ? min(k.to, lim_max) : k.to;
     const int ntile = max(t1 - t0 + 31, 0) / 32;
     const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
 
@@ -543,12 +560,13 @@ kv4_split_kernel(const Args args) {
                                    : -1;
       }
     };
+    const int first = WIDE ? 0 : wave;
     int blk[2], base[2], nbase[2];
-    load_blocks(wave, blk);
+    load_blocks(first, blk);
 
-    // Query and head of a column of the tile; row -1 past the last.
+    // Query and head of a column of the wave's; row -1 past the last.
     auto column = [&](const Args& a, int col, int& row, int& head, int& i) {
-      col += t.col0;
+      col += col0;
       i = (int)a.gdiv.div(min(col, ncols - 1));
       row = col < ncols ? t.row0 + i : -1;
       head = x.hc * a.G + (min(col, ncols - 1) - i * a.G);
@@ -569,20 +587,26 @@ kv4_split_kernel(const Args args) {
     }
     const Lane<D> lanes(n, g);
     Codes<D> cur;
-    groups(wave, blk, base);
-    if (wave < ntile) {
+    groups(first, blk, base);
+    if (first < ntile) {
       load_keys<D>(a, base, lanes, cur);
       load_scales<D>(a, base, lanes, cur);
       load_values<D>(a, base, lanes, cur);
     }
-    load_blocks(wave + WAVES, blk);
-    if (table != x.hc) {
+    load_blocks(first + STRIDE, blk);
+    if (!WIDE || table != x.hc) {
+      if (WIDE && table >= 0) lds_barrier();  // its last look-ups are done
       table = x.hc;
       fill_table<THREADS>(a, x.hc, lds, tid);
+      lds_barrier();
     }
-    lds_barrier();
 
-    // Maxima are of q k before the (positive) score scale.
+    // bf16: m is the largest score before its (positive) scale zscale, and a
+    // weight is 2^(z zscale - m zscale).  fp16 has few exponents, and a token's
+    // value scale is part of what is rounded to it: m is the largest z zscale +
+    // log2 of the value scale (rounded up), and a weight 2^(z zscale - m + 14),
+    // so that weight times scale is at most 2^14 and the column's largest above
+    // 2^12, whatever the scales are.
     float m[NT], l[NT];
     f32x4 o[NT][ND];
 #pragma unroll
@@ -592,17 +616,16 @@ kv4_split_kernel(const Args args) {
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[y][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    // fp16 weights are kept within the type's range whatever the scales are:
-    // times 2^14 over a power of two that no scale so far exceeds.
-    float vref = 0.f, vmul = 1.f;
+    // What the weights so far are relative to, as a power of two.
+    auto base2 = [](float m, float zscale) { return DT == FKC_F16 ? m - 14.f : m * zscale; };
 
     // What a tile has used up is fetched for the next one at once, into the
     // same registers: with a second set of them four waves a SIMD do not fit,
     // and it is they that hide the loads' latency.
-    for (int it = wave; it < ntile; it += WAVES) {
-      const bool more = it + WAVES < ntile;
-      groups(it + WAVES, blk, nbase);
-      load_blocks(it + 2 * WAVES, blk);
+    for (int it = first; it < ntile; it += STRIDE) {
+      const bool more = it + STRIDE < ntile;
+      groups(it + STRIDE, blk, nbase);
+      load_blocks(it + 2 * STRIDE, blk);
 
       f32x4 s[NT][2];
 #pragma unroll
@@ -639,38 +662,13 @@ kv4_split_kernel(const Args args) {
             rare(vs[j][i]);
           }
       }
+      float ve[2][4];  // fp16: the value scales' exponents; zero counts as 2^-60
       if constexpr (DT == FKC_F16) {
-        float top = 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(vs[j][i]));
-        if (__any(top > vref)) {
-          top = 0.f;  // of the finite ones; the others are what they are
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              top = fmaxf(top, fabsf(vs[j][i]) < INFINITY ? fabsf(vs[j][i]) : 0.f);
-#pragma unroll
-          for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-          if (top > vref) {
-            // next power of two: times 2^14 over it stays in range
-            const float ref = __uint_as_float((__float_as_uint(top) + 0x7fffffu) & 0x7f800000u);
-            const float mul = 16384.f / ref;
-            const float f = vref > 0.f ? mul / vmul : 0.f;  // nothing yet: o is 0
-            vref = ref;
-            vmul = mul;
-#pragma unroll
-            for (int y = 0; y < NT; ++y)
-#pragma unroll
-              for (int d = 0; d < ND; ++d) o[y][d] *= f;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vs[j][i] *= vmul;
+          for (int i = 0; i < 4; ++i)
+            ve[j][i] = fmaxf((float)(int)(__float_as_uint(fabsf(vs[j][i])) >> 23) - 126.f, -60.f);
       }
       u32x4 pf[NT];
 #pragma unroll
@@ -692,18 +690,21 @@ kv4_split_kernel(const Args args) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = fmaxf(top, z[j][i]);
+          for (int i = 0; i < 4; ++i)
+            top = fmaxf(top, DT == FKC_F16 ? __builtin_fmaf(z[j][i], a.zscale, ve[j][i])
+                                           : z[j][i]);
         if (__any(top > m[y])) {
           top = fmaxf(top, __shfl_xor(top, 16, 64));
           top = fmaxf(top, __shfl_xor(top, 32, 64));
           const float nm = fmaxf(m[y], top);
-          const float f = __builtin_amdgcn_exp2f((m[y] - nm) * a.zscale);
+          const float f = __builtin_amdgcn_exp2f(
+              DT == FKC_F16 ? m[y] - nm : (m[y] - nm) * a.zscale);
           m[y] = nm;
           l[y] *= f;
 #pragma unroll
           for (int d = 0; d < ND; ++d) o[y][d] *= f;
         }
-        const float mz = m[y] * a.zscale;
+        const float mz = base2(m[y], a.zscale);
         float w[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -754,24 +755,68 @@ kv4_split_kernel(const Args args) {
       base[1] = nbase[1];
     }
 
-    // Join the lanes of a column (they share m), then the waves that had
-    // tokens: their outputs, relative to the largest maximum, go to LDS as
-    // rows of features (over the table, 16-byte pieces turned by the column
-    // so that no two lanes meet in a bank) and are summed as they are written.
-    const int waves = min(ntile, WAVES);
-    table = -1;
+    // Join the lanes of a column (they share m).
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
       l[y] += __shfl_xor(l[y], 16, 64);
       l[y] += __shfl_xor(l[y], 32, 64);
+    }
+    if constexpr (WIDE) {
+      const Args& a = arguments();
+#pragma unroll
+      for (int y = 0; y < NT; ++y) {
+        int row, head, i;
+        column(a, 16 * y + n, row, head, i);
+        if (row < 0) continue;
+        if (!k.cut()) {
+          const float f = l[y] > 0.f ? 1.f / l[y] : 0.f;
+          const int64_t at = (int64_t)row * a.H + head;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[ND / 2];
+#pragma unroll
+            for (int d = 0; d < ND / 2; ++d)
+              w[d] = pack2<DT>(o[y][2 * d][i] * f, o[y][2 * d + 1][i] * f);
+            uint32_t* op = reinterpret_cast<uint32_t*>(a.out + at * D + (4 * g + i) * ND);
+#pragma unroll
+            for (int d = 0; d < ND / 2; ++d) op[d] = w[d];
+          }
+          if (g == 0 && a.lse != nullptr)
+            a.lse[at] = log_sum(base2(m[y], a.zscale), l[y]);
+        } else {
+          const int64_t at = k.slot() * COLS + wave * 16 * NT + 16 * y + n;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < ND / 4; ++d)
+              *reinterpret_cast<f32x4*>(a.part + at * D + (4 * g + i) * ND + 4 * d) =
+                  f32x4{o[y][4 * d][i], o[y][4 * d + 1][i], o[y][4 * d + 2][i],
+                        o[y][4 * d + 3][i]};
+          if (g == 0)
+            *reinterpret_cast<float2*>(a.part_ml + 2 * at) =
+                float2{base2(m[y], a.zscale), l[y]};
+        }
+      }
+      if (args.whole) return;
+      if (tid == 0) k.announce(arguments());
+      if (!k.next(arguments())) return;
+      continue;
+    }
+    // Join the waves that had tokens: their outputs, relative to the largest
+    // maximum, go to LDS as rows of features (over the table, 16-byte pieces
+    // turned by the column so that no two lanes meet in a bank) and are summed
+    // as they are written.
+    const int waves = min(ntile, WAVES);
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
       if (y) lds_barrier();  // the last tile's pieces are read
-      if (g == 0) sml[wave * 16 + n] = float2{m[y], l[y]};
+      const float rel = base2(m[y], a.zscale);
+      if (g == 0) sml[wave * 16 + n] = float2{rel, l[y]};
       lds_barrier();
       const Args& a = arguments();
       float top = kLowest;
       for (int w = 0; w < waves; ++w) top = fmaxf(top, sml[w * 16 + n].x);
-      const float f = __builtin_amdgcn_exp2f((m[y] - top) * a.zscale) *
-                      (DT == FKC_F16 ? 1.f / vmul : 1.f);
+      const float f = __builtin_amdgcn_exp2f(rel - top);
       f32x4* so = reinterpret_cast<f32x4*>(lds);
       if (wave < waves) {
 #pragma unroll
@@ -798,7 +843,7 @@ kv4_split_kernel(const Args args) {
         for (int w = 0; w < waves; ++w) top = fmaxf(top, sml[w * 16 + col].x);
         for (int w = 0; w < waves; ++w) {
           const float2 ml = sml[w * 16 + col];
-          sum += ml.y * __builtin_amdgcn_exp2f((ml.x - top) * a.zscale);
+          sum += ml.y * __builtin_amdgcn_exp2f(ml.x - top);
           v += so[(w * 16 + col) * (D / 4) + (piece ^ col)];
         }
         const int64_t at = (int64_t)row * a.H + head;
@@ -809,12 +854,12 @@ kv4_split_kernel(const Args args) {
           w.y = pack2<DT>(v[2] * f, v[3] * f);
           *reinterpret_cast<uint2*>(a.out + at * D + 4 * piece) = w;
           if (piece == 0 && a.lse != nullptr)
-            a.lse[at] = sum > 0.f ? top * a.zscale * kLn2 + __logf(sum) : -INFINITY;
+            a.lse[at] = log_sum(top, sum);
         } else {
           const int64_t at = slot * COLS + 16 * y + col;
           *reinterpret_cast<f32x4*>(a.part + at * D + 4 * piece) = v;
           if (piece == 0)
-            *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top * a.zscale, sum};
+            *reinterpret_cast<float2*>(a.part_ml + 2 * at) = float2{top, sum};
         }
       }
     }
@@ -826,90 +871,124 @@ kv4_split_kernel(const Args args) {
 }
 
 // Joins the parts of a cut item: the workgroup's that its first unit was in
-// (its second slot) and the following ones' (their first).  A workgroup per
-// four columns: their weights into LDS, PARTS parts at a time, then D / 4
-// lanes per part, every load independent of the others.
+// (its second slot) and the following ones' (their first).  D / 4 lanes per
+// column; of few parts each thread adds its own up, of many all threads share
+// the parts of JC columns: weights into LDS, PARTS parts at a time, every load
+// independent of the others.
+template <int DT, int D>
+__device__ inline void write_joined(const Args& a, const int4& item, int col, int sub, f32x4 v,
+                                    float m, float l) {
+  const int i = (int)a.gdiv.div(item.z + col);
+  const int64_t at =
+      (int64_t)(item.y + i) * a.H + (item.w & 0xffff) * a.G + (item.z + col - i * a.G);
+  const float f = l > 0.f ? 1.f / l : 0.f;
+  uint2 w;
+  w.x = pack2<DT>(v[0] * f, v[1] * f);
+  w.y = pack2<DT>(v[2] * f, v[3] * f);
+  *reinterpret_cast<uint2*>(a.out + at * D + 4 * sub) = w;
+  if (sub == 0 && a.lse != nullptr) a.lse[at] = log_sum(m, l);
+}
+
 template <int DT, int D, int COLS>
 __global__ void __launch_bounds__(256)
 kv4_join_kernel(const Args a) {
-  constexpr int LPC = D / 4, CP = 256 / LPC, JC = 4, PARTS = 64;
+  constexpr int LPC = D / 4, CP = 256 / LPC, JC = 4, PARTS = 64, FEW = 4;
   __shared__ f32x4 so[256];
   __shared__ float sw[JC][PARTS];
   const int4 item = a.desc[blockIdx.x];
   if (item.x == 0) return;
-  const int ncols = item.w >> 16, hc = item.w & 0xffff, col0 = blockIdx.y * JC;
-  if (col0 >= ncols) return;
+  const int ncols = item.w >> 16;
   const int sub = threadIdx.x % LPC, part = threadIdx.x / LPC;
-  // row of part c, column col0 + j in part and part_ml
-  auto place = [&](int c, int j) {
-    return (((int64_t)blockIdx.x + c) * 2 + (c ? 0 : 1)) * COLS + min(col0 + j, COLS - 1);
+  // row of part c, column col in part and part_ml
+  auto place = [&](int c, int col) {
+    return (((int64_t)blockIdx.x + c) * 2 + (c ? 0 : 1)) * COLS + min(col, COLS - 1);
   };
+  if (item.x <= FEW) {
+    for (int col = blockIdx.y * CP + part; col < ncols; col += gridDim.y * CP) {
+      f32x4 v[FEW];
+      float2 ml[FEW];
+      float m = kLowest, l = 0.f;
+#pragma unroll
+      for (int c = 0; c < FEW; ++c) {
+        if (c >= item.x) break;
+        ml[c] = *reinterpret_cast<const float2*>(a.part_ml + 2 * place(c, col));
+        v[c] = *reinterpret_cast<const f32x4*>(a.part + place(c, col) * D + 4 * sub);
+      }
+#pragma unroll
+      for (int c = 0; c < FEW; ++c)
+        if (c < item.x) m = fmaxf(m, ml[c].x);
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < FEW; ++c) {
+        if (c >= item.x) break;
+        const float w = __builtin_amdgcn_exp2f(ml[c].x - m);
+        l += ml[c].y * w;
+        o += v[c] * w;
+      }
+      write_joined<DT, D>(a, item, col, sub, o, m, l);
+    }
+    return;
+  }
   // One wave per column: a lane per part.
   const int j = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float m = kLowest, l = 0.f;
-  f32x4 o[JC];
+  for (int col0 = blockIdx.y * JC; col0 < ncols; col0 += gridDim.y * JC) {
+    float m = kLowest, l = 0.f;
+    f32x4 o[JC];
 #pragma unroll
-  for (int x = 0; x < JC; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int c0 = 0; c0 < item.x; c0 += PARTS) {
-    f32x4 v[JC][PARTS / CP];
+    for (int x = 0; x < JC; ++x) o[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = 0; c0 < item.x; c0 += PARTS) {
+      f32x4 v[JC][PARTS / CP];
 #pragma unroll
-    for (int i = 0; i < PARTS / CP; ++i)
+      for (int i = 0; i < PARTS / CP; ++i)
+#pragma unroll
+        for (int x = 0; x < JC; ++x)
+          if (c0 + i * CP < item.x)
+            v[x][i] = *reinterpret_cast<const f32x4*>(
+                a.part + place(min(c0 + i * CP + part, item.x - 1), col0 + x) * D + 4 * sub);
+      float m2 = kLowest, l2 = 0.f;
+      if (c0 + lane < item.x) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * place(c0 + lane, col0 + j));
+        m2 = ml.x;
+        l2 = ml.y;
+      }
+      float nm = fmaxf(m, m2);
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) nm = fmaxf(nm, __shfl_xor(nm, off, 64));
+      const float f = __builtin_amdgcn_exp2f(m - nm), w = __builtin_amdgcn_exp2f(m2 - nm);
+      m = nm;
+      l = l * f + wave_sum(l2 * w);
+      __syncthreads();  // sw is read
+      sw[j][lane] = c0 + lane < item.x ? w : 0.f;
+      if (lane == 0) reinterpret_cast<float*>(so)[j] = f;
+      __syncthreads();
 #pragma unroll
       for (int x = 0; x < JC; ++x) {
-        const int c = min(c0 + i * CP + part, item.x - 1);
-        v[x][i] = *reinterpret_cast<const f32x4*>(a.part + place(c, x) * D + 4 * sub);
-      }
-    float m2 = kLowest, l2 = 0.f;
-    if (c0 + lane < item.x) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * place(c0 + lane, j));
-      m2 = ml.x;
-      l2 = ml.y;
-    }
-    float nm = fmaxf(m, m2);
+        o[x] *= reinterpret_cast<const float*>(so)[x];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) nm = fmaxf(nm, __shfl_xor(nm, off, 64));
-    const float f = __builtin_amdgcn_exp2f(m - nm), w = __builtin_amdgcn_exp2f(m2 - nm);
-    m = nm;
-    l = l * f + wave_sum(l2 * w);
-    __syncthreads();  // sw is read
-    sw[j][lane] = c0 + lane < item.x ? w : 0.f;
-    if (lane == 0) reinterpret_cast<float*>(so)[j] = f;
+        for (int i = 0; i < PARTS / CP; ++i) {
+          const float wt = sw[x][i * CP + part];
+          // (the column or part may not exist; what stands there may be NaN)
+          if (wt != 0.f) o[x] += v[x][i] * wt;
+        }
+      }
+    }
     __syncthreads();
+    if (lane == 0) {
+      sw[j][0] = l;
+      sw[j][1] = m;
+    }
 #pragma unroll
     for (int x = 0; x < JC; ++x) {
-      o[x] *= reinterpret_cast<const float*>(so)[x];
+      __syncthreads();
+      so[threadIdx.x] = o[x];
+      __syncthreads();
+      if (threadIdx.x >= LPC || col0 + x >= ncols) continue;
+      f32x4 sum = so[sub];
 #pragma unroll
-      for (int i = 0; i < PARTS / CP; ++i) {
-        const float wt = sw[x][i * CP + part];
-        // (the column or part may not exist; what stands there may be NaN)
-        o[x] += wt != 0.f ? v[x][i] * wt : f32x4{0.f, 0.f, 0.f, 0.f};
-      }
+      for (int c = 1; c < CP; ++c) sum += so[c * LPC + sub];
+      write_joined<DT, D>(a, item, col0 + x, sub, sum, sw[x][1], sw[x][0]);
     }
-  }
-  __syncthreads();
-  if (lane == 0) {
-    sw[j][0] = l;
-    sw[j][1] = m;
-  }
-#pragma unroll
-  for (int x = 0; x < JC; ++x) {
     __syncthreads();
-    so[threadIdx.x] = o[x];
-    __syncthreads();
-    const int col = col0 + x;
-    if (threadIdx.x >= LPC || col >= ncols) continue;
-    f32x4 sum = so[sub];
-#pragma unroll
-    for (int c = 1; c < CP; ++c) sum += so[c * LPC + sub];
-    const int i = (int)a.gdiv.div(item.z + col);
-    const int64_t at = (int64_t)(item.y + i) * a.H + hc * a.G + (item.z + col - i * a.G);
-    const float den = sw[x][0], f = den > 0.f ? 1.f / den : 0.f;
-    uint2 w;
-    w.x = pack2<DT>(sum[0] * f, sum[1] * f);
-    w.y = pack2<DT>(sum[2] * f, sum[3] * f);
-    *reinterpret_cast<uint2*>(a.out + at * D + 4 * sub) = w;
-    if (sub == 0 && a.lse != nullptr)
-      a.lse[at] = den > 0.f ? sw[x][1] * kLn2 + __logf(den) : -INFINITY;
   }
 }
 
@@ -929,44 +1008,54 @@ int by_shape(int dtype, int64_t D, F&& f) {
 constexpr int kMinShare = 4;
 
 struct Plan {
-  int nt;             // column tiles per workgroup
+  bool wide;
+  int nt;             // column tiles per wave
   int waves;
   bool whole;         // one item per workgroup
   int64_t wgs;
   int tiles_per_req;  // without cu_q
-  size_t part_rows() const { return (size_t)wgs * 2 * 16 * nt; }
+  int cols() const { return 16 * nt * (wide ? waves : 1); }
+  size_t part_rows() const { return (size_t)wgs * 2 * cols(); }
 };
+
+constexpr int kWide = 8;  // waves of the wide form
+constexpr int wide_tiles(int D) { return D == 256 ? 1 : 2; }
+constexpr int waves_of(int D) { return D == 256 ? 4 : 8; }
 
 Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t max_seq,
                bool ragged) {
   Plan p;
   const int64_t G = H / c.heads;
-  // Column tiles: as many as an average request fills, up to two.
-  p.nt = R > 0 && T * G > 16 * R ? 2 : 1;
-  p.waves = p.nt == 2 || c.D == 256 ? 4 : 8;
-  const int64_t cols = 16 * p.nt;
+  // Column tiles: as many as an average request fills; waves with columns of
+  // their own from 96 columns on.
+  const int64_t avg = R > 0 ? T * G / R : 0;
+  p.wide = avg > 96;
+  p.nt = p.wide ? wide_tiles((int)c.D) : avg > 16 ? 2 : 1;
+  p.waves = p.wide ? kWide : p.nt > 1 ? 4 : waves_of((int)c.D);
+  const int64_t cols = p.cols();
   p.tiles_per_req = (int)((G + cols - 1) / cols);
   const int64_t tiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
   // Contexts that no share would be smaller than are not cut.
   p.whole = max_seq <= kMinShare * 32 * p.waves;
-  p.wgs = p.whole ? tiles * c.heads : 2 * (int64_t)device_shape().cus;
+  p.wgs = p.whole ? tiles * c.heads : (p.wide ? 1 : 2) * (int64_t)device_shape().cus;
   return p;
 }
 
-template <int DT, int D, int NT, int WAVES>
-int launch_split(const Args& a, const Plan& p, hipStream_t s) {
-  const int bytes = kTable + kJoin + Shares<16 * NT, WAVES * 64, WAVES * 32>::kInts * 4;
-  auto* kernel = &kv4_split_kernel<DT, D, NT, WAVES>;
+template <int DT, int D, int NT, int WAVES, bool WIDE>
+int launch(const Args& a, const Plan& p, hipStream_t s) {
+  constexpr int COLS = 16 * NT * (WIDE ? WAVES : 1);
+  const int bytes = kTable + kJoin + Shares<COLS, WAVES * 64, 1>::kInts * 4;
+  auto* kernel = &kv4_attend_kernel<DT, D, NT, WAVES, WIDE>;
   if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                           hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
     return fail(FKC_ERR_LAUNCH, "kv4_attend: %d bytes of LDS refused", bytes);
-  hipLaunchKernelGGL((kv4_split_kernel<DT, D, NT, WAVES>), dim3((uint32_t)p.wgs),
-                     dim3(WAVES * 64), bytes, s, a);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)p.wgs), dim3(WAVES * 64), bytes, s, a);
   if (int rc = check_launch("kv4_attend")) return rc;
   if (p.whole) return FKC_OK;
-  const int64_t cols = std::min<int64_t>(16 * NT, a.cu_q ? 16 * NT : a.G);
-  hipLaunchKernelGGL((kv4_join_kernel<DT, D, 16 * NT>),
-                     dim3((uint32_t)p.wgs, (uint32_t)((cols + 3) / 4)), dim3(256), 0, s, a);
+  const int64_t cols = std::min<int64_t>(COLS, a.cu_q ? COLS : a.G);
+  hipLaunchKernelGGL((kv4_join_kernel<DT, D, COLS>),
+                     dim3((uint32_t)p.wgs, (uint32_t)std::min<int64_t>((cols + 3) / 4, 16)),
+                     dim3(256), 0, s, a);
   return check_launch("kv4_attend (join)");
 }
 
@@ -987,8 +1076,9 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
                       hipStream_t s) {
   const Plan p = make_plan(c, x.H, x.T, x.R, x.max_seq, x.cu_q != nullptr);
   const int G = (int)(x.H / c.heads);
-  const int64_t units = x.max_seq / (32 * p.waves) + 1 + kItem;
-  if (p.wgs > INT32_MAX || x.T * G / 16 + x.R + 1 > INT32_MAX / units)
+  // Weights of a head's items are summed in 32 bits.
+  const int64_t most = x.max_seq / (p.wide ? 32 : 32 * p.waves) + 2 + kItem;
+  if (p.wgs > INT32_MAX || x.T * G / p.cols() + x.R + 1 > INT32_MAX / most)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   Args a{(const uint16_t*)x.q.p, x.q.token_stride, x.q.head_stride,
          (const uint8_t*)c.k_codes, (const uint8_t*)c.v_codes,
@@ -1009,8 +1099,9 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
   }
   return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     constexpr int DT = dt.value, DD = d.value;
-    return p.nt == 1 ? launch_split<DT, DD, 1, DD == 256 ? 4 : 8>(a, p, s)
-                     : launch_split<DT, DD, 2, 4>(a, p, s);
+    if (p.wide) return launch<DT, DD, wide_tiles(DD), kWide, true>(a, p, s);
+    return p.nt == 1 ? launch<DT, DD, 1, waves_of(DD), false>(a, p, s)
+                     : launch<DT, DD, 2, 4, false>(a, p, s);
   });
 }
 
