@@ -21,6 +21,7 @@
 // The products are then of levels, exact in 16 bits.  A token's scales stay
 // outside: the key's multiplies the score, the value's the weight.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -1046,9 +1047,17 @@ int launch(const Args& a, const Plan& p, hipStream_t s) {
   constexpr int COLS = 16 * NT * (WIDE ? WAVES : 1);
   const int bytes = kTable + kJoin + Shares<COLS, WAVES * 64, 1>::kInts * 4;
   auto* kernel = &kv4_attend_kernel<DT, D, NT, WAVES, WIDE>;
-  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                          hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
-    return fail(FKC_ERR_LAUNCH, "kv4_attend: %d bytes of LDS refused", bytes);
+  // The attribute stays with the kernel: once per device is enough.
+  static std::atomic<uint64_t> set{0};
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess) dev = -1;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if ((set.load(std::memory_order_relaxed) & bit) == 0) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                            hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+      return fail(FKC_ERR_LAUNCH, "kv4_attend: %d bytes of LDS refused", bytes);
+    set.fetch_or(bit, std::memory_order_relaxed);
+  }
   hipLaunchKernelGGL(kernel, dim3((uint32_t)p.wgs), dim3(WAVES * 64), bytes, s, a);
   if (int rc = check_launch("kv4_attend")) return rc;
   if (p.whole) return FKC_OK;

@@ -43,19 +43,37 @@ def _on_gpu(name: str, t: torch.Tensor, device: Optional[torch.device] = None) -
         raise RuntimeError(f"{name} must be on {device}, found on {t.device}")
 
 
+# Decoding calls these functions for a few microseconds of GPU work: what usually
+# holds is tested first, in one expression, and explained only if it does not.
+
 def _i32(name: str, t: torch.Tensor, dim: int, device: torch.device) -> torch.Tensor:
+    if (t.dtype is torch.int32 and t.dim() == dim and t.get_device() == device.index
+            and t.is_contiguous()):
+        return t
     _on_gpu(name, t, device)
     if t.dtype != torch.int32 or t.dim() != dim:
         raise RuntimeError(f"{name} must be int32 with {dim} dimension(s)")
-    return t if t.is_contiguous() else t.contiguous()
+    return t.contiguous()
+
+
+def _check_tables(t: torch.Tensor, R: int, device: torch.device) -> Tuple[int, int]:
+    """(max_blocks, row stride) of tables (R, max_blocks) int32 with dense rows."""
+    if t.get_device() != device.index:
+        _on_gpu("tables", t, device)
+    _require(t.dtype is torch.int32 and t.dim() == 2, "tables must be int32 (R, max_blocks)")
+    rows, width = t.shape
+    stride, dense = t.stride()
+    _require(rows == R and (width <= 1 or dense == 1),
+             f"tables must be ({R}, max_blocks) with dense rows")
+    return width, stride if rows > 1 else width
 
 
 def _rows(name: str, t: torch.Tensor, heads: int, cache: "Cache") -> torch.Tensor:
     """(T, heads, D) rows of the cache's dtype that the kernels can load 16
     bytes at a time; any token and head stride (a slice of a fused projection)
     that keeps them aligned, otherwise a dense copy."""
-    _on_gpu(name, t, cache.device)
-    if t.dtype != cache.dtype:
+    if t.dtype is not cache.dtype or t.get_device() != cache.index:
+        _on_gpu(name, t, cache.device)
         raise RuntimeError(f"{name} must have the cache's dtype {cache.dtype}")
     if t.dim() != 3 or (heads and t.shape[1] != heads) or t.shape[2] != cache.head_dim:
         raise RuntimeError(f"{name} must be (T, {heads or 'H'}, {cache.head_dim})")
@@ -89,6 +107,7 @@ class Cache:
                  v_scales: torch.Tensor, k_levels: torch.Tensor, v_levels: torch.Tensor) -> None:
         _on_gpu("k_codes", k_codes)
         self.device = k_codes.device
+        self.index = self.device.index
         self.dtype = k_scales.dtype
         _require(self.dtype in (torch.float16, torch.bfloat16),
                  f"the cache's dtype must be fp16 or bf16, not {self.dtype}")
@@ -164,27 +183,24 @@ def block_tables(seq_lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.T
     free_blocks does not reach (taken is then more than it holds) and the
     slots past max_blocks.
     """
-    _on_gpu("seq_lens", seq_lens)
     dev = seq_lens.device
+    if dev.type != "cuda":
+        _on_gpu("seq_lens", seq_lens)
     seq_lens = _i32("seq_lens", seq_lens, 1, dev)
     new_lens = _i32("new_lens", new_lens, 1, dev)
     free_blocks = _i32("free_blocks", free_blocks, 1, dev)
-    _on_gpu("tables", tables, dev)
     R = seq_lens.shape[0]
     _require(new_lens.shape[0] == R, "new_lens must be as long as seq_lens")
-    _require(tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == R
-             and (tables.shape[1] <= 1 or tables.stride(1) == 1),
-             "tables must be int32 (R, max_blocks) with dense rows")
+    width, stride = _check_tables(tables, R, dev)
     _require(num_tokens >= 0, "num_tokens must not be negative")
-    width = tables.shape[1]
-    buf = torch.empty(num_tokens + R + 2, dtype=torch.int32, device=dev)
-    slots, cu_new, taken = buf.split((num_tokens, R + 1, 1))
+    slots, cu_new, taken = torch.split_with_sizes(seq_lens.new_empty(num_tokens + R + 2),
+                                                  (num_tokens, R + 1, 1))
     with _lib.on_device(seq_lens):
         _lib.check(_lib.lib.fkc_block_tables(
-            seq_lens.data_ptr(), new_lens.data_ptr(), R, tables.data_ptr(),
-            tables.stride(0) if R > 1 else width, width, free_blocks.data_ptr(),
-            free_blocks.shape[0], block_size, num_tokens, slots.data_ptr(), cu_new.data_ptr(),
-            taken.data_ptr(), _lib.stream_of(seq_lens)), "block_tables")
+            seq_lens.data_ptr(), new_lens.data_ptr(), R, tables.data_ptr(), stride, width,
+            free_blocks.data_ptr(), free_blocks.shape[0], block_size, num_tokens,
+            slots.data_ptr(), cu_new.data_ptr(), taken.data_ptr(), _lib.stream_of(seq_lens)),
+            "block_tables")
     return slots, cu_new, taken
 
 
@@ -212,9 +228,8 @@ def read(cache: Cache, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]
     level rounded once to the cache's dtype; zeros outside the cache."""
     slots = _i32("slots", slots, 1, cache.device)
     T = slots.shape[0]
-    out = torch.empty((2, T, cache.heads, cache.head_dim), dtype=cache.dtype,
-                      device=cache.device)
-    k, v = out.unbind(0)
+    k = cache.k_scales.new_empty((T, cache.heads, cache.head_dim))
+    v = torch.empty_like(k)
     with _lib.on_device(slots):
         _lib.check(_lib.lib.fkc_kv4_read(cache._ref, slots.data_ptr(), T, k.data_ptr(),
                                          v.data_ptr(), _lib.stream_of(slots)), "read")
@@ -244,23 +259,19 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
     seq_lens = _i32("seq_lens", seq_lens, 1, dev)
     if cu_q is not None:
         cu_q = _i32("cu_q", cu_q, 1, dev)
-    _on_gpu("tables", tables, dev)
     T, H, D = q.shape
     R = seq_lens.shape[0]
     _require(H > 0 and H % cache.heads == 0,
              f"q's heads must be a multiple of the cache's {cache.heads}")
-    _require(tables.dtype == torch.int32 and tables.dim() == 2 and tables.shape[0] == R
-             and (tables.shape[1] <= 1 or tables.stride(1) == 1),
-             "tables must be int32 (R, max_blocks) with dense rows")
+    width, stride = _check_tables(tables, R, dev)
     _require(T == R if cu_q is None else cu_q.shape[0] == R + 1,
              "q must have one row per request, or cu_q R + 1 entries")
-    width = tables.shape[1]
     if max_seq is None:
         max_seq = width * cache.block_size
     _require(0 <= max_seq <= width * cache.block_size,
              f"max_seq {max_seq} does not fit {width} blocks of {cache.block_size}")
     if out is None:
-        out = torch.empty((T, H, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((T, H, D))
     else:
         _on_gpu("out", out, dev)
         _require(out.dtype == q.dtype and tuple(out.shape) == (T, H, D)
@@ -272,8 +283,7 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
         need = _lib.lib.fkc_kv4_attend_workspace_bytes(cache._ref, H, T, R, max_seq)
         ws = _lib.workspace(need, dev) if need else None
         _lib.check(_lib.lib.fkc_kv4_attend(
-            cache._ref, q.data_ptr(), q.stride(0), q.stride(1), H, T, tables.data_ptr(),
-            tables.stride(0) if R > 1 else width, width, seq_lens.data_ptr(), _lib.ptr(cu_q),
-            R, max_seq, int(causal), sm_scale, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws),
-            need, _lib.stream_of(q)), "attend")
+            cache._ref, q.data_ptr(), q.stride(0), q.stride(1), H, T, tables.data_ptr(), stride,
+            width, seq_lens.data_ptr(), _lib.ptr(cu_q), R, max_seq, int(causal), sm_scale,
+            out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need, _lib.stream_of(q)), "attend")
     return (out, lse) if return_lse else out
