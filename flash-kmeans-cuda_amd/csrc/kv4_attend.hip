@@ -489,6 +489,130 @@ struct Walk {
 // would run for every tile).
 __device__ inline void rare(float& v) { asm volatile("" : "+v"(v)); }
 
+// A wave's NT tiles of 16 columns: outputs and running maxima and sums.
+//   bf16: m is the largest score before its (positive) scale zscale, and a
+// weight is 2^(z zscale - m zscale).
+//   fp16 has few exponents, and a token's value scale is part of what is rounded
+// to it: m is the largest z zscale + log2 of the value scale (rounded up), and a
+// weight 2^(z zscale - m + 14), so that weight times scale is at most 2^14 and
+// the column's largest above 2^12, whatever the scales are.
+template <int DT, int D, int NT>
+struct State {
+  static constexpr int ND = D / 16;
+  float m[NT], l[NT];
+  f32x4 o[NT][ND];
+  __device__ inline void clear() {
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      m[y] = kLowest;
+      l[y] = 0.f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[y][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  // What the weights so far are relative to, as a power of two.
+  __device__ inline float base2(int y, float zscale) const {
+    return DT == FKC_F16 ? m[y] - 14.f : m[y] * zscale;
+  }
+  // Scores s of 32 tokens (their halves' groups base, this lane's first token
+  // tok) to weights, packed as the second product reads them.  masked: some
+  // column does not see all of them; lim: what each column sees, lim_max the
+  // last.
+  __device__ inline void weights(f32x4 (&s)[NT][2], const uint2 (&kw)[2], const uint2 (&vw)[2],
+                                 bool masked, int base0, int base1, int tok, const int (&lim)[NT],
+                                 int lim_max, float zscale, u32x4 (&pf)[NT]) {
+    float ks[2][4], vs[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t kx = i < 2 ? kw[j].x : kw[j].y, vx = i < 2 ? vw[j].x : vw[j].y;
+        ks[j][i] = from16<DT>((i & 1) ? kx >> 16 : kx & 0xffffu);
+        vs[j][i] = from16<DT>((i & 1) ? vx >> 16 : vx & 0xffffu);
+      }
+    if (masked) {  // what lies past the requests' tokens is anything
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if ((j ? base1 : base0) < 0 || tok + 16 * j + i >= lim_max) vs[j][i] = 0.f;
+          rare(vs[j][i]);
+        }
+    }
+    float ve[2][4];  // fp16: the value scales' exponents; zero counts as 2^-60
+    if constexpr (DT == FKC_F16) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          ve[j][i] = fmaxf((float)(int)(__float_as_uint(fabsf(vs[j][i])) >> 23) - 126.f, -60.f);
+    }
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      float z[2][4], top = kLowest;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[j][i] = s[y][j][i] * ks[j][i];
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if ((j ? base1 : base0) < 0 || tok + 16 * j + i >= lim[y]) z[j][i] = -INFINITY;
+            rare(z[j][i]);
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = fmaxf(top, DT == FKC_F16 ? __builtin_fmaf(z[j][i], zscale, ve[j][i]) : z[j][i]);
+      if (__any(top > m[y])) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float nm = fmaxf(m[y], top);
+        const float f =
+            __builtin_amdgcn_exp2f(DT == FKC_F16 ? m[y] - nm : (m[y] - nm) * zscale);
+        m[y] = nm;
+        l[y] *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[y][d] *= f;
+      }
+      const float mz = base2(y, zscale);
+      float w[2][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][i], zscale, -mz));
+          l[y] += p;
+          w[j][i] = p * vs[j][i];
+        }
+      if (masked) {  // a scale that is not finite counts where it is seen
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[j][i] = z[j][i] == -INFINITY ? 0.f : w[j][i];
+            rare(w[j][i]);
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        pf[y][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
+    }
+  }
+  // Sums of a column over its four lanes (which share m).
+  __device__ inline void join_lanes() {
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      l[y] += __shfl_xor(l[y], 16, 64);
+      l[y] += __shfl_xor(l[y], 32, 64);
+    }
+  }
+};
+
 // The kernel's (only) argument, read again from where it lies: what is not used
 // between two such places takes no registers there.
 __device__ inline const Args& arguments() {
@@ -497,18 +621,15 @@ __device__ inline const Args& arguments() {
   return *(const Args*)p;
 }
 
-// Two forms, over 32 tokens and NT column tiles per wave at a time, each wave
-// with its own running maxima and sums:
-//   split  the waves of a workgroup share the tiles and take the tokens in
-//          turn; they are joined in LDS at the end of an item
-//   wide   (prompts) every wave has tiles of its own and goes over all tokens
-// Items that the shares cut are joined by a second kernel.
-template <int DT, int D, int NT, int WAVES, bool WIDE>
-__global__ void __launch_bounds__(WAVES * 64, WIDE ? WAVES / 4
-                                                   : WAVES * (NT * D > 256 ? 1 : 2) / 4)
-kv4_attend_kernel(const Args args) {
-  constexpr int COLS = 16 * NT * (WIDE ? WAVES : 1), THREADS = WAVES * 64;
-  constexpr int STRIDE = WIDE ? 1 : WAVES, UNIT = STRIDE * 32;
+// The split form, for few columns: the waves of a workgroup share NT tiles of 16
+// columns and take 32 tokens each in turn, with their own running maxima and
+// sums; they are joined in LDS at the end of an item, cut items by a second
+// kernel.  Codes go straight from memory to registers, through the table and
+// into the products.
+template <int DT, int D, int NT, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, WAVES * (NT * D > 256 ? 1 : 2) / 4)
+kv4_split_kernel(const Args args) {
+  constexpr int COLS = 16 * NT, THREADS = WAVES * 64, UNIT = WAVES * 32;
   constexpr int KS = D / 32;  // steps of the first product
   constexpr int ND = D / 16;  // feature tiles of the second
   extern __shared__ __align__(16) char lds[];
@@ -516,7 +637,6 @@ kv4_attend_kernel(const Args args) {
   int* s_pre = reinterpret_cast<int*>(lds + kTable + kJoin);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int table = -1;  // head whose table is in LDS
   typedef Walk<COLS, THREADS, UNIT> W;
   W k = args.whole ? W(s_pre) : W(arguments(), s_pre);
   if (!(args.whole ? k.whole(arguments()) : k.next(arguments()))) return;
@@ -531,14 +651,8 @@ kv4_attend_kernel(const Args args) {
     const Item& x = k.x;
     const Tile& t = x.t;
     const int ncols = t.nq * a.G;
-    // The wave's columns, counted in the request, and what the first and the
-    // last of them see.
-    const int col0 = t.col0 + (WIDE ? wave * 16 * NT : 0);
-    const int lim_min = sees(a, t, (int)a.gdiv.div(min(col0, ncols - 1)));
-    const int lim_max =
-        !WIDE ? k.lim
-              : col0 < ncols ? sees(a, t, (int)a.gdiv.div(min(col0 + 16 * NT, ncols) - 1)) : 0;
-    const int t0 = k.from, t1 = WIDE ? min(k.to, lim_max) : k.to;
+    const int lim_min = sees(a, t, (int)a.gdiv.div(t.col0)), lim_max = k.lim;
+    const int t0 = k.from, t1 = k.to;
     const int ntile = max(t1 - t0 + 31, 0) / 32;
     const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
 
@@ -561,13 +675,12 @@ kv4_attend_kernel(const Args args) {
                                    : -1;
       }
     };
-    const int first = WIDE ? 0 : wave;
     int blk[2], base[2], nbase[2];
-    load_blocks(first, blk);
+    load_blocks(wave, blk);
 
-    // Query and head of a column of the wave's; row -1 past the last.
+    // Query and head of a column of the tile's; row -1 past the last.
     auto column = [&](const Args& a, int col, int& row, int& head, int& i) {
-      col += col0;
+      col += t.col0;
       i = (int)a.gdiv.div(min(col, ncols - 1));
       row = col < ncols ? t.row0 + i : -1;
       head = x.hc * a.G + (min(col, ncols - 1) - i * a.G);
@@ -588,45 +701,25 @@ kv4_attend_kernel(const Args args) {
     }
     const Lane<D> lanes(n, g);
     Codes<D> cur;
-    groups(first, blk, base);
-    if (first < ntile) {
+    groups(wave, blk, base);
+    if (wave < ntile) {
       load_keys<D>(a, base, lanes, cur);
       load_scales<D>(a, base, lanes, cur);
       load_values<D>(a, base, lanes, cur);
     }
-    load_blocks(first + STRIDE, blk);
-    if (!WIDE || table != x.hc) {
-      if (WIDE && table >= 0) lds_barrier();  // its last look-ups are done
-      table = x.hc;
-      fill_table<THREADS>(a, x.hc, lds, tid);
-      lds_barrier();
-    }
+    load_blocks(wave + WAVES, blk);
+    fill_table<THREADS>(a, x.hc, lds, tid);
+    lds_barrier();
 
-    // bf16: m is the largest score before its (positive) scale zscale, and a
-    // weight is 2^(z zscale - m zscale).  fp16 has few exponents, and a token's
-    // value scale is part of what is rounded to it: m is the largest z zscale +
-    // log2 of the value scale (rounded up), and a weight 2^(z zscale - m + 14),
-    // so that weight times scale is at most 2^14 and the column's largest above
-    // 2^12, whatever the scales are.
-    float m[NT], l[NT];
-    f32x4 o[NT][ND];
-#pragma unroll
-    for (int y = 0; y < NT; ++y) {
-      m[y] = kLowest;
-      l[y] = 0.f;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[y][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    // What the weights so far are relative to, as a power of two.
-    auto base2 = [](float m, float zscale) { return DT == FKC_F16 ? m - 14.f : m * zscale; };
-
+    State<DT, D, NT> st;
+    st.clear();
     // What a tile has used up is fetched for the next one at once, into the
     // same registers: with a second set of them four waves a SIMD do not fit,
     // and it is they that hide the loads' latency.
-    for (int it = first; it < ntile; it += STRIDE) {
-      const bool more = it + STRIDE < ntile;
-      groups(it + STRIDE, blk, nbase);
-      load_blocks(it + 2 * STRIDE, blk);
+    for (int it = wave; it < ntile; it += WAVES) {
+      const bool more = it + WAVES < ntile;
+      groups(it + WAVES, blk, nbase);
+      load_blocks(it + 2 * WAVES, blk);
 
       f32x4 s[NT][2];
 #pragma unroll
@@ -641,93 +734,11 @@ kv4_attend_kernel(const Args args) {
             s[y][j] = mfma<DT>(kf, qf[y][c], c ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
       if (more) load_keys<D>(a, nbase, lanes, cur);
-      const int tok = t0 + it * 32 + 4 * g;  // token (j, i): tok + 16 j + i
-      const bool masked = t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0;
-      float ks[2][4], vs[2][4];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t kw = i < 2 ? cur.ks[j].x : cur.ks[j].y;
-          const uint32_t vw = i < 2 ? cur.vs[j].x : cur.vs[j].y;
-          ks[j][i] = from16<DT>((i & 1) ? kw >> 16 : kw & 0xffffu);
-          vs[j][i] = from16<DT>((i & 1) ? vw >> 16 : vw & 0xffffu);
-        }
+      const uint2 kw[2] = {cur.ks[0], cur.ks[1]}, vw[2] = {cur.vs[0], cur.vs[1]};
       if (more) load_scales<D>(a, nbase, lanes, cur);
-      if (masked) {  // what lies past the requests' tokens is anything
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (base[j] < 0 || tok + 16 * j + i >= lim_max) vs[j][i] = 0.f;
-            rare(vs[j][i]);
-          }
-      }
-      float ve[2][4];  // fp16: the value scales' exponents; zero counts as 2^-60
-      if constexpr (DT == FKC_F16) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            ve[j][i] = fmaxf((float)(int)(__float_as_uint(fabsf(vs[j][i])) >> 23) - 126.f, -60.f);
-      }
       u32x4 pf[NT];
-#pragma unroll
-      for (int y = 0; y < NT; ++y) {
-        float z[2][4], top = kLowest;
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) z[j][i] = s[y][j][i] * ks[j][i];
-        if (masked) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (base[j] < 0 || tok + 16 * j + i >= lim[y]) z[j][i] = -INFINITY;
-              rare(z[j][i]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            top = fmaxf(top, DT == FKC_F16 ? __builtin_fmaf(z[j][i], a.zscale, ve[j][i])
-                                           : z[j][i]);
-        if (__any(top > m[y])) {
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64));
-          const float nm = fmaxf(m[y], top);
-          const float f = __builtin_amdgcn_exp2f(
-              DT == FKC_F16 ? m[y] - nm : (m[y] - nm) * a.zscale);
-          m[y] = nm;
-          l[y] *= f;
-#pragma unroll
-          for (int d = 0; d < ND; ++d) o[y][d] *= f;
-        }
-        const float mz = base2(m[y], a.zscale);
-        float w[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j][i], a.zscale, -mz));
-            l[y] += p;
-            w[j][i] = p * vs[j][i];
-          }
-        if (masked) {  // a scale that is not finite counts where it is seen
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              w[j][i] = z[j][i] == -INFINITY ? 0.f : w[j][i];
-              rare(w[j][i]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          pf[y][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
-      }
+      st.weights(s, kw, vw, t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0, base[0],
+                 base[1], t0 + it * 32 + 4 * g, lim, lim_max, a.zscale, pf);
       // Features 2 b and 2 b + 1 of the lane's row, two tokens a dword.
 #pragma unroll
       for (int v = 0; v < (ND + 7) / 8; ++v) {
@@ -746,8 +757,8 @@ kv4_attend_kernel(const Args args) {
           }
 #pragma unroll
           for (int y = 0; y < NT; ++y) {
-            o[y][8 * v + 2 * b] = mfma<DT>(lo, pf[y], o[y][8 * v + 2 * b]);
-            o[y][8 * v + 2 * b + 1] = mfma<DT>(hi, pf[y], o[y][8 * v + 2 * b + 1]);
+            st.o[y][8 * v + 2 * b] = mfma<DT>(lo, pf[y], st.o[y][8 * v + 2 * b]);
+            st.o[y][8 * v + 2 * b + 1] = mfma<DT>(hi, pf[y], st.o[y][8 * v + 2 * b + 1]);
           }
         }
       }
@@ -756,53 +767,7 @@ kv4_attend_kernel(const Args args) {
       base[1] = nbase[1];
     }
 
-    // Join the lanes of a column (they share m).
-#pragma unroll
-    for (int y = 0; y < NT; ++y) {
-      l[y] += __shfl_xor(l[y], 16, 64);
-      l[y] += __shfl_xor(l[y], 32, 64);
-    }
-    if constexpr (WIDE) {
-      const Args& a = arguments();
-#pragma unroll
-      for (int y = 0; y < NT; ++y) {
-        int row, head, i;
-        column(a, 16 * y + n, row, head, i);
-        if (row < 0) continue;
-        if (!k.cut()) {
-          const float f = l[y] > 0.f ? 1.f / l[y] : 0.f;
-          const int64_t at = (int64_t)row * a.H + head;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[ND / 2];
-#pragma unroll
-            for (int d = 0; d < ND / 2; ++d)
-              w[d] = pack2<DT>(o[y][2 * d][i] * f, o[y][2 * d + 1][i] * f);
-            uint32_t* op = reinterpret_cast<uint32_t*>(a.out + at * D + (4 * g + i) * ND);
-#pragma unroll
-            for (int d = 0; d < ND / 2; ++d) op[d] = w[d];
-          }
-          if (g == 0 && a.lse != nullptr)
-            a.lse[at] = log_sum(base2(m[y], a.zscale), l[y]);
-        } else {
-          const int64_t at = k.slot() * COLS + wave * 16 * NT + 16 * y + n;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int d = 0; d < ND / 4; ++d)
-              *reinterpret_cast<f32x4*>(a.part + at * D + (4 * g + i) * ND + 4 * d) =
-                  f32x4{o[y][4 * d][i], o[y][4 * d + 1][i], o[y][4 * d + 2][i],
-                        o[y][4 * d + 3][i]};
-          if (g == 0)
-            *reinterpret_cast<float2*>(a.part_ml + 2 * at) =
-                float2{base2(m[y], a.zscale), l[y]};
-        }
-      }
-      if (args.whole) return;
-      if (tid == 0) k.announce(arguments());
-      if (!k.next(arguments())) return;
-      continue;
-    }
+    st.join_lanes();
     // Join the waves that had tokens: their outputs, relative to the largest
     // maximum, go to LDS as rows of features (over the table, 16-byte pieces
     // turned by the column so that no two lanes meet in a bank) and are summed
@@ -811,8 +776,8 @@ kv4_attend_kernel(const Args args) {
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
       if (y) lds_barrier();  // the last tile's pieces are read
-      const float rel = base2(m[y], a.zscale);
-      if (g == 0) sml[wave * 16 + n] = float2{rel, l[y]};
+      const float rel = st.base2(y, a.zscale);
+      if (g == 0) sml[wave * 16 + n] = float2{rel, st.l[y]};
       lds_barrier();
       const Args& a = arguments();
       float top = kLowest;
@@ -826,8 +791,8 @@ kv4_attend_kernel(const Args args) {
           for (int d = 0; d < ND / 4; ++d) {
             const int piece = (4 * g + i) * (ND / 4) + d;
             so[(wave * 16 + n) * (D / 4) + (piece ^ n)] =
-                f32x4{o[y][4 * d][i], o[y][4 * d + 1][i], o[y][4 * d + 2][i],
-                      o[y][4 * d + 3][i]} * f;
+                f32x4{st.o[y][4 * d][i], st.o[y][4 * d + 1][i], st.o[y][4 * d + 2][i],
+                      st.o[y][4 * d + 3][i]} * f;
           }
       }
       lds_barrier();
@@ -868,6 +833,256 @@ kv4_attend_kernel(const Args args) {
     if (tid == 0) k.announce(arguments());
     if (!k.next(arguments())) return;
     lds_barrier();  // the next item fills the table again
+  }
+}
+
+// The wide form, for prompts: every wave has NT tiles of 16 columns of its own,
+// and all of a workgroup's go over the same TT tokens at a time.  These are
+// looked up once for all: each wave turns its share of the codes into the
+// fragments of both products, laid out so that a fragment is read by 64 lanes
+// in a row (16 bytes each, no bank conflict), in one of two buffers; while a
+// tile is computed on, the next one is filled into the other.  Per 32 tokens
+// and wave that leaves 2 D / 16 LDS reads where looking up costs 16 times as
+// many operations of three kinds: bound then by the vector unit's work on the
+// scores (about nine operations and one exponential each).
+//
+// Feature row n of fragment d of the second product is feature 32 (d / 2) + 2 n +
+// d % 2: the two codes of one byte go to two fragments, and 16 lanes read 16
+// bytes of a token.
+template <int DT, int D, int NT, int TT>
+__global__ void __launch_bounds__(512, 2)
+kv4_wide_kernel(const Args args) {
+  constexpr int WAVES = 8, COLS = 16 * NT * WAVES, THREADS = WAVES * 64;
+  constexpr int KS = D / 32, ND = D / 16, HALVES = TT / 16, GROUPS = TT / 32;
+  constexpr int KPW = HALVES * KS / WAVES;  // key fragments a wave fills
+  constexpr int VW = GROUPS * ND / 2;       // waves that fill two value fragments
+  static_assert(KPW >= 1 && KS % KPW == 0 && VW <= WAVES, "a wave fills within one half");
+  constexpr int KBYTES = TT * D * 2, BUF = 2 * KBYTES;
+  extern __shared__ __align__(16) char lds[];
+  int* s_pre = reinterpret_cast<int*>(lds + kTable + 2 * BUF);
+
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kj = wave * KPW / KS, kc0 = wave * KPW % KS;  // its half, first step
+  const int vg = wave / (ND / 2), vu = wave % (ND / 2);   // its group, fragment pair
+  int table = -1;  // head whose table is in LDS
+  typedef Walk<COLS, THREADS, TT> W;
+  W k = args.whole ? W(s_pre) : W(arguments(), s_pre);
+  if (!(args.whole ? k.whole(arguments()) : k.next(arguments()))) return;
+  for (;;) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const Args& a = arguments();
+    const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const uint32_t loff = (uint32_t)(lane & 31) * 4;
+    const Item& x = k.x;
+    const Tile& t = x.t;
+    const int ncols = t.nq * a.G;
+    // The wave's columns, counted in the request, and what the first and the
+    // last of them see.
+    const int col0 = t.col0 + wave * 16 * NT;
+    const int lim_min = sees(a, t, (int)a.gdiv.div(min(col0, ncols - 1)));
+    const int lim_max =
+        col0 < ncols ? sees(a, t, (int)a.gdiv.div(min(col0 + 16 * NT, ncols) - 1)) : 0;
+    const int t0 = k.from, t1 = k.to, tiles = (max(t1 - t0, 0) + TT - 1) / TT;
+
+    // The arguments that every tile needs, in scalar registers (left to itself
+    // the compiler reads them again at each use, and waits).
+    const uint8_t* k_codes = a.k_codes;
+    const uint8_t* v_codes = a.v_codes;
+    const uint16_t* k_scales = a.k_scales;
+    const uint16_t* v_scales = a.v_scales;
+    uint32_t bs = a.bs.d, bs_m = a.bs.m, num_blocks = a.num_blocks;
+    int bs_sh = a.bs.sh, heads = a.heads;
+    float zscale = a.zscale;
+    asm volatile("" : "+s"(k_codes), "+s"(v_codes), "+s"(k_scales), "+s"(v_scales));
+    asm volatile("" : "+s"(bs), "+s"(bs_m), "+s"(num_blocks), "+s"(bs_sh), "+s"(heads),
+                 "+s"(zscale));
+    const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
+    // 16-slot groups of a tile's halves over all heads, -1 where there is none.
+    auto find_groups = [&](int tile, int (&base)[HALVES]) {
+#pragma unroll
+      for (int j = 0; j < HALVES; ++j) {
+        const uint32_t tok = t0 + tile * TT + 16 * j;
+        const uint32_t at = __umulhi(tok, bs_m) >> bs_sh;  // (block sizes are 16 at least)
+        const uint32_t b = (int)tok < t1 ? (uint32_t)blocks[at] : 0xffffffffu;
+        base[j] = b < num_blocks ? (int)((b * heads + x.hc) * (bs / 16) + (tok - at * bs) / 16)
+                                 : -1;
+      }
+    };
+    uint32_t kcode[KPW], vcode[8];
+    uint2 ks[HALVES], vs[HALVES];
+    auto pick = [](const int (&base)[HALVES], int j) {
+      int v = base[0];
+#pragma unroll
+      for (int i = 1; i < HALVES; ++i) v = j == i ? base[i] : v;
+      return (int64_t)max(v, 0);  // a missing half reads slot 0
+    };
+    auto load_tile = [&](const int (&base)[HALVES]) {
+      const uint8_t* kp = k_codes + pick(base, kj) * (16 * D / 2);
+#pragma unroll
+      for (int e = 0; e < KPW; ++e)
+        kcode[e] = at<uint32_t>(kp, n * (D / 2) + g * (D / 8) + (kc0 + e) * 4);
+      if (wave < VW) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint8_t* vp = v_codes + pick(base, 2 * vg + j) * (16 * D / 2);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            vcode[4 * j + i] = at<uint8_t>(vp, (4 * g + i) * (D / 2) + 16 * vu + n);
+        }
+      }
+    };
+    auto load_scales = [&](const int (&base)[HALVES], int j) {
+      const int64_t row = (int64_t)max(base[j], 0) * 16;
+      ks[j] = at<uint2>(k_scales + row, 8 * g);
+      vs[j] = at<uint2>(v_scales + row, 8 * g);
+    };
+    auto fill_buffer = [&](int tile) {
+      char* buf = lds + kTable + (tile & 1) * BUF + lane * 16;
+#pragma unroll
+      for (int e = 0; e < KPW; ++e) {
+        u32x4 f;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) f[b] = lookup<0>(kcode[e], b, loff);
+        *reinterpret_cast<u32x4*>(buf + (kj * KS + kc0 + e) * 1024) = f;
+      }
+      if (wave < VW) {
+        u32x4 even, odd;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t b0 = vcode[2 * c], b1 = vcode[2 * c + 1];
+          even[c] = lookup<128>((b0 & 15u) | (b1 << 4 & 0xf0u), 0, loff);
+          odd[c] = lookup<128>(b0 >> 4 | (b1 & 0xf0u), 0, loff);
+        }
+        char* vb = buf + KBYTES + (vg * ND + 2 * vu) * 1024;
+        *reinterpret_cast<u32x4*>(vb) = even;
+        *reinterpret_cast<u32x4*>(vb + 1024) = odd;
+      }
+    };
+    auto column = [&](const Args& a, int y, int& row, int& head, int& i) {
+      const int col = col0 + 16 * y + n;
+      i = (int)a.gdiv.div(min(col, ncols - 1));
+      row = col < ncols ? t.row0 + i : -1;
+      head = x.hc * a.G + (min(col, ncols - 1) - i * a.G);
+    };
+
+    int base[HALVES], nbase[HALVES];  // of this tile and the next
+    find_groups(0, base);
+    find_groups(1, nbase);
+    if (tiles > 0) {
+      load_tile(base);
+#pragma unroll
+      for (int j = 0; j < HALVES; ++j) load_scales(base, j);
+    }
+    int lim[NT];
+    u32x4 qf[NT][KS];
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      int row, head, i;
+      column(a, y, row, head, i);
+      const bool ok = row >= 0;
+      lim[y] = ok ? sees(a, t, i) : 0;
+      const uint16_t* qp = a.q + max(row, t.row0) * a.q_ts + head * a.q_hs + g * (D / 4);
+#pragma unroll
+      for (int c = 0; c < KS; ++c)
+        qf[y][c] = (ok ? *reinterpret_cast<const u32x4*>(qp + c * 8) : u32x4{0, 0, 0, 0}) ^
+                   a.qsign;
+    }
+    if (table != x.hc) {  // (every look-up of the last item was before its last barrier)
+      table = x.hc;
+      fill_table<THREADS>(a, x.hc, lds, tid);
+      lds_barrier();
+    }
+    if (tiles > 0) fill_buffer(0);
+    if (tiles > 1) load_tile(nbase);
+    lds_barrier();
+
+    State<DT, D, NT> st;
+    st.clear();
+    for (int tile = 0; tile < tiles; ++tile) {
+      int after[HALVES];
+      if (tile + 1 < tiles) fill_buffer(tile + 1);
+      find_groups(tile + 2, after);
+      if (tile + 2 < tiles) load_tile(after);
+      const char* buf = lds + kTable + (tile & 1) * BUF + lane * 16;
+      auto group = [&](auto H) {
+        constexpr int h = H.value;
+        const int tok = t0 + tile * TT + 32 * h;
+        const uint2 kw[2] = {ks[2 * h], ks[2 * h + 1]}, vw[2] = {vs[2 * h], vs[2 * h + 1]};
+        if (tile + 1 < tiles) {
+          load_scales(nbase, 2 * h);
+          load_scales(nbase, 2 * h + 1);
+        }
+        if (tok >= lim_max) return;  // none of the wave's columns sees them
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int c = 0; c < KS; ++c)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const u32x4 kf =
+                *reinterpret_cast<const u32x4*>(buf + ((2 * h + j) * KS + c) * 1024);
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
+              s[y][j] = mfma<DT>(kf, qf[y][c], c ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+          }
+        u32x4 pf[NT];
+        st.weights(s, kw, vw, tok + 32 > lim_min || (base[2 * h] | base[2 * h + 1]) < 0,
+                   base[2 * h], base[2 * h + 1], tok + 4 * g, lim, lim_max, zscale, pf);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const u32x4 vf = *reinterpret_cast<const u32x4*>(buf + KBYTES + (h * ND + d) * 1024);
+#pragma unroll
+          for (int y = 0; y < NT; ++y) st.o[y][d] = mfma<DT>(vf, pf[y], st.o[y][d]);
+        }
+      };
+      group(std::integral_constant<int, 0>{});
+      if constexpr (GROUPS > 1) group(std::integral_constant<int, 1>{});
+#pragma unroll
+      for (int j = 0; j < HALVES; ++j) {
+        base[j] = nbase[j];
+        nbase[j] = after[j];
+      }
+      lds_barrier();
+    }
+
+    st.join_lanes();
+    {
+      const Args& a = arguments();
+#pragma unroll
+      for (int y = 0; y < NT; ++y) {
+        int row, head, i;
+        column(a, y, row, head, i);
+        if (row < 0) continue;
+        if (!k.cut()) {
+          const float f = st.l[y] > 0.f ? 1.f / st.l[y] : 0.f;
+          const int64_t at = (int64_t)row * a.H + head;
+#pragma unroll
+          for (int u = 0; u < ND / 2; ++u) {
+            u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = pack2<DT>(st.o[y][2 * u][i] * f, st.o[y][2 * u + 1][i] * f);
+            *reinterpret_cast<u32x4*>(a.out + at * D + 32 * u + 8 * g) = w;
+          }
+          if (g == 0 && a.lse != nullptr) a.lse[at] = log_sum(st.base2(y, a.zscale), st.l[y]);
+        } else {
+          const int64_t at = k.slot() * COLS + wave * 16 * NT + 16 * y + n;
+#pragma unroll
+          for (int u = 0; u < ND / 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2)
+              *reinterpret_cast<f32x4*>(a.part + at * D + 32 * u + 8 * g + 2 * i) =
+                  f32x4{st.o[y][2 * u][i], st.o[y][2 * u + 1][i], st.o[y][2 * u][i + 1],
+                        st.o[y][2 * u + 1][i + 1]};
+          if (g == 0)
+            *reinterpret_cast<float2*>(a.part_ml + 2 * at) =
+                float2{st.base2(y, a.zscale), st.l[y]};
+        }
+      }
+    }
+    if (args.whole) return;
+    if (tid == 0) k.announce(arguments());
+    if (!k.next(arguments())) return;
   }
 }
 
@@ -1021,6 +1236,7 @@ struct Plan {
 
 constexpr int kWide = 8;  // waves of the wide form
 constexpr int wide_tiles(int D) { return D == 256 ? 1 : 2; }
+constexpr int wide_tokens(int D) { return D == 256 ? 32 : 64; }
 constexpr int waves_of(int D) { return D == 256 ? 4 : 8; }
 
 Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t max_seq,
@@ -1042,13 +1258,10 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
   return p;
 }
 
-template <int DT, int D, int NT, int WAVES, bool WIDE>
-int launch(const Args& a, const Plan& p, hipStream_t s) {
-  constexpr int COLS = 16 * NT * (WIDE ? WAVES : 1);
-  const int bytes = kTable + kJoin + Shares<COLS, WAVES * 64, 1>::kInts * 4;
-  auto* kernel = &kv4_attend_kernel<DT, D, NT, WAVES, WIDE>;
+template <int DT, int D, int COLS, int THREADS, typename K>
+int launch(K kernel, std::atomic<uint64_t>& set, int bytes, const Args& a, const Plan& p,
+           hipStream_t s) {
   // The attribute stays with the kernel: once per device is enough.
-  static std::atomic<uint64_t> set{0};
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess) dev = -1;
   const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
@@ -1058,7 +1271,7 @@ int launch(const Args& a, const Plan& p, hipStream_t s) {
       return fail(FKC_ERR_LAUNCH, "kv4_attend: %d bytes of LDS refused", bytes);
     set.fetch_or(bit, std::memory_order_relaxed);
   }
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)p.wgs), dim3(WAVES * 64), bytes, s, a);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)p.wgs), dim3(THREADS), bytes, s, a);
   if (int rc = check_launch("kv4_attend")) return rc;
   if (p.whole) return FKC_OK;
   const int64_t cols = std::min<int64_t>(COLS, a.cu_q ? COLS : a.G);
@@ -1066,6 +1279,23 @@ int launch(const Args& a, const Plan& p, hipStream_t s) {
                      dim3((uint32_t)p.wgs, (uint32_t)std::min<int64_t>((cols + 3) / 4, 16)),
                      dim3(256), 0, s, a);
   return check_launch("kv4_attend (join)");
+}
+
+template <int DT, int D, int NT, int WAVES>
+int launch_split(const Args& a, const Plan& p, hipStream_t s) {
+  static std::atomic<uint64_t> set{0};
+  return launch<DT, D, 16 * NT, WAVES * 64>(
+      &kv4_split_kernel<DT, D, NT, WAVES>, set,
+      kTable + kJoin + Shares<16 * NT, WAVES * 64, 1>::kInts * 4, a, p, s);
+}
+
+template <int DT, int D>
+int launch_wide(const Args& a, const Plan& p, hipStream_t s) {
+  static std::atomic<uint64_t> set{0};
+  constexpr int NT = wide_tiles(D), TT = wide_tokens(D), COLS = 16 * NT * kWide;
+  return launch<DT, D, COLS, kWide * 64>(
+      &kv4_wide_kernel<DT, D, NT, TT>, set,
+      kTable + 2 * (TT * D * 4) + Shares<COLS, kWide * 64, 1>::kInts * 4, a, p, s);
 }
 
 }  // namespace
@@ -1108,9 +1338,9 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
   }
   return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     constexpr int DT = dt.value, DD = d.value;
-    if (p.wide) return launch<DT, DD, wide_tiles(DD), kWide, true>(a, p, s);
-    return p.nt == 1 ? launch<DT, DD, 1, waves_of(DD), false>(a, p, s)
-                     : launch<DT, DD, 2, 4, false>(a, p, s);
+    if (p.wide) return launch_wide<DT, DD>(a, p, s);
+    return p.nt == 1 ? launch_split<DT, DD, 1, waves_of(DD)>(a, p, s)
+                     : launch_split<DT, DD, 2, 4>(a, p, s);
   });
 }
 
