@@ -858,6 +858,7 @@ kv4_wide_kernel(const Args args) {
   constexpr int VW = GROUPS * ND / 2;       // waves that fill two value fragments
   static_assert(KPW >= 1 && KS % KPW == 0 && VW <= WAVES, "a wave fills within one half");
   constexpr int KBYTES = TT * D * 2, BUF = 2 * KBYTES;
+  typedef int Groups __attribute__((ext_vector_type(HALVES)));
   extern __shared__ __align__(16) char lds[];
   int* s_pre = reinterpret_cast<int*>(lds + kTable + 2 * BUF);
 
@@ -899,7 +900,7 @@ kv4_wide_kernel(const Args args) {
                  "+s"(zscale));
     const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
     // 16-slot groups of a tile's halves over all heads, -1 where there is none.
-    auto find_groups = [&](int tile, int (&base)[HALVES]) {
+    auto find_groups = [&](int tile, Groups& base) {
 #pragma unroll
       for (int j = 0; j < HALVES; ++j) {
         const uint32_t tok = t0 + tile * TT + 16 * j;
@@ -911,13 +912,13 @@ kv4_wide_kernel(const Args args) {
     };
     uint32_t kcode[KPW], vcode[8];
     uint2 ks[HALVES], vs[HALVES];
-    auto pick = [](const int (&base)[HALVES], int j) {
+    auto pick = [](const Groups& base, int j) {
       int v = base[0];
 #pragma unroll
       for (int i = 1; i < HALVES; ++i) v = j == i ? base[i] : v;
       return (int64_t)max(v, 0);  // a missing half reads slot 0
     };
-    auto load_tile = [&](const int (&base)[HALVES]) {
+    auto load_tile = [&](const Groups& base) {
       const uint8_t* kp = k_codes + pick(base, kj) * (16 * D / 2);
 #pragma unroll
       for (int e = 0; e < KPW; ++e)
@@ -932,7 +933,7 @@ kv4_wide_kernel(const Args args) {
         }
       }
     };
-    auto load_scales = [&](const int (&base)[HALVES], int j) {
+    auto load_scales = [&](const Groups& base, int j) {
       const int64_t row = (int64_t)max(base[j], 0) * 16;
       ks[j] = at<uint2>(k_scales + row, 8 * g);
       vs[j] = at<uint2>(v_scales + row, 8 * g);
@@ -966,7 +967,7 @@ kv4_wide_kernel(const Args args) {
       head = x.hc * a.G + (min(col, ncols - 1) - i * a.G);
     };
 
-    int base[HALVES], nbase[HALVES];  // of this tile and the next
+    Groups base, nbase;  // of this tile and the next
     find_groups(0, base);
     find_groups(1, nbase);
     if (tiles > 0) {
@@ -1000,7 +1001,7 @@ kv4_wide_kernel(const Args args) {
     State<DT, D, NT> st;
     st.clear();
     for (int tile = 0; tile < tiles; ++tile) {
-      int after[HALVES];
+      Groups after;
       if (tile + 1 < tiles) fill_buffer(tile + 1);
       find_groups(tile + 2, after);
       if (tile + 2 < tiles) load_tile(after);
@@ -1037,11 +1038,8 @@ kv4_wide_kernel(const Args args) {
       };
       group(std::integral_constant<int, 0>{});
       if constexpr (GROUPS > 1) group(std::integral_constant<int, 1>{});
-#pragma unroll
-      for (int j = 0; j < HALVES; ++j) {
-        base[j] = nbase[j];
-        nbase[j] = after[j];
-      }
+      base = nbase;
+      nbase = after;
       lds_barrier();
     }
 
