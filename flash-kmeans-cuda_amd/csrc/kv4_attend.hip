@@ -713,11 +713,11 @@ kv4_split_kernel(const Args args) {
 
     State<DT, D, NT> st;
     st.clear();
-    // What a tile has used up is fetched for the next one at once, into the
-    // same registers: with a second set of them four waves a SIMD do not fit,
+    // What a tile has used up is fetched for the next one at once, after the last
+    // tile slot 0's (a load that may or may not be on its way would have to be
+    // waited for with every older one), into the same registers: with a second set of them four waves a SIMD do not fit,
     // and it is they that hide the loads' latency.
     for (int it = wave; it < ntile; it += WAVES) {
-      const bool more = it + WAVES < ntile;
       groups(it + WAVES, blk, nbase);
       load_blocks(it + 2 * WAVES, blk);
 
@@ -733,9 +733,9 @@ kv4_split_kernel(const Args args) {
           for (int y = 0; y < NT; ++y)
             s[y][j] = mfma<DT>(kf, qf[y][c], c ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
-      if (more) load_keys<D>(a, nbase, lanes, cur);
+      load_keys<D>(a, nbase, lanes, cur);
       const uint2 kw[2] = {cur.ks[0], cur.ks[1]}, vw[2] = {cur.vs[0], cur.vs[1]};
-      if (more) load_scales<D>(a, nbase, lanes, cur);
+      load_scales<D>(a, nbase, lanes, cur);
       u32x4 pf[NT];
       st.weights(s, kw, vw, t0 + it * 32 + 32 > lim_min || (base[0] | base[1]) < 0, base[0],
                  base[1], t0 + it * 32 + 4 * g, lim, lim_max, a.zscale, pf);
@@ -762,7 +762,7 @@ kv4_split_kernel(const Args args) {
           }
         }
       }
-      if (more) load_values<D>(a, nbase, lanes, cur);
+      load_values<D>(a, nbase, lanes, cur);
       base[0] = nbase[0];
       base[1] = nbase[1];
     }
@@ -864,7 +864,7 @@ kv4_wide_kernel(const Args args) {
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kj = wave * KPW / KS, kc0 = wave * KPW % KS;  // its half, first step
-  const int vg = wave / (ND / 2), vu = wave % (ND / 2);   // its group, fragment pair
+  const int vg = wave % VW / (ND / 2), vu = wave % (ND / 2);  // its group, fragment pair
   int table = -1;  // head whose table is in LDS
   typedef Walk<COLS, THREADS, TT> W;
   W k = args.whole ? W(s_pre) : W(arguments(), s_pre);
@@ -923,7 +923,8 @@ kv4_wide_kernel(const Args args) {
 #pragma unroll
       for (int e = 0; e < KPW; ++e)
         kcode[e] = at<uint32_t>(kp, n * (D / 2) + g * (D / 8) + (kc0 + e) * 4);
-      if (wave < VW) {
+      // (waves without value fragments load those of others)
+      {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const uint8_t* vp = v_codes + pick(base, 2 * vg + j) * (16 * D / 2);
@@ -995,7 +996,7 @@ kv4_wide_kernel(const Args args) {
       lds_barrier();
     }
     if (tiles > 0) fill_buffer(0);
-    if (tiles > 1) load_tile(nbase);
+    if (tiles > 0) load_tile(nbase);
     lds_barrier();
 
     State<DT, D, NT> st;
@@ -1004,16 +1005,16 @@ kv4_wide_kernel(const Args args) {
       Groups after;
       if (tile + 1 < tiles) fill_buffer(tile + 1);
       find_groups(tile + 2, after);
-      if (tile + 2 < tiles) load_tile(after);
+      // Past the last tile slot 0's codes, unused: a load that may or may not be
+      // on its way would have to be waited for with every older one.
+      load_tile(after);
       const char* buf = lds + kTable + (tile & 1) * BUF + lane * 16;
       auto group = [&](auto H) {
         constexpr int h = H.value;
         const int tok = t0 + tile * TT + 32 * h;
         const uint2 kw[2] = {ks[2 * h], ks[2 * h + 1]}, vw[2] = {vs[2 * h], vs[2 * h + 1]};
-        if (tile + 1 < tiles) {
-          load_scales(nbase, 2 * h);
-          load_scales(nbase, 2 * h + 1);
-        }
+        load_scales(nbase, 2 * h);
+        load_scales(nbase, 2 * h + 1);
         if (tok >= lim_max) return;  // none of the wave's columns sees them
         f32x4 s[NT][2];
 #pragma unroll
