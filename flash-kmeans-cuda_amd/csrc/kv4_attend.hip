@@ -206,6 +206,19 @@ struct Lane {
       : k(n * (D / 2) + g * (D / 8)), v(4 * g * (D / 2) + n * (D / 32)), s(8 * g) {}
 };
 
+typedef const char __attribute__((address_space(1))) * Global;
+
+template <typename T>
+__device__ inline T at(Global base, uint32_t off) {
+  typedef uint32_t Two __attribute__((ext_vector_type(2)));
+  if constexpr (std::is_same<T, uint2>::value) {
+    const Two v = *(const Two __attribute__((address_space(1)))*)(base + off);
+    return uint2{v[0], v[1]};
+  } else {
+    return *(const T __attribute__((address_space(1)))*)(base + off);
+  }
+}
+
 template <typename T>
 __device__ inline T at(const void* base, uint32_t off) {
   return *reinterpret_cast<const T*>(static_cast<const char*>(base) + off);
@@ -888,10 +901,10 @@ kv4_wide_kernel(const Args args) {
 
     // The arguments that every tile needs, in scalar registers (left to itself
     // the compiler reads them again at each use, and waits).
-    const uint8_t* k_codes = a.k_codes;
-    const uint8_t* v_codes = a.v_codes;
-    const uint16_t* k_scales = a.k_scales;
-    const uint16_t* v_scales = a.v_scales;
+    // (Global addresses by type: behind the asm nothing else says so, and a
+    // load that might be LDS's would be waited for with every LDS read.)
+    Global k_codes = (Global)a.k_codes, v_codes = (Global)a.v_codes;
+    Global k_scales = (Global)a.k_scales, v_scales = (Global)a.v_scales;
     uint32_t bs = a.bs.d, bs_m = a.bs.m, num_blocks = a.num_blocks;
     int bs_sh = a.bs.sh, heads = a.heads;
     float zscale = a.zscale;
@@ -919,7 +932,7 @@ kv4_wide_kernel(const Args args) {
       return (int64_t)max(v, 0);  // a missing half reads slot 0
     };
     auto load_tile = [&](const Groups& base) {
-      const uint8_t* kp = k_codes + pick(base, kj) * (16 * D / 2);
+      const Global kp = k_codes + pick(base, kj) * (16 * D / 2);
 #pragma unroll
       for (int e = 0; e < KPW; ++e)
         kcode[e] = at<uint32_t>(kp, n * (D / 2) + g * (D / 8) + (kc0 + e) * 4);
@@ -927,7 +940,7 @@ kv4_wide_kernel(const Args args) {
       {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint8_t* vp = v_codes + pick(base, 2 * vg + j) * (16 * D / 2);
+          const Global vp = v_codes + pick(base, 2 * vg + j) * (16 * D / 2);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             vcode[4 * j + i] = at<uint8_t>(vp, (4 * g + i) * (D / 2) + 16 * vu + n);
@@ -935,7 +948,7 @@ kv4_wide_kernel(const Args args) {
       }
     };
     auto load_scales = [&](const Groups& base, int j) {
-      const int64_t row = (int64_t)max(base[j], 0) * 16;
+      const int64_t row = (int64_t)max(base[j], 0) * 32;  // bytes
       ks[j] = at<uint2>(k_scales + row, 8 * g);
       vs[j] = at<uint2>(v_scales + row, 8 * g);
     };
