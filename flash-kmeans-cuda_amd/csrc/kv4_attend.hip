@@ -640,7 +640,7 @@ __device__ inline const Args& arguments() {
 // kernel.  Codes go straight from memory to registers, through the table and
 // into the products.
 template <int DT, int D, int NT, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, WAVES * (NT * D > 256 ? 1 : 2) / 4)
+__global__ void __launch_bounds__(WAVES * 64, WAVES / 2)
 kv4_split_kernel(const Args args) {
   constexpr int COLS = 16 * NT, THREADS = WAVES * 64, UNIT = WAVES * 32;
   constexpr int KS = D / 32;  // steps of the first product
@@ -1231,9 +1231,13 @@ int by_shape(int dtype, int64_t D, F&& f) {
                           : with(std::integral_constant<int, FKC_BF16>{});
 }
 
-// Units of a share at least, times two: where no context is longer, every item
-// goes to a workgroup of its own and nothing has to be joined.
-constexpr int kMinShare = 4;
+// Granules of a share at least, and up to how many granules a context is never
+// cut: every item then goes to a workgroup of its own, and nothing has to be
+// joined by a second kernel.  (bf16, D = 128, 8 heads, 4 query heads each, one
+// query, us: contexts of 1536 whole 16.2 / 16.8 / 24.7 for 1 / 8 / 64 requests,
+// cut 17.2 / 19.2 / 29.7; of 3000 whole 24.6 / 25.0 / 39.3, cut 18.3 / 22.4 /
+// 42.6.)
+constexpr int kMinShare = 2, kWhole = 8, kWideWhole = 32;
 
 struct Plan {
   bool wide;
@@ -1255,17 +1259,22 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
                bool ragged) {
   Plan p;
   const int64_t G = H / c.heads;
-  // Column tiles: as many as an average request fills; waves with columns of
-  // their own from 96 columns on.
+  // By the columns of an average request.  Measured on 8 requests of 4096
+  // tokens, 8 heads of 4 query heads, bf16, us with one tile per workgroup /
+  // with two / in the wide form, for so many columns each:
+  //   D =  64    32: 25 / 25 / 52    96: 44 / 38 / 60    256:  86 /  72 /  89
+  //             512: 148 / 114 / 111
+  //   D = 128    32: 29 / 33 / 60    96: 54 / 49 / 74    256: 110 /  94 / 109
+  //             512: 205 / 149 / 139
+  //   D = 256    32: 51 / 77 / 84    96: 89 / 129 / 140  256: 193 / 268 / 171
   const int64_t avg = R > 0 ? T * G / R : 0;
-  p.wide = avg > 96;
-  p.nt = p.wide ? wide_tiles((int)c.D) : avg > 16 ? 2 : 1;
-  p.waves = p.wide ? kWide : p.nt > 1 ? 4 : waves_of((int)c.D);
+  p.wide = avg > (c.D == 256 ? 224 : 448);
+  p.nt = p.wide ? wide_tiles((int)c.D) : c.D < 256 && avg > 64 ? 2 : 1;
+  p.waves = p.wide ? kWide : p.nt == 2 ? 4 : waves_of((int)c.D);
   const int64_t cols = p.cols();
   p.tiles_per_req = (int)((G + cols - 1) / cols);
   const int64_t tiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
-  // Contexts that no share would be smaller than are not cut.
-  p.whole = max_seq <= kMinShare * 32 * p.waves;
+  p.whole = max_seq <= (p.wide ? kWideWhole * 32 : kWhole * 32 * p.waves);
   p.wgs = p.whole ? tiles * c.heads : (p.wide ? 1 : 2) * (int64_t)device_shape().cus;
   return p;
 }
@@ -1338,7 +1347,7 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
          x.tables, x.table_stride, x.seq, x.cu_q, (uint16_t*)x.out, x.lse, nullptr, nullptr,
          nullptr, FastDiv((uint32_t)c.block_size), FastDiv((uint32_t)G), (uint32_t)c.num_blocks,
          (int)c.heads, (int)x.H, G, (int)x.T, (int)x.R, (int)x.max_seq, (int)x.causal,
-         (int)p.whole, kMinShare / 2, p.tiles_per_req,
+         (int)p.whole, kMinShare, p.tiles_per_req,
          // (of scores times 0 the masked ones would be NaN)
          std::max(std::fabs(x.sm_scale) * kLog2e, 1e-30f),
          std::signbit(x.sm_scale) ? 0x80008000u : 0u};
@@ -1351,8 +1360,9 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
   return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     constexpr int DT = dt.value, DD = d.value;
     if (p.wide) return launch_wide<DT, DD>(a, p, s);
-    return p.nt == 1 ? launch_split<DT, DD, 1, waves_of(DD)>(a, p, s)
-                     : launch_split<DT, DD, 2, 4>(a, p, s);
+    if constexpr (DD < 256)
+      if (p.nt == 2) return launch_split<DT, DD, 2, 4>(a, p, s);
+    return launch_split<DT, DD, 1, waves_of(DD)>(a, p, s);
   });
 }
 
