@@ -295,7 +295,8 @@ def test_decode_long(kv4, dtype, bs):
 
 @pytest.mark.parametrize("dtype,D,heads,G,bs", [
     (BF16, 128, 2, 4, 16), (F16, 64, 3, 1, 32), (F16, 256, 1, 8, 48), (BF16, 64, 1, 16, 128),
-    (BF16, 128, 1, 7, 64), (BF16, 256, 2, 2, 16)])
+    (BF16, 128, 1, 7, 64), (BF16, 256, 2, 2, 16), (BF16, 128, 1, 32, 16), (F16, 64, 2, 24, 48),
+    (F16, 256, 1, 16, 64), (F16, 128, 2, 33, 32), (BF16, 256, 1, 24, 16)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_several_queries(kv4, dtype, D, heads, G, bs, causal):
     """Drafted tokens and prompts, ragged: none, one, a few and many queries,
@@ -318,7 +319,33 @@ def test_prompts(kv4, dtype, D, heads, G):
     _check_attend(kv4, cache, tables, q, seq, nq)
 
 
-@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("dtype,D,heads,G,n", [(BF16, 128, 1, 4, 1500), (F16, 64, 2, 2, 1300),
+                                              (F16, 256, 1, 2, 1200)])
+def test_long_prompts(kv4, dtype, D, heads, G, n):
+    """Prompts and prefixes that are cut into shares."""
+    seq, nq = [n, 20, 2100], [n, 20, 300]
+    cache, tables, g = _setup(seq, 32, heads, D, dtype, 5)
+    q = (1.5 * torch.randn(sum(nq), heads * G, D, generator=g)).to(dtype)
+    _check_attend(kv4, cache, tables, q, seq, nq)
+    _check_attend(kv4, cache, tables, q, seq, nq, causal=False)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("long", [40, 2600])
+def test_many_requests(kv4, ragged, long):
+    """More requests than a workgroup has threads, with and without cuts."""
+    rng = random.Random(long)
+    R = 1100
+    seq = [rng.choice([0, 1, 17, rng.randrange(40)]) for _ in range(R)]
+    seq[0] = seq[700] = seq[-1] = long
+    nq = [rng.choice([0, 1, 2, 3]) for _ in range(R)] if ragged else [1] * R
+    nq[700] = 1
+    cache, tables, g = _setup(seq, 16, 1, 64, BF16, 6)
+    q = torch.randn(sum(nq), 2, 64, generator=g).to(BF16)
+    _check_attend(kv4, cache, tables, q, seq, nq, decode=not ragged)
+
+
+@pytest.mark.parametrize("nq", [1, 40, 300])
 def test_missing_blocks_are_not_seen(kv4, nq):
     seq = [100, 60, 48]
     cache, tables, g = _setup(seq, 16, 2, 64, BF16, 4)
@@ -332,7 +359,7 @@ def test_missing_blocks_are_not_seen(kv4, nq):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("nq", [1, 70])
+@pytest.mark.parametrize("nq", [1, 70, 130])
 def test_extreme_scores_and_scales(kv4, dtype, nq):
     """Scores far apart in both directions, scales over the type's range,
     one dominating token, all scores equal."""
@@ -354,7 +381,7 @@ def test_extreme_scores_and_scales(kv4, dtype, nq):
     _check_attend(kv4, cache, tables, q, seq, [nq] * 4, sm_scale=0.0)
 
 
-@pytest.mark.parametrize("nq", [1, 70])
+@pytest.mark.parametrize("nq", [1, 70, 240])
 def test_values_that_are_not_finite_stay_where_they_are_seen(kv4, nq):
     seq = [90, 90]
     cache, tables, g = _setup(seq, 16, 1, 64, F16, 12)
@@ -394,7 +421,8 @@ def test_strides_streams_and_out(kv4):
     assert bool((none == 0).all())
 
 
-@pytest.mark.parametrize("nq,seq", [(1, [3000, 40]), (100, [300, 120])])
+@pytest.mark.parametrize("nq,seq", [(1, [3000, 40]), (100, [300, 120]), (250, [300, 270]),
+                                    (1, [120, 700])])
 def test_a_step_in_a_graph(kv4, nq, seq):
     """Tables, append, read and attention captured together and replayed with
     other lengths and inputs."""
