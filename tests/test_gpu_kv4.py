@@ -533,3 +533,19 @@ def test_refusals(kv4):
                  lambda: kv4.block_tables(s.cpu(), s, tb, s, 16, 3)):
         with pytest.raises(ValueError):
             call()
+
+
+# ------------------------------------------------------------ together
+
+def test_serving_example():
+    """Learned levels, tables, append and attention in a loop.  Sixteen levels
+    leave a normal vector's elements about a tenth off (their quantisation
+    error is 1% of the variance), and attention averages it."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                        "flash-kmeans-cuda_amd", "examples", "kv4_serving.py")
+    spec = importlib.util.spec_from_file_location("kv4_serving", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main(steps=3) < 0.2
