@@ -81,10 +81,13 @@ constexpr int kTable = 256 * kEntry;
 constexpr int kItem = 3;                   // granules that an item costs by itself
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
+// 1 / l for a sum of weights, 0 where nothing was seen; NaN stays.
+__device__ inline float inverse(float l) { return l != 0.f ? 1.f / l : 0.f; }
+
 // log(2^m l): the exponents of both are added before anything is rounded.
 __device__ inline float log_sum(float m, float l) {
   const int e = (int)(__float_as_uint(l) >> 23) - 127;
-  return l > 0.f ? (m + e) * kLn2 + __logf(ldexpf(l, -e)) : -INFINITY;
+  return l != 0.f ? (m + e) * kLn2 + __logf(ldexpf(l, -e)) : -INFINITY;
 }
 
 // Read by scalar loads: nothing writes it while the kernel runs.
@@ -836,7 +839,7 @@ kv4_split_kernel(const Args args) {
         }
         const int64_t at = (int64_t)row * a.H + head;
         if (!cut) {
-          const float f = sum > 0.f ? 1.f / sum : 0.f;
+          const float f = inverse(sum);
           uint2 w;
           w.x = pack2<DT>(v[0] * f, v[1] * f);
           w.y = pack2<DT>(v[2] * f, v[3] * f);
@@ -1081,7 +1084,7 @@ kv4_wide_kernel(const Args args) {
         column(a, y, row, head, i);
         if (row < 0) continue;
         if (!k.cut()) {
-          const float f = st.l[y] > 0.f ? 1.f / st.l[y] : 0.f;
+          const float f = inverse(st.l[y]);
           const int64_t at = (int64_t)row * a.H + head;
 #pragma unroll
           for (int u = 0; u < ND / 2; ++u) {
@@ -1124,7 +1127,7 @@ __device__ inline void write_joined(const Args& a, const int4& item, int col, in
   const int i = (int)a.gdiv.div(item.z + col);
   const int64_t at =
       (int64_t)(item.y + i) * a.H + (item.w & 0xffff) * a.G + (item.z + col - i * a.G);
-  const float f = l > 0.f ? 1.f / l : 0.f;
+  const float f = inverse(l);
   uint2 w;
   w.x = pack2<DT>(v[0] * f, v[1] * f);
   w.y = pack2<DT>(v[2] * f, v[3] * f);

@@ -396,6 +396,30 @@ def test_values_that_are_not_finite_stay_where_they_are_seen(kv4, nq):
     assert torch.equal(out[nq:], clean[nq:])
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nq", [1, 240])
+@pytest.mark.parametrize("where", ["key", "query"])
+def test_scores_that_are_not_numbers_show(kv4, dtype, nq, where):
+    """A NaN among what a row sees makes that row NaN, not 0, and no other."""
+    seq = [90, 90]
+    cache, tables, g = _setup(seq, 16, 1, 64, dtype, 13)
+    q = torch.randn(2 * nq, 2, 64, generator=g).to(dtype)
+    clean = _check_attend(kv4, cache, tables, q, seq, [nq] * 2).cpu()
+    sees = torch.zeros(2 * nq, 2, dtype=torch.bool)
+    if where == "key":
+        cache[2][tables[0, 5], 0, 4] = math.nan  # token 84
+        sees[:nq] = (torch.arange(90 - nq, 90) >= 84)[:, None]
+    else:
+        q[nq - 1, 1, 7] = math.nan
+        sees[nq - 1, 1] = True
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    out, lse = kv4.attend(q.cuda(), dev, tables.cuda(), i32(seq), i32([0, nq, 2 * nq]),
+                          return_lse=True)
+    assert torch.equal(torch.isnan(out.cpu()).all(-1), sees)
+    assert torch.equal(torch.isnan(lse.cpu()), sees)
+    assert torch.equal(out.cpu()[~sees], clean[~sees])
+
+
 def test_strides_streams_and_out(kv4):
     seq = [130, 77, 300]
     cache, tables, g = _setup(seq, 16, 2, 128, BF16, 6)
