@@ -357,12 +357,13 @@ kv4_read_kernel(const int32_t* __restrict__ slots, int T, int per_wg,
 }
 
 // Tokens per workgroup: about four workgroups (all that fit) per CU over all
-// heads, keys and values, in whole passes.
+// heads, keys and values, in whole passes; at most 2^20, so that an int holds it
+// for any T.
 int tokens_per_wg(int64_t T, int64_t heads, int D) {
   const int64_t vp = KT / (D / 8);
   const int64_t passes = (T + vp - 1) / vp * heads * 2;
   const int64_t want = 4 * (int64_t)device_shape().cus;
-  return (int)(vp * std::max<int64_t>(1, (passes + want - 1) / want));
+  return (int)std::min<int64_t>(vp * std::max<int64_t>(1, (passes + want - 1) / want), 1 << 20);
 }
 
 template <typename F>
