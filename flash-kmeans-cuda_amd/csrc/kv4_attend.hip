@@ -78,7 +78,10 @@ constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
                                            // a difference of two is no NaN
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
-constexpr int kItem = 3;                   // granules that an item costs by itself
+// Granules that an item costs by itself (us with 2 / 3 / 5 / 8: 64 ragged requests
+// 142 / 132 / 134 / 137, drafted tokens 38.9 / 38.5 / 40.4 / 44.1, prompts 399 /
+// 397 / 408 / 430).
+constexpr int kItem = 3;
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
 // 1 / l for a sum of weights, 0 where nothing was seen; NaN stays.
