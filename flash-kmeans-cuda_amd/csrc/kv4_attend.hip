@@ -74,8 +74,9 @@ __device__ inline float from16(uint32_t bits) {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
-                                           // a difference of two is no NaN
+constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that a
+                                           // difference of two is no NaN (products
+                                           // of it are kept finite: State::base2)
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
 // Granules that an item costs by itself (us with 2 / 3 / 5 / 8: 64 ragged requests
@@ -529,9 +530,13 @@ struct State {
       for (int d = 0; d < ND; ++d) o[y][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
-  // What the weights so far are relative to, as a power of two.
+  // What the weights so far are relative to, as a power of two.  Finite: of a
+  // column that has seen nothing m is kLowest, and with a scale above 1 the
+  // product would be -inf, from which a masked score's own -inf differs by NaN.
+  // (Nor +inf: of scores that large every weight would be 0 instead.)
   __device__ inline float base2(int y, float zscale) const {
-    return DT == FKC_F16 ? m[y] - 14.f : m[y] * zscale;
+    return DT == FKC_F16 ? m[y] - 14.f
+                         : __builtin_amdgcn_fmed3f(m[y] * zscale, kLowest, -kLowest);
   }
   // Scores s of 32 tokens (their halves' groups base, this lane's first token
   // tok) to weights, packed as the second product reads them.  masked: some

@@ -1,0 +1,74 @@
+"""The 4-bit cache's operators at the ends of their ranges: large score
+scales, steps padded far past their queries, rows of one token or head, slots
+that no cache has, the cache's fixed tensors, gradients."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import kv4_ref as ref
+from test_gpu_kv4 import BF16, F16, _check_attend, _setup, i32
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kv4():
+    from flash_kmeans_cuda import kv4
+    return kv4
+
+
+# ------------------------------------------------------------ score scales
+
+SCALES = [1.0, -1.0, 8.0, 0.7]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("sm_scale", SCALES)
+def test_large_score_scales_of_a_few_queries(kv4, dtype, D, sm_scale):
+    """Scales above ln 2, where a masked score's stand-in times the scale
+    leaves fp32: tiles past an earlier query's last token, queries that see
+    nothing beside some that do, 32 tokens in missing blocks, idle rows."""
+    seq, nq = [100, 3, 33, 0, 70, 290], [7, 5, 1, 1, 2, 3]
+    cache, tables, g = _setup(seq, 16, 2, D, dtype, D)
+    tables[4, 2:4] = -1
+    tables[5, 0:2] = cache[0].shape[0]
+    q = (1.5 * torch.randn(sum(nq) + 3, 6, D, generator=g)).to(dtype)
+    _check_attend(kv4, cache, tables, q, seq, nq, sm_scale=sm_scale)
+    _check_attend(kv4, cache, tables, q, seq, nq, sm_scale=sm_scale, causal=False)
+    one = [1] * len(seq)
+    _check_attend(kv4, cache, tables, q[:len(seq)], seq, one, decode=True, sm_scale=sm_scale)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("sm_scale", SCALES[:2])
+def test_large_score_scales_of_prompts(kv4, dtype, D, sm_scale):
+    """The same for prompts in shares, which begin past some rows' last
+    token, and for contexts cut over workgroups."""
+    seq, nq = [1300, 20, 1500], [1300, 20, 300]
+    cache, tables, g = _setup(seq, 32, 1, D, dtype, D + 1)
+    q = (1.5 * torch.randn(sum(nq), 2, D, generator=g)).to(dtype)
+    _check_attend(kv4, cache, tables, q, seq, nq, sm_scale=sm_scale)
+    seq, nq = [6000, 90, 2500], [7, 5, 1]
+    cache, tables, g = _setup(seq, 16, 1, D, dtype, D + 2)
+    tables[2, 4:100] = -1
+    q = (1.5 * torch.randn(sum(nq), 4, D, generator=g)).to(dtype)
+    _check_attend(kv4, cache, tables, q, seq, nq, sm_scale=sm_scale)
+
+
+@pytest.mark.parametrize("nq", [6, 240])
+def test_large_score_scales_of_missing_blocks(kv4, nq):
+    seq = [100, 60, 48]
+    cache, tables, g = _setup(seq, 16, 2, 64, BF16, 4)
+    tables[0, 2:4] = -1
+    tables[1, 0:2] = 2 ** 31 - 1
+    tables[2] = -1  # nothing left
+    q = torch.randn(3 * nq, 4, 64, generator=g).to(BF16)
+    for sm_scale in 1.0, -2.5:
+        out = _check_attend(kv4, cache, tables, q, seq, [nq] * 3, sm_scale=sm_scale)
+        assert bool((out[2 * nq:] == 0).all())
