@@ -27,6 +27,7 @@
 
 #include "device_util.hpp"
 #include "fkc_internal.hpp"
+#include "kv4_shares.hpp"
 
 namespace fkc {
 namespace {
@@ -79,10 +80,6 @@ constexpr float kLowest = -3.4028235e38f;  // below every score; finite, so that
                                            // of it are kept finite: State::base2)
 constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
-// Granules that an item costs by itself (us with 2 / 3 / 5 / 8: 64 ragged requests
-// 142 / 132 / 134 / 137, drafted tokens 38.9 / 38.5 / 40.4 / 44.1, prompts 399 /
-// 397 / 408 / 430).
-constexpr int kItem = 3;
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
 // 1 / l for a sum of weights, 0 where nothing was seen; NaN stays.
@@ -312,8 +309,7 @@ __device__ inline uint32_t lookup(uint32_t w, int b, uint32_t off) {
 // lengths of any mixture fill the chip evenly, a workgroup meets few heads
 // (whose tables it has to fill), and an item that is cut is joined afterwards.
 //
-// Tile j of a causal request sees about A + (j + 1) COLS / G tokens, A those in
-// front of its queries, so j tiles weigh a sum in closed form, from which a
+// j tiles of a request weigh a sum in closed form (kv4_shares.hpp), from which a
 // tile is found again without a list of them.  (A weight only has to be the
 // same for everyone; what a share takes is in tokens.)
 struct Item {
@@ -341,9 +337,7 @@ __device__ inline void request(const Args& a, int r, Tile& t, int& tiles) {
 // Weight of the first j tiles.
 template <int COLS, int GR>
 __device__ inline int weight(const Args& a, const Tile& t, int j) {
-  const int own = (a.causal ? max(t.end - t.nq, 0) : t.end) / GR + 1 + kItem;
-  if (!a.causal || j <= 1) return j * own;
-  return j * own + (int)((int64_t)COLS * j * (j + 1) / 2 / (a.G * GR));
+  return kv4_weight(COLS, GR, a.G, a.causal != 0, t.nq, t.end, j);
 }
 
 // Running sums of the requests' weights, THREADS slices of `per` requests.
@@ -1363,7 +1357,8 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
   const Plan p = make_plan(c, x.H, x.T, x.R, x.max_seq, x.cu_q != nullptr);
   const int G = (int)(x.H / c.heads);
   // Weights of a head's items are summed in 32 bits.
-  const int64_t most = x.max_seq / (p.wide ? 32 : 32 * p.waves) + 2 + kItem;
+  const int64_t most =
+      kv4_most_weight(p.cols(), p.wide ? wide_tokens((int)c.D) : 32 * p.waves, G, x.max_seq);
   if (p.wgs > INT32_MAX || x.T * G / p.cols() + x.R + 1 > INT32_MAX / most)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   Args a{(const uint16_t*)x.q.p, x.q.token_stride, x.q.head_stride,

@@ -72,3 +72,26 @@ def test_large_score_scales_of_missing_blocks(kv4, nq):
     for sm_scale in 1.0, -2.5:
         out = _check_attend(kv4, cache, tables, q, seq, [nq] * 3, sm_scale=sm_scale)
         assert bool((out[2 * nq:] == 0).all())
+
+
+# ------------------------------------------------------------ padded steps
+
+@pytest.mark.parametrize("dtype,D,G", [(BF16, 128, 4), (F16, 64, 1), (F16, 256, 2)])
+def test_rows_of_no_request_beside_cut_ones(kv4, dtype, D, G):
+    """Steps padded to many times their queries, and requests with many more
+    queries than tokens, where the work is cut into shares: those rows are 0,
+    the others what they are without them."""
+    seq, nq = [1300, 40, 0, 5], [300, 900, 500, 1]
+    cache, tables, g = _setup(seq, 64, 2, D, dtype, 3)
+    q = (1.5 * torch.randn(9000, 2 * G, D, generator=g)).to(dtype)
+    out = _check_attend(kv4, cache, tables, q, seq, nq)
+    assert bool((out[sum(nq):] == 0).all())
+
+
+def test_a_padded_step_of_single_tokens(kv4):
+    """Many requests' worth of padding behind a few single tokens."""
+    seq, nq = [5000, 0, 700], [1, 1, 1]
+    cache, tables, g = _setup(seq, 16, 2, 128, BF16, 3)
+    q = torch.randn(700, 8, 128, generator=g).to(BF16)
+    out = _check_attend(kv4, cache, tables, q, seq, nq)
+    assert bool((out[3:] == 0).all())
