@@ -79,9 +79,14 @@ def _rows(name: str, t: torch.Tensor, heads: int, cache: "Cache") -> torch.Tenso
         raise RuntimeError(f"{name} must be (T, {heads or 'H'}, {cache.head_dim})")
     a, b, c = t.stride()
     if c != 1 or a % 8 or b % 8 or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:  # a dense view at an odd offset
-            t = t.clone()
+        T, H, D = t.shape
+        # the stride of a dimension of one entry is never used: 0 does as well
+        a, b = a if T > 1 else 0, b if H > 1 else 0
+        if c != 1 or a % 8 or b % 8 or t.data_ptr() % 16:
+            # (contiguous() and clone() may keep such strides, or the offset)
+            t = torch.empty((T, H, D), dtype=t.dtype, device=t.device).copy_(t)
+        else:
+            t = t.as_strided((T, H, D), (a, b, 1))
     return t
 
 

@@ -95,3 +95,31 @@ def test_a_padded_step_of_single_tokens(kv4):
     q = torch.randn(700, 8, 128, generator=g).to(BF16)
     out = _check_attend(kv4, cache, tables, q, seq, nq)
     assert bool((out[3:] == 0).all())
+
+
+# ------------------------------------------------------------ strides of one row
+
+@pytest.mark.parametrize("T,H", [(1, 1), (1, 3), (5, 1)])
+def test_strides_of_single_rows_do_not_matter(kv4, T, H):
+    """A dimension of one entry may have any stride: one token or one head out
+    of rows whose length is no multiple of eight."""
+    D = 128
+    g = torch.Generator().manual_seed(T + H)
+    levels = [ref.random_levels(H, BF16, i).cuda() for i in (1, 2)]
+    slots, tables, seq = i32(list(range(T))), i32([[0]] * T), i32(list(range(1, T + 1)))
+    dense = [torch.randn(T, H, D, generator=g).to(BF16).cuda() for _ in range(3)]
+
+    def odd(x, n):
+        step = [n if T == 1 else H * D, n if H == 1 else D, 1]
+        y = torch.zeros(4096, dtype=BF16, device="cuda").as_strided((T, H, D), step)
+        return y.copy_(x)
+
+    def step(q, k, v):
+        cache = kv4.Cache.empty(2, 16, D, *levels, BF16)
+        kv4.append(cache, k, v, slots)
+        return (*kv4.read(cache, slots), kv4.attend(q, cache, tables, seq))
+
+    want = step(*dense)
+    for n in 132, 129, 4, 1:
+        for a, b in zip(want, step(*(odd(x, n) for x in dense))):
+            assert torch.equal(a, b)
