@@ -122,8 +122,10 @@ block_tables_kernel(const int32_t* __restrict__ seq, const int32_t* __restrict__
           if (within == 0) *entry = blk;
         }
       }
-      if (i < num_tokens)
-        slots[i] = blk < 0 ? -1 : (int32_t)((uint32_t)blk * bs + within);
+      // (a block whose slots 31 bits do not hold has none: cut to 32, their
+      // numbers could be another block's)
+      const uint64_t slot = (uint64_t)(uint32_t)blk * bs + within;
+      if (i < num_tokens) slots[i] = blk < 0 || slot > INT32_MAX ? -1 : (int32_t)slot;
     }
     cu_base += ta;
     first_base += tb;

@@ -387,6 +387,7 @@ typedef struct fkc_kv4_cache {
  * slots has num_tokens entries; those past the last token are -1, and so are
  * the slots (and table entries) of a block that free_blocks does not reach,
  * of a position past max_blocks, and of a held block whose entry is negative.
+ * Slot numbers that 31 bits do not hold are -1 as well.
  * Tokens past num_tokens are dropped, but the table entries of their blocks
  * are written.  Negative lengths count as 0, new_lens past seq_lens as
  * seq_lens; the sums of both stay below 2^31.

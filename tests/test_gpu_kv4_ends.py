@@ -123,3 +123,23 @@ def test_strides_of_single_rows_do_not_matter(kv4, T, H):
     for n in 132, 129, 4, 1:
         for a, b in zip(want, step(*(odd(x, n) for x in dense))):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------ slots
+
+@pytest.mark.parametrize("bs", [16, 48, 128])
+def test_blocks_past_every_slot_give_no_slot(kv4, bs):
+    """A block whose slots 31 bits do not hold, in a table or on the free list,
+    gives -1, not another block's slots."""
+    top = (2 ** 31 - 1) // bs  # the last slot of block top - 1 fits
+    seq, new = [bs + 3, bs + 3, 2 * bs, 5], [3, 3, bs, 2]
+    tables = torch.tensor([[0, -1], [0, -1], [0, -1], [0, -1]], dtype=torch.int32)
+    tables[3, 0] = -(-2 ** 32 // bs)  # its slots would wrap around to the first ones
+    free = [2 ** 31 - 1, top - 1, 2 ** 31 // bs + 1]
+    tb = tables.cuda()
+    slots, cu, taken = kv4.block_tables(i32(seq), i32(new), tb, i32(free), bs, sum(new))
+    got = slots.tolist()
+    assert got[:3] == [-1] * 3
+    assert got[3:6] == [(top - 1) * bs + i for i in range(3)]
+    assert got[6:] == [-1] * (bs + 2)
+    assert tb[:3, 1].tolist() == free and taken.tolist() == [3]
