@@ -106,6 +106,9 @@ class Cache:
     (num_blocks, heads, block_size) and k_levels, v_levels (heads, 16) of one
     dtype, fp16 or bf16.  D is 64, 128 or 256, block_size a multiple of 16.
     A token's slot is block * block_size + its position in the block.
+
+    The calls go on reading the tensors that the cache was made of: what they
+    hold may be written, but none of them, nor any size, can be replaced.
     """
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scales: torch.Tensor,
@@ -139,6 +142,14 @@ class Cache:
                           self.heads, self.block_size, self.head_dim,
                           _lib.dtype_code(self.dtype))
         self._ref = ctypes.addressof(self._c)
+
+    def __setattr__(self, name: str, value: object) -> None:
+        if name in self.__dict__:
+            raise AttributeError(f"a cache's {name} cannot be replaced: make another Cache")
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name: str) -> None:
+        raise AttributeError(f"a cache's {name} cannot be taken from it")
 
     @classmethod
     def empty(cls, num_blocks: int, block_size: int, head_dim: int, k_levels: torch.Tensor,

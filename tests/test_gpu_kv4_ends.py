@@ -143,3 +143,27 @@ def test_blocks_past_every_slot_give_no_slot(kv4, bs):
     assert got[3:6] == [(top - 1) * bs + i for i in range(3)]
     assert got[6:] == [-1] * (bs + 2)
     assert tb[:3, 1].tolist() == free and taken.tolist() == [3]
+
+
+# ------------------------------------------------------------ the cache's tensors
+
+def test_a_cache_keeps_its_tensors(kv4):
+    """The kernels go on reading the tensors a cache was made of: none of them,
+    and no size, can be replaced or dropped."""
+    lv = ref.random_levels(2, BF16, 0).cuda()
+    c = kv4.Cache.empty(4, 16, 64, lv, lv, BF16)
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_levels", "v_levels",
+                 "num_blocks", "heads", "block_size", "head_dim", "dtype", "device"):
+        old = getattr(c, name)
+        with pytest.raises(AttributeError, match=name):
+            setattr(c, name, old)
+        with pytest.raises(AttributeError, match=name):
+            delattr(c, name)
+        assert getattr(c, name) is old
+    c.k_levels.copy_(-lv)  # their values are the caller's
+    x = torch.randn(3, 2, 64, device="cuda").to(BF16)
+    kv4.append(c, x, x, i32([0, 1, 2]))
+    other = kv4.Cache.empty(4, 16, 64, -lv, lv, BF16)
+    kv4.append(other, x, x, i32([0, 1, 2]))
+    for a, b in zip(kv4.read(c, i32([0, 1, 2])), kv4.read(other, i32([0, 1, 2]))):
+        assert torch.equal(a, b)
