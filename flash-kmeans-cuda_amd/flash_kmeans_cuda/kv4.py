@@ -20,6 +20,9 @@ them new:
 
 `tables` is updated in place.  Lengths, tables and slots stay on the GPU:
 nothing here waits for it.
+
+The cache holds codes, which have no gradient: `append` and `read` take and give
+values only, and going back through `attend` raises.
 """
 
 from __future__ import annotations
@@ -252,6 +255,20 @@ def read(cache: Cache, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]
     return k, v
 
 
+class _NoGradient(torch.autograd.Function):
+    """Puts attend's results into the graph of its queries, so that a gradient
+    that would have to pass through them raises instead of being left out."""
+
+    @staticmethod
+    def forward(ctx, q, *results):
+        ctx.mark_dirty(*results)
+        return results
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("kv4.attend has no gradient: detach q, or call it under no_grad")
+
+
 def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.Tensor,
            cu_q: Optional[torch.Tensor] = None, *, causal: bool = True,
            sm_scale: Optional[float] = None, max_seq: Optional[int] = None,
@@ -268,7 +285,8 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
     seq_lens that the caller knows (the tables' width otherwise); longer
     requests are cut to it.  Returns (T, H, D) in q's dtype, in `out` when
     given, and with return_lse also log sum exp of each row's scores, fp32
-    (T, H), -inf for rows that see nothing.
+    (T, H), -inf for rows that see nothing.  There is no gradient: going back
+    through the result of a q that requires one raises RuntimeError.
     """
     q = _rows("q", q, 0, cache)
     dev = cache.device
@@ -302,4 +320,9 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
             cache._ref, q.data_ptr(), q.stride(0), q.stride(1), H, T, tables.data_ptr(), stride,
             width, seq_lens.data_ptr(), _lib.ptr(cu_q), R, max_seq, int(causal), sm_scale,
             out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need, _lib.stream_of(q)), "attend")
+    if q.requires_grad and torch.is_grad_enabled():
+        if lse is not None:
+            out, lse = _NoGradient.apply(q, out, lse)
+        else:
+            out, = _NoGradient.apply(q, out)
     return (out, lse) if return_lse else out

@@ -167,3 +167,32 @@ def test_a_cache_keeps_its_tensors(kv4):
     kv4.append(other, x, x, i32([0, 1, 2]))
     for a, b in zip(kv4.read(c, i32([0, 1, 2])), kv4.read(other, i32([0, 1, 2]))):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------ gradients
+
+def test_a_gradient_through_the_cache_is_refused(kv4):
+    """Attention over codes has no gradient: its result belongs to q's graph,
+    and going back through it raises instead of leaving q's out."""
+    lv = ref.random_levels(2, BF16, 0).cuda()
+    c = kv4.Cache.empty(4, 16, 64, lv, lv, BF16)
+    x = torch.randn(3, 2, 64, device="cuda").to(BF16)
+    s, tb = i32([1, 1, 1]), i32([[0], [1], [2]])
+    kv4.append(c, x, x, i32([0, 16, 32]))
+    want, want_lse = kv4.attend(x, c, tb, s, return_lse=True)
+    assert not want.requires_grad and not want_lse.requires_grad
+    q = x.clone().requires_grad_()
+    out, lse = kv4.attend(q * 1, c, tb, s, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    for y in out, lse, kv4.attend(q, c, tb, s), kv4.attend(q.transpose(0, 1).contiguous()
+                                                           .transpose(0, 1), c, tb, s):
+        with pytest.raises(RuntimeError, match="gradient"):
+            (y.float().sum() + q.float().sum()).backward()
+    room = torch.empty_like(x)
+    held = kv4.attend(q, c, tb, s, out=room)
+    assert held is room and torch.equal(room, want)
+    with pytest.raises(RuntimeError, match="gradient"):
+        held.float().sum().backward()
+    with torch.no_grad():
+        assert not kv4.attend(q, c, tb, s).requires_grad
+    assert not kv4.attend(q.detach(), c, tb, s).requires_grad
