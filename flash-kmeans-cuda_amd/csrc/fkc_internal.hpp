@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "fkc.h"
 
 namespace fkc {
@@ -231,6 +233,17 @@ int launch_block_tables(const int32_t* seq, const int32_t* nw, int R,
                         const int32_t* free_blocks, int64_t num_free,
                         int block_size, int64_t num_tokens, int32_t* slots,
                         int32_t* cu_new, int32_t* taken, hipStream_t s);
+// f(dtype, D) as compile-time constants.
+template <typename F>
+int kv4_by_shape(int dtype, int64_t D, F&& f) {
+  auto with = [&](auto dt) {
+    if (D == 64) return f(dt, std::integral_constant<int, 64>{});
+    if (D == 128) return f(dt, std::integral_constant<int, 128>{});
+    return f(dt, std::integral_constant<int, 256>{});
+  };
+  return dtype == FKC_F16 ? with(std::integral_constant<int, FKC_F16>{})
+                          : with(std::integral_constant<int, FKC_BF16>{});
+}
 struct Kv4Rows {
   const void* p;
   int64_t token_stride, head_stride;

@@ -1240,17 +1240,6 @@ kv4_join_kernel(const Args a) {
   }
 }
 
-template <typename F>
-int by_shape(int dtype, int64_t D, F&& f) {
-  auto with = [&](auto dt) {
-    if (D == 64) return f(dt, std::integral_constant<int, 64>{});
-    if (D == 128) return f(dt, std::integral_constant<int, 128>{});
-    return f(dt, std::integral_constant<int, 256>{});
-  };
-  return dtype == FKC_F16 ? with(std::integral_constant<int, FKC_F16>{})
-                          : with(std::integral_constant<int, FKC_BF16>{});
-}
-
 // Granules of a share at least, and up to how many granules a context is never
 // cut: every item then goes to a workgroup of its own, and nothing has to be
 // joined by a second kernel.  (bf16, D = 128, 8 heads, 4 query heads each, one
@@ -1378,7 +1367,7 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
     a.part_ml = w.take<float>(p.part_rows() * 2);
     a.desc = w.take<int4>((size_t)p.wgs);
   }
-  return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
+  return kv4_by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     constexpr int DT = dt.value, DD = d.value;
     if (p.wide) return launch_wide<DT, DD>(a, p, s);
     if constexpr (DD < 256)

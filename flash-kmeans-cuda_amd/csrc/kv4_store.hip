@@ -366,23 +366,12 @@ int tokens_per_wg(int64_t T, int64_t heads, int D) {
   return (int)std::min<int64_t>(vp * std::max<int64_t>(1, (passes + want - 1) / want), 1 << 20);
 }
 
-template <typename F>
-int by_shape(int dtype, int64_t D, F&& f) {
-  auto with = [&](auto dt) {
-    if (D == 64) return f(dt, std::integral_constant<int, 64>{});
-    if (D == 128) return f(dt, std::integral_constant<int, 128>{});
-    return f(dt, std::integral_constant<int, 256>{});
-  };
-  return dtype == FKC_F16 ? with(std::integral_constant<int, FKC_F16>{})
-                          : with(std::integral_constant<int, FKC_BF16>{});
-}
-
 }  // namespace
 
 int launch_kv4_append(const fkc_kv4_cache& c, Kv4Rows k, Kv4Rows v,
                       const int32_t* slots, int64_t T, hipStream_t s) {
   if (c.num_blocks == 0) return FKC_OK;  // no slot is inside
-  return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
+  return kv4_by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     const int per = tokens_per_wg(T, c.heads, d.value);
     const dim3 grid((uint32_t)((T + per - 1) / per), (uint32_t)c.heads, 2);
     hipLaunchKernelGGL((kv4_append_kernel<dt.value, d.value>), grid, dim3(KT), 0, s, k, v,
@@ -397,7 +386,7 @@ int launch_kv4_append(const fkc_kv4_cache& c, Kv4Rows k, Kv4Rows v,
 
 int launch_kv4_read(const fkc_kv4_cache& c, const int32_t* slots, int64_t T,
                     void* k_out, void* v_out, hipStream_t s) {
-  return by_shape(c.dtype, c.D, [&](auto dt, auto d) {
+  return kv4_by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     const int per = tokens_per_wg(T, c.heads, d.value);
     const dim3 grid((uint32_t)((T + per - 1) / per), (uint32_t)c.heads, 2);
     hipLaunchKernelGGL((kv4_read_kernel<dt.value, d.value>), grid, dim3(KT), 0, s, slots,
