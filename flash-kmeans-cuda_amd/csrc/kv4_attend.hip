@@ -503,7 +503,14 @@ struct Walk {
 // would run for every tile).
 __device__ inline void rare(float& v) { asm volatile("" : "+v"(v)); }
 
-// A wave's NT tiles of 16 columns: outputs and running maxima and sums.
+// A wave's NT tiles of 16 columns: outputs and running maxima and sums, all fp32.
+// What is rounded to the type is a weight times its value scale, for the second
+// product: matrix cores take both factors in 16 bits or both in 32 at a sixteenth
+// of the rate.  The sum of weights is that of the unrounded ones, so each term of
+// an output is off by half a unit in the last place at most, and these errors
+// average out: relative to 64-bit results single bf16 tokens are 1.69e-3 off and
+// prompts 1.76e-3, of which 1.66e-3 is the rounding of the result, fp16 prompts of 256
+// columns 2.16e-4 and 2.07e-4.
 //   bf16: m is the largest score before its (positive) scale zscale, and a
 // weight is 2^(z zscale - m zscale).
 //   fp16 has few exponents, and a token's value scale is part of what is rounded
@@ -742,8 +749,9 @@ kv4_split_kernel(const Args args) {
     st.clear();
     // What a tile has used up is fetched for the next one at once, after the last
     // tile slot 0's (a load that may or may not be on its way would have to be
-    // waited for with every older one), into the same registers: with a second set of them four waves a SIMD do not fit,
-    // and it is they that hide the loads' latency.
+    // waited for with every older one), into the same registers: with a second
+    // set of them four waves a SIMD do not fit, and it is they that hide the loads'
+    // latency.
     for (int it = wave; it < ntile; it += WAVES) {
       groups(it + WAVES, blk, nbase);
       load_blocks(it + 2 * WAVES, blk);
@@ -870,14 +878,18 @@ kv4_split_kernel(const Args args) {
 // in a row (16 bytes each, no bank conflict), in one of two buffers; while a
 // tile is computed on, the next one is filled into the other.
 //
-// Bound by the LDS reads of those fragments (1 KB for NT products) and the
-// vector unit's work on the scores (about nine operations and an exponential
-// each): ragged prompts of 700 to 4096 tokens, 32 heads of 128 columns, bf16, take
-// 393 us (0.5 PFLOP/s), 370 if the buffers are not filled, 296 if the scores
-// are packed as they are, 247 with neither; D = 256, where NT = 1, 1081 / 890 /
-// 1024 / 918.  Four waves with NT = 4, or NT = 3, need more registers than the
-// compiler finds (spills cost more than the reads), and waves that look up
-// for themselves measured 420 and 1264.
+// No unit is busy half of the time; what bounds it is that a wave's phases (score
+// products, softmax, value products of 32 tokens) follow one another with two
+// waves a SIMD to overlap them, and all eight meet at a barrier every TT tokens.
+// Ragged prompts of 700 to 4096 tokens, 32 heads of 128 columns, bf16, 366 us a call
+// (0.52 PFLOP/s): vector unit 46%, matrix cores 21%, LDS 18%, waves waiting for
+// data or a barrier 37% and for an issue slot 22%; 341 if the buffers are neither
+// loaded nor filled, 289 if the scores are packed as they are, 228 with neither.
+// D = 256, where NT = 1 and a fragment of 1 KB feeds one product, 12000 to 16000
+// tokens: 1002 us, 45 / 21 / 32 / 36 / 24%; 807 / 851 / 741.  Four waves with NT = 4,
+// or NT = 3, need more registers than the compiler finds (spills cost more than
+// the reads); waves that looked up for themselves were slower (prompts 438 to 420
+// then, D = 256 1264 to 1044).
 //
 // Feature row n of fragment d of the second product is feature 32 (d / 2) + 2 n +
 // d % 2: the two codes of one byte go to two fragments, and 16 lanes read 16

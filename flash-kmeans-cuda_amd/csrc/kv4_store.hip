@@ -10,10 +10,10 @@
 // time of those bytes has room for.  Sixteen distances, compares and selects
 // are 64, halving the sorted levels' 15 thresholds 33; one look into a table of
 // y's CELLS cells, each with the one threshold that falls into it, is 10.
-// Measured: 32768 tokens of 16 heads of 64 columns, bf16, keys and values, 48.8 us
-// (170 MB, 3.5 TB/s; with sixteen distances 366 us) and reading them back 35.1
-// (4.9 TB/s); 8191 tokens of 8 heads of 128, fp16, 15.1 and 10.8; 64 tokens 5.8
-// and 3.5, of which the table's making (loads, sorting, a search) is about 3.
+// Measured: 32768 tokens of 16 heads of 64 columns, bf16, keys and values, 48.7 us
+// (170 MB, 3.5 TB/s; with sixteen distances 366 us) and reading them back 36.1
+// (4.7 TB/s); 8191 tokens of 8 heads of 128, fp16, 14.5 and 10.7; 64 tokens 5.8
+// and 3.6, of which the table's making (loads, sorting, a search) is about 3.
 #include <algorithm>
 #include <type_traits>
 

@@ -428,8 +428,9 @@ FKC_CAPI int fkc_kv4_read(const fkc_kv4_cache* cache, const int32_t* slots,
  * Attention of T queries over the cache.  q (T, H, D) of the cache's dtype,
  * strides in elements, rows of D contiguous and 16-byte aligned; query head h
  * reads cache head h / (H / heads).  Request r owns the queries
- * cu_q[r] .. cu_q[r+1] (cu_q NULL: T = R, one query each), which are its last
- * tokens: query i of n sits at position seq_lens[r] - n + i and sees the
+ * cu_q[r] .. cu_q[r+1] (cu_q R + 1 entries, ascending from 0 to T at most; rows
+ * past the last are rows that see nothing; NULL: T = R, one query each), which
+ * are its last tokens: query i of n sits at position seq_lens[r] - n + i and sees the
  * tokens up to it (causal) or all seq_lens[r] of them.  Token t lies in block
  * tables[r * table_stride + t / block_size]; tokens of a block outside the
  * cache are not seen.  Over the seen tokens
