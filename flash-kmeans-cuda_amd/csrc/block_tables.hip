@@ -118,7 +118,8 @@ block_tables_kernel(const int32_t* __restrict__ seq, const int32_t* __restrict__
           blk = *entry;
         } else {
           const int64_t f = (int64_t)s_first[x] + (j - h.have);
-          if (f < num_free) blk = free_blocks[f];
+          // (below 0 where lengths that make no sense sum past 31 bits)
+          if (f >= 0 && f < num_free) blk = free_blocks[f];
           if (within == 0) *entry = blk;
         }
       }

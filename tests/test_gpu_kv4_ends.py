@@ -196,3 +196,16 @@ def test_a_gradient_through_the_cache_is_refused(kv4):
     with torch.no_grad():
         assert not kv4.attend(q, c, tb, s).requires_grad
     assert not kv4.attend(q.detach(), c, tb, s).requires_grad
+
+
+# ------------------------------------------------------------ lengths past the sums
+
+def test_block_tables_of_lengths_past_31_bits(kv4):
+    """Lengths whose sums leave 31 bits (garbage in a padded row) reach no free
+    block, and nothing outside the free list is read."""
+    big = 2 ** 31 - 2  # two of them: 2^32 - 4 tokens, 2^31 - 2 blocks of two
+    seq = [big, big, 10, 8]
+    tb = torch.full((4, 3), 5, dtype=torch.int32, device="cuda")
+    slots, cu, taken = kv4.block_tables(i32(seq), i32(seq), tb, i32([7, 8, 9]), 2, 20)
+    assert slots.tolist() == [-1] * 20
+    assert tb[3].tolist() == [-1] * 3
