@@ -412,7 +412,9 @@ struct Shares {
     }
     const int w = weight<COLS, GR>(a, x.t, tile);
     x.n = weight<COLS, GR>(a, x.t, tile + 1) - w;
-    x.at = u - w;
+    // Query offsets that do not ascend can sum past 32 bits: within the item all
+    // the same, so that every share goes forward and ends.
+    x.at = min(max(u - w, 0), x.n - 1);
     x.t.col0 = tile * COLS;
     return x;
   }
@@ -1155,8 +1157,9 @@ kv4_join_kernel(const Args a) {
   constexpr int LPC = D / 4, CP = 256 / LPC, JC = 4, PARTS = 64, FEW = 4;
   __shared__ f32x4 so[256];
   __shared__ float sw[JC][PARTS];
-  const int4 item = a.desc[blockIdx.x];
+  int4 item = a.desc[blockIdx.x];
   if (item.x == 0) return;
+  item.x = min(item.x, (int)(gridDim.x - blockIdx.x));  // (see Shares::find)
   const int ncols = item.w >> 16;
   const int sub = threadIdx.x % LPC, part = threadIdx.x / LPC;
   // row of part c, column col in part and part_ml

@@ -209,3 +209,22 @@ def test_block_tables_of_lengths_past_31_bits(kv4):
     slots, cu, taken = kv4.block_tables(i32(seq), i32(seq), tb, i32([7, 8, 9]), 2, 20)
     assert slots.tolist() == [-1] * 20
     assert tb[3].tolist() == [-1] * 3
+
+
+def test_query_offsets_that_do_not_ascend_end(kv4):
+    """Offsets that go back and forth weigh every request as the whole step; the
+    sum leaves 32 bits.  What is computed is anything, but every share ends, and
+    the next call is as ever."""
+    T, R, bs = 65536, 7, 1 << 20
+    lv = ref.random_levels(1, BF16, 0).cuda()
+    c = kv4.Cache.empty(1, bs, 64, lv, lv, BF16)
+    q = torch.randn(T, 4, 64, device="cuda").to(BF16)
+    # four requests of 1024 tiles of 2^20 + 16 granules: 2^32 + 2^16 in all
+    tables = torch.full((R, 65), -1, dtype=torch.int32, device="cuda")
+    out = kv4.attend(q, c, tables, i32([64 * (2 ** 20 + 12)] * R),
+                     i32([0, T] * 4), causal=False)
+    torch.cuda.synchronize()
+    assert out.shape == (T, 4, 64)
+    seq, nq = [130, 40], [130, 3]
+    cache, tables, g = _setup(seq, 16, 1, 64, BF16, 3)
+    _check_attend(kv4, cache, tables, q[:133].cpu(), seq, nq)
