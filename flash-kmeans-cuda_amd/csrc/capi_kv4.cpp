@@ -68,6 +68,53 @@ int attend_sizes_ok(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R,
   return FKC_OK;
 }
 
+int tables_ok(const int32_t* tables, int64_t stride, int64_t max_blocks,
+              const int32_t* seq, int64_t R, const char* what) {
+  if (R < 0 || R > kI32 || max_blocks < 0 || max_blocks > kI32)
+    return fail(FKC_ERR_INVALID, "%s: size out of range", what);
+  if (stride < max_blocks)
+    return fail(FKC_ERR_INVALID, "%s: rows of tables overlap", what);
+  if (R && (!seq || (max_blocks && !tables)))
+    return fail(FKC_ERR_INVALID, "%s: null pointer argument", what);
+  return FKC_OK;
+}
+
+int workspace_ok(const void* ws, size_t bytes, size_t need, const char* what) {
+  if (need && (!ws || bytes < need))
+    return fail(FKC_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", what, bytes, need);
+  if (need && reinterpret_cast<uintptr_t>(ws) % kWorkspaceAlign)
+    return fail(FKC_ERR_WORKSPACE, "%s: workspace not %d-byte aligned", what,
+                kWorkspaceAlign);
+  return FKC_OK;
+}
+
+// Blocks of one cache fit the other.
+int alike(const fkc_kv4_cache& a, const fkc_kv4_cache& b, const char* what) {
+  if (a.heads != b.heads || a.block_size != b.block_size || a.D != b.D || a.dtype != b.dtype)
+    return fail(FKC_ERR_INVALID,
+                "%s: the caches differ in heads, block_size, D or dtype", what);
+  // The kernels count the 16-byte units of a block in 32 bits.
+  if (a.block_size * a.heads > kI32 / (a.D + 4))
+    return fail(FKC_ERR_UNSUPPORTED, "%s: blocks of 2^31 bytes and more", what);
+  return FKC_OK;
+}
+
+bool overlap(const fkc_kv4_cache& a, const fkc_kv4_cache& b) {
+  const int64_t vectors = a.heads * a.block_size;
+  auto part = [&](const fkc_kv4_cache& c, int i, uintptr_t* lo) {
+    const void* p[] = {c.k_codes, c.v_codes, c.k_scales, c.v_scales};
+    *lo = reinterpret_cast<uintptr_t>(p[i]);
+    return *lo + (uintptr_t)(c.num_blocks * vectors * (i < 2 ? c.D / 2 : 2));
+  };
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) {
+      uintptr_t lo, lo2;
+      const uintptr_t hi = part(a, i, &lo), hi2 = part(b, j, &lo2);
+      if (lo < hi2 && lo2 < hi) return true;
+    }
+  return false;
+}
+
 }  // namespace
 }  // namespace fkc
 
@@ -173,6 +220,109 @@ int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
                     causal != 0, sm_scale, out, lse};
   return launch_kv4_attend(*cache, a, workspace, workspace_bytes,
                            reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t fkc_free_blocks_workspace_bytes(int64_t num_blocks) {
+  clear_error();
+  if (num_blocks < 0 || num_blocks > kI32) {
+    fail(FKC_ERR_INVALID, "free_blocks_workspace_bytes: size out of range");
+    return 0;
+  }
+  return free_blocks_workspace_bytes(num_blocks);
+}
+
+int fkc_free_blocks(const int32_t* tables, int64_t table_stride, int64_t max_blocks,
+                    const int32_t* seq_lens, int64_t R, int64_t block_size,
+                    int64_t num_blocks, int32_t* free_blocks, int32_t* count,
+                    void* workspace, size_t workspace_bytes, fkc_stream_t stream) {
+  clear_error();
+  if (int rc = tables_ok(tables, table_stride, max_blocks, seq_lens, R, "free_blocks"))
+    return rc;
+  if (block_size < 1 || block_size > (1 << 20) || num_blocks < 0 || num_blocks > kI32)
+    return fail(FKC_ERR_INVALID, "free_blocks: size out of range");
+  if (!count || (num_blocks && !free_blocks))
+    return fail(FKC_ERR_INVALID, "free_blocks: null pointer argument");
+  if (int rc = workspace_ok(workspace, workspace_bytes,
+                            free_blocks_workspace_bytes(num_blocks), "free_blocks"))
+    return rc;
+  return launch_free_blocks({tables, table_stride, max_blocks, seq_lens, R}, block_size,
+                            num_blocks, free_blocks, count, workspace,
+                            reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t fkc_kv4_fork_workspace_bytes(const fkc_kv4_cache* cache, int64_t F) {
+  clear_error();
+  if (cache_ok(cache, "kv4_fork_workspace_bytes")) return 0;
+  if (F < 0 || F > kI32) {
+    fail(FKC_ERR_INVALID, "kv4_fork_workspace_bytes: F out of range");
+    return 0;
+  }
+  return kv4_fork_workspace_bytes(*cache, F);
+}
+
+int fkc_kv4_fork(const fkc_kv4_cache* cache, const int32_t* tables, int64_t table_stride,
+                 int64_t max_blocks, const int32_t* seq_lens, int64_t R,
+                 const int32_t* parents, int64_t F, const int32_t* free_blocks,
+                 int64_t num_free, int32_t* new_tables, int32_t* new_seq, int32_t* taken,
+                 void* workspace, size_t workspace_bytes, fkc_stream_t stream) {
+  clear_error();
+  if (int rc = cache_ok(cache, "kv4_fork")) return rc;
+  if (int rc = alike(*cache, *cache, "kv4_fork")) return rc;
+  if (int rc = tables_ok(tables, table_stride, max_blocks, seq_lens, R, "kv4_fork"))
+    return rc;
+  if (F < 0 || F > kI32 || num_free < 0)
+    return fail(FKC_ERR_INVALID, "kv4_fork: size out of range");
+  if (!taken || (F && (!parents || !new_seq || (max_blocks && !new_tables))) ||
+      (num_free && !free_blocks))
+    return fail(FKC_ERR_INVALID, "kv4_fork: null pointer argument");
+  if (int rc = workspace_ok(workspace, workspace_bytes, kv4_fork_workspace_bytes(*cache, F),
+                            "kv4_fork"))
+    return rc;
+  return launch_kv4_fork(*cache, {tables, table_stride, max_blocks, seq_lens, R}, parents, F,
+                         free_blocks, num_free, new_tables, new_seq, taken, workspace,
+                         reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t fkc_kv4_compact_workspace_bytes(const fkc_kv4_cache* cache) {
+  clear_error();
+  return cache_ok(cache, "kv4_compact_workspace_bytes") ? 0
+                                                        : kv4_compact_workspace_bytes(*cache);
+}
+
+int fkc_kv4_compact(const fkc_kv4_cache* cache, const int32_t* tables, int64_t table_stride,
+                    int64_t max_blocks, const int32_t* seq_lens, int64_t R,
+                    const fkc_kv4_cache* into, int32_t* new_tables, int32_t* used,
+                    void* workspace, size_t workspace_bytes, fkc_stream_t stream) {
+  clear_error();
+  if (int rc = cache_ok(cache, "kv4_compact")) return rc;
+  if (int rc = cache_ok(into, "kv4_compact")) return rc;
+  if (int rc = alike(*cache, *into, "kv4_compact")) return rc;
+  if (overlap(*cache, *into))
+    return fail(FKC_ERR_INVALID, "kv4_compact: the caches share memory");
+  if (int rc = tables_ok(tables, table_stride, max_blocks, seq_lens, R, "kv4_compact"))
+    return rc;
+  if (!used || (R && max_blocks && !new_tables))
+    return fail(FKC_ERR_INVALID, "kv4_compact: null pointer argument");
+  if (int rc = workspace_ok(workspace, workspace_bytes, kv4_compact_workspace_bytes(*cache),
+                            "kv4_compact"))
+    return rc;
+  return launch_kv4_compact(*cache, {tables, table_stride, max_blocks, seq_lens, R}, *into,
+                            new_tables, used, workspace,
+                            reinterpret_cast<hipStream_t>(stream));
+}
+
+int fkc_kv4_copy_blocks(const fkc_kv4_cache* cache, const int32_t* src,
+                        const fkc_kv4_cache* into, const int32_t* dst, int64_t n,
+                        fkc_stream_t stream) {
+  clear_error();
+  if (int rc = cache_ok(cache, "kv4_copy_blocks")) return rc;
+  if (int rc = cache_ok(into, "kv4_copy_blocks")) return rc;
+  if (int rc = alike(*cache, *into, "kv4_copy_blocks")) return rc;
+  if (n < 0 || n > kI32) return fail(FKC_ERR_INVALID, "kv4_copy_blocks: n out of range");
+  if (n == 0 || cache->num_blocks == 0 || into->num_blocks == 0) return FKC_OK;
+  if (!src || !dst) return fail(FKC_ERR_INVALID, "kv4_copy_blocks: null pointer argument");
+  return launch_kv4_copy_blocks(*cache, src, *into, dst, n,
+                                reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

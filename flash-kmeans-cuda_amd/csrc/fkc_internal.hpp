@@ -269,6 +269,30 @@ size_t kv4_attend_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int64_t T,
                                   int64_t R, int64_t max_seq);
 int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& a, void* ws,
                       size_t ws_bytes, hipStream_t s);
+// Pages: tables of R rows over block numbers, with the rows' lengths.
+struct Kv4Tables {
+  const int32_t* tables;
+  int64_t stride, max_blocks;
+  const int32_t* seq;
+  int64_t R;
+};
+size_t free_blocks_workspace_bytes(int64_t num_blocks);
+int launch_free_blocks(const Kv4Tables& t, int64_t block_size, int64_t num_blocks,
+                       int32_t* free_blocks, int32_t* count, void* ws,
+                       hipStream_t s);
+size_t kv4_fork_workspace_bytes(const fkc_kv4_cache& c, int64_t F);
+int launch_kv4_fork(const fkc_kv4_cache& c, const Kv4Tables& t,
+                    const int32_t* parents, int64_t F,
+                    const int32_t* free_blocks, int64_t num_free,
+                    int32_t* new_tables, int32_t* new_seq, int32_t* taken,
+                    void* ws, hipStream_t s);
+size_t kv4_compact_workspace_bytes(const fkc_kv4_cache& c);
+int launch_kv4_compact(const fkc_kv4_cache& c, const Kv4Tables& t,
+                       const fkc_kv4_cache& into, int32_t* new_tables,
+                       int32_t* used, void* ws, hipStream_t s);
+int launch_kv4_copy_blocks(const fkc_kv4_cache& c, const int32_t* src,
+                           const fkc_kv4_cache& into, const int32_t* dst,
+                           int64_t n, hipStream_t s);
 
 // ---------------------------------------------------------------- loop
 // The Lloyd loop behind fkc_kmeans_lloyd*; profile = false ignores the

@@ -66,7 +66,7 @@ def _check_tables(t: torch.Tensor, R: int, device: torch.device) -> Tuple[int, i
     _require(t.dtype is torch.int32 and t.dim() == 2, "tables must be int32 (R, max_blocks)")
     rows, width = t.shape
     stride, dense = t.stride()
-    _require(rows == R and (width <= 1 or dense == 1),
+    _require(rows == R and (width <= 1 or dense == 1 or rows == 0),
              f"tables must be ({R}, max_blocks) with dense rows")
     return width, stride if rows > 1 else width
 
@@ -330,3 +330,113 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
         else:
             out, = _NoGradient.apply(q, out)
     return (out, lse) if return_lse else out
+
+
+def free_blocks(tables: torch.Tensor, seq_lens: torch.Tensor, block_size: int, num_blocks: int
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The blocks that no row holds; -> (free, count).
+
+    Row r of tables (R, max_blocks) holds its first ceil(seq_lens[r] /
+    block_size) entries; a request that is over gives its blocks back with a
+    length of 0, one that is cut back with a smaller one, and a block that
+    several rows hold is free when the last has let go.  free (num_blocks,)
+    int32 lists the free blocks in ascending order, -1 behind them, as
+    `block_tables` takes it; count (1) int32 is how many there are.
+    """
+    dev = seq_lens.device
+    if dev.type != "cuda":
+        _on_gpu("seq_lens", seq_lens)
+    seq_lens = _i32("seq_lens", seq_lens, 1, dev)
+    R = seq_lens.shape[0]
+    width, stride = _check_tables(tables, R, dev)
+    _require(num_blocks >= 0, "num_blocks must not be negative")
+    free, count = torch.split_with_sizes(seq_lens.new_empty(num_blocks + 1), (num_blocks, 1))
+    with _lib.on_device(seq_lens):
+        need = _lib.lib.fkc_free_blocks_workspace_bytes(num_blocks)
+        ws = _lib.workspace(need, dev)
+        _lib.check(_lib.lib.fkc_free_blocks(
+            tables.data_ptr(), stride, width, seq_lens.data_ptr(), R, block_size, num_blocks,
+            free.data_ptr(), count.data_ptr(), ws.data_ptr(), need, _lib.stream_of(seq_lens)),
+            "free_blocks")
+    return free, count
+
+
+def fork(cache: Cache, tables: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
+         free_blocks: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Rows that go on from others' tokens; -> (tables, seq_lens, taken).
+
+    Row j of the new tables (F, max_blocks) and lengths (F,) has the tokens of
+    row parents[j] (F,) int32: several samples of a prompt, the next beams of a
+    search; a parent that is no row (-1) gives a row without tokens.  Whole
+    blocks are shared.  A last block that is not full is appended to, so each
+    child needs its own: the first child that ends in a block keeps it, unless
+    another has it as a whole one, and every other child's becomes the next of
+    free_blocks, with a copy of what the block holds.  taken (1) int32 counts
+    the copies; where free_blocks does not reach, a child's entry is -1.  Rows
+    that no child goes on from give their blocks back (`free_blocks` of the new
+    tables).  After a cut (a smaller length) into blocks that other rows hold
+    too, fork all rows onto themselves before anything is appended.
+    """
+    dev = cache.device
+    seq_lens = _i32("seq_lens", seq_lens, 1, dev)
+    parents = _i32("parents", parents, 1, dev)
+    free_blocks = _i32("free_blocks", free_blocks, 1, dev)
+    R, F = seq_lens.shape[0], parents.shape[0]
+    width, stride = _check_tables(tables, R, dev)
+    new, seq, taken = torch.split_with_sizes(seq_lens.new_empty(F * width + F + 1),
+                                             (F * width, F, 1))
+    new = new.view(F, width)
+    with _lib.on_device(seq_lens):
+        need = _lib.lib.fkc_kv4_fork_workspace_bytes(cache._ref, F)
+        ws = _lib.workspace(need, dev)
+        _lib.check(_lib.lib.fkc_kv4_fork(
+            cache._ref, tables.data_ptr(), stride, width, seq_lens.data_ptr(), R,
+            parents.data_ptr(), F, free_blocks.data_ptr(), free_blocks.shape[0], new.data_ptr(),
+            seq.data_ptr(), taken.data_ptr(), ws.data_ptr(), need, _lib.stream_of(seq_lens)),
+            "fork")
+    return new, seq, taken
+
+
+def compact(cache: Cache, tables: torch.Tensor, seq_lens: torch.Tensor, into: Cache
+            ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The held blocks moved into another cache; -> (tables, used).
+
+    A cache's size is fixed: a smaller or larger one is another cache.  The i-th
+    block that some row holds, in ascending order, becomes block i of `into`
+    (its heads, block_size, head_dim, dtype, and, which is not checked, its
+    levels are the cache's), shared ones once; the new tables (R, max_blocks)
+    name them, -1 behind a row's tokens.  used (1) int32 counts the held
+    blocks; those that `into` is too small for are not moved, and their entries
+    are -1.  `cache` and the old tables stay as they are.
+    """
+    dev = cache.device
+    _on_gpu("into", into.k_codes, dev)
+    seq_lens = _i32("seq_lens", seq_lens, 1, dev)
+    R = seq_lens.shape[0]
+    width, stride = _check_tables(tables, R, dev)
+    new, used = torch.split_with_sizes(seq_lens.new_empty(R * width + 1), (R * width, 1))
+    with _lib.on_device(seq_lens):
+        need = _lib.lib.fkc_kv4_compact_workspace_bytes(cache._ref)
+        ws = _lib.workspace(need, dev)
+        _lib.check(_lib.lib.fkc_kv4_compact(
+            cache._ref, tables.data_ptr(), stride, width, seq_lens.data_ptr(), R, into._ref,
+            new.data_ptr(), used.data_ptr(), ws.data_ptr(), need, _lib.stream_of(seq_lens)),
+            "compact")
+    return new.view(R, width), used
+
+
+def copy_blocks(cache: Cache, src: torch.Tensor, into: Cache, dst: torch.Tensor) -> None:
+    """Copy block src[i] of `cache` to block dst[i] of `into` (N,) int32, codes
+    and scales: a request handed to another cache, or to other blocks of the
+    same one.  Blocks outside their cache (-1) are skipped.  The caches are
+    alike as for `compact`.  dst names no block twice, and within one cache
+    none that src names: what such blocks hold afterwards is not defined.
+    """
+    dev = cache.device
+    _on_gpu("into", into.k_codes, dev)
+    src, dst = _i32("src", src, 1, dev), _i32("dst", dst, 1, dev)
+    _require(src.shape == dst.shape, "src and dst must be of one length")
+    with _lib.on_device(src):
+        _lib.check(_lib.lib.fkc_kv4_copy_blocks(
+            cache._ref, src.data_ptr(), into._ref, dst.data_ptr(), src.shape[0],
+            _lib.stream_of(src)), "copy_blocks")

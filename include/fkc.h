@@ -455,6 +455,73 @@ FKC_CAPI int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
                             void* workspace, size_t workspace_bytes,
                             fkc_stream_t stream);
 
+/*
+ * Pages of the cache.  Row r of tables (R rows, table_stride apart, max_blocks
+ * entries each) holds its first ceil(seq_lens[r] / block_size) entries, those
+ * there are (negative lengths count as 0); entries outside the cache name no
+ * block.  Any number of rows may hold the same block.
+ *
+ * fkc_free_blocks: the blocks 0 .. num_blocks - 1 that no row holds, ascending,
+ * in free_blocks (num_blocks entries), -1 behind them; count (1): how many.
+ * The list may be handed to fkc_block_tables as it is: its -1 are blocks that
+ * it does not have.
+ */
+FKC_CAPI size_t fkc_free_blocks_workspace_bytes(int64_t num_blocks);
+FKC_CAPI int fkc_free_blocks(const int32_t* tables, int64_t table_stride,
+                             int64_t max_blocks, const int32_t* seq_lens,
+                             int64_t R, int64_t block_size, int64_t num_blocks,
+                             int32_t* free_blocks, int32_t* count,
+                             void* workspace, size_t workspace_bytes,
+                             fkc_stream_t stream);
+
+/*
+ * Rows that go on from others' tokens: row j of new_tables (F, max_blocks)
+ * dense and new_seq (F) is row parents[j] of tables (a parent outside 0 .. R - 1:
+ * a row without tokens), -1 behind its held entries and where one names no
+ * block.  Whole blocks are shared.  The last block of a row whose length is no
+ * multiple of block_size is the row's to go on in: the child keeps it if no
+ * child before it ends in the same block and none has it as a whole one;
+ * otherwise its entry becomes the next of free_blocks, which gets a copy of the
+ * block, codes and scales.  taken (1): such copies; where free_blocks does not
+ * reach, or names no block, the child's entry is -1.  tables and seq_lens are
+ * not written.  What rows that are no child's parent hold is not looked at.
+ */
+FKC_CAPI size_t fkc_kv4_fork_workspace_bytes(const fkc_kv4_cache* cache, int64_t F);
+FKC_CAPI int fkc_kv4_fork(const fkc_kv4_cache* cache, const int32_t* tables,
+                          int64_t table_stride, int64_t max_blocks,
+                          const int32_t* seq_lens, int64_t R,
+                          const int32_t* parents, int64_t F,
+                          const int32_t* free_blocks, int64_t num_free,
+                          int32_t* new_tables, int32_t* new_seq, int32_t* taken,
+                          void* workspace, size_t workspace_bytes,
+                          fkc_stream_t stream);
+
+/*
+ * The held blocks moved into another cache of the same heads, block_size, D and
+ * dtype: the i-th held block in ascending order becomes block i of `into`, and
+ * new_tables (R, max_blocks) dense names them by their new numbers, -1 behind
+ * a row's held entries, where one names no block, and for those that `into` is
+ * too small for.  used (1): held blocks in all.  Levels are not copied: both
+ * caches are made with the same.  The caches share no memory.
+ */
+FKC_CAPI size_t fkc_kv4_compact_workspace_bytes(const fkc_kv4_cache* cache);
+FKC_CAPI int fkc_kv4_compact(const fkc_kv4_cache* cache, const int32_t* tables,
+                             int64_t table_stride, int64_t max_blocks,
+                             const int32_t* seq_lens, int64_t R,
+                             const fkc_kv4_cache* into, int32_t* new_tables,
+                             int32_t* used, void* workspace,
+                             size_t workspace_bytes, fkc_stream_t stream);
+
+/*
+ * Block src[i] of cache to block dst[i] of into, i below n; entries outside
+ * their cache are skipped.  Both may be one cache.  Of two copies to one block
+ * any mixture stays, and of a block that is read and written in one call the
+ * copy may be of either.
+ */
+FKC_CAPI int fkc_kv4_copy_blocks(const fkc_kv4_cache* cache, const int32_t* src,
+                                 const fkc_kv4_cache* into, const int32_t* dst,
+                                 int64_t n, fkc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
