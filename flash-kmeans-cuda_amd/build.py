@@ -57,6 +57,7 @@ KERNEL_SOURCES = [
     "block_tables.hip",
     "kv4_store.hip",
     "kv4_attend.hip",
+    "kv4_attend_scored.hip",
     "kv4_pages.hip",
 ]
 HOST_SOURCES = ["capi.cpp", "capi_kv4.cpp"]

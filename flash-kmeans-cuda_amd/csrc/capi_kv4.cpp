@@ -68,6 +68,43 @@ int attend_sizes_ok(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R,
   return FKC_OK;
 }
 
+int attend_ok(const fkc_kv4_cache& c, const Kv4Attend& a, int64_t max_blocks) {
+  if (int rc = attend_sizes_ok(c, a.H, a.T, a.R, a.max_seq, "kv4_attend")) return rc;
+  if (!a.cu_q && a.T != a.R)
+    return fail(FKC_ERR_INVALID, "kv4_attend: one query per request needs T == R");
+  if (max_blocks < 0 || a.table_stride < max_blocks)
+    return fail(FKC_ERR_INVALID, "kv4_attend: rows of tables overlap");
+  if (a.max_seq > 0 && (a.max_seq - 1) / c.block_size >= max_blocks)
+    return fail(FKC_ERR_INVALID,
+                "kv4_attend: max_seq %lld is longer than %lld blocks of %lld",
+                (long long)a.max_seq, (long long)max_blocks, (long long)c.block_size);
+  if (a.T == 0) return FKC_OK;
+  if (int rc = rows_ok(a.q.p, a.q.token_stride, a.q.head_stride, "q", "kv4_attend"))
+    return rc;
+  if (!a.out || (a.R && !a.seq) || (a.R && a.max_seq && !a.tables))
+    return fail(FKC_ERR_INVALID, "kv4_attend: null pointer argument");
+  if (!aligned16(a.out))
+    return fail(FKC_ERR_INVALID, "kv4_attend: out not 16-byte aligned");
+  return FKC_OK;
+}
+
+int scores_ok(const fkc_kv4_scores* x, const char* what) {
+  if (!x) return fail(FKC_ERR_INVALID, "%s: null scores", what);
+  if (!(x->softcap >= 0.f && x->softcap <= std::numeric_limits<float>::max()))
+    return fail(FKC_ERR_INVALID, "%s: softcap is not a positive finite number", what);
+  if (x->window < 0 || x->window > kI32)
+    return fail(FKC_ERR_INVALID, "%s: window out of range", what);
+  return FKC_OK;
+}
+
+bool plain(const fkc_kv4_scores& x) {
+  return x.softcap == 0.f && !x.slopes && x.window == 0 && !x.starts && !x.prefix_lens;
+}
+
+Kv4Scores inner(const fkc_kv4_scores& x) {
+  return {x.softcap, x.slopes, x.window, x.starts, x.prefix_lens};
+}
+
 int tables_ok(const int32_t* tables, int64_t stride, int64_t max_blocks,
               const int32_t* seq, int64_t R, const char* what) {
   if (R < 0 || R > kI32 || max_blocks < 0 || max_blocks > kI32)
@@ -191,35 +228,57 @@ int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
                    size_t workspace_bytes, fkc_stream_t stream) {
   clear_error();
   if (int rc = cache_ok(cache, "kv4_attend")) return rc;
-  if (int rc = attend_sizes_ok(*cache, H, T, R, max_seq, "kv4_attend")) return rc;
-  if (!cu_q && T != R)
-    return fail(FKC_ERR_INVALID, "kv4_attend: one query per request needs T == R");
-  if (max_blocks < 0 || table_stride < max_blocks)
-    return fail(FKC_ERR_INVALID, "kv4_attend: rows of tables overlap");
-  if (max_seq > 0 && (max_seq - 1) / cache->block_size >= max_blocks)
-    return fail(FKC_ERR_INVALID,
-                "kv4_attend: max_seq %lld is longer than %lld blocks of %lld",
-                (long long)max_seq, (long long)max_blocks,
-                (long long)cache->block_size);
-  if (T == 0) return FKC_OK;
-  if (int rc = rows_ok(q, q_token_stride, q_head_stride, "q", "kv4_attend"))
-    return rc;
-  if (!out || (R && !seq_lens) || (R && max_seq && !tables))
-    return fail(FKC_ERR_INVALID, "kv4_attend: null pointer argument");
-  if (!aligned16(out))
-    return fail(FKC_ERR_INVALID, "kv4_attend: out not 16-byte aligned");
-  const size_t need = kv4_attend_workspace_bytes(*cache, H, T, R, max_seq);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(FKC_ERR_WORKSPACE, "kv4_attend: workspace %zu < %zu bytes",
-                workspace_bytes, need);
-  if (need && reinterpret_cast<uintptr_t>(workspace) % kWorkspaceAlign)
-    return fail(FKC_ERR_WORKSPACE, "kv4_attend: workspace not %d-byte aligned",
-                kWorkspaceAlign);
   const Kv4Attend a{{q, q_token_stride, q_head_stride},
                     H, T, tables, table_stride, seq_lens, cu_q, R, max_seq,
                     causal != 0, sm_scale, out, lse};
+  if (int rc = attend_ok(*cache, a, max_blocks)) return rc;
+  if (T == 0) return FKC_OK;
+  if (int rc = workspace_ok(workspace, workspace_bytes,
+                            kv4_attend_workspace_bytes(*cache, H, T, R, max_seq),
+                            "kv4_attend"))
+    return rc;
   return launch_kv4_attend(*cache, a, workspace, workspace_bytes,
                            reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t fkc_kv4_attend_scored_workspace_bytes(const fkc_kv4_cache* cache, int64_t H,
+                                             int64_t T, int64_t R, int64_t max_seq,
+                                             int causal, const fkc_kv4_scores* scores) {
+  clear_error();
+  if (cache_ok(cache, "kv4_attend_scored_workspace_bytes") ||
+      attend_sizes_ok(*cache, H, T, R, max_seq, "kv4_attend_scored_workspace_bytes") ||
+      scores_ok(scores, "kv4_attend_scored_workspace_bytes"))
+    return 0;
+  if (plain(*scores)) return kv4_attend_workspace_bytes(*cache, H, T, R, max_seq);
+  return kv4_attend_scored_workspace_bytes(*cache, H, T, R, max_seq, causal != 0,
+                                           inner(*scores));
+}
+
+int fkc_kv4_attend_scored(const fkc_kv4_cache* cache, const void* q,
+                          int64_t q_token_stride, int64_t q_head_stride, int64_t H,
+                          int64_t T, const int32_t* tables, int64_t table_stride,
+                          int64_t max_blocks, const int32_t* seq_lens,
+                          const int32_t* cu_q, int64_t R, int64_t max_seq, int causal,
+                          float sm_scale, const fkc_kv4_scores* scores, void* out,
+                          float* lse, void* workspace, size_t workspace_bytes,
+                          fkc_stream_t stream) {
+  clear_error();
+  if (int rc = cache_ok(cache, "kv4_attend")) return rc;
+  if (int rc = scores_ok(scores, "kv4_attend")) return rc;
+  const Kv4Attend a{{q, q_token_stride, q_head_stride},
+                    H, T, tables, table_stride, seq_lens, cu_q, R, max_seq,
+                    causal != 0, sm_scale, out, lse};
+  if (int rc = attend_ok(*cache, a, max_blocks)) return rc;
+  if (T == 0) return FKC_OK;
+  const Kv4Scores x = inner(*scores);
+  const bool without = plain(*scores);
+  const size_t need =
+      without ? kv4_attend_workspace_bytes(*cache, H, T, R, max_seq)
+              : kv4_attend_scored_workspace_bytes(*cache, H, T, R, max_seq, causal != 0, x);
+  if (int rc = workspace_ok(workspace, workspace_bytes, need, "kv4_attend")) return rc;
+  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return without ? launch_kv4_attend(*cache, a, workspace, workspace_bytes, s)
+                 : launch_kv4_attend_scored(*cache, a, x, workspace, s);
 }
 
 size_t fkc_free_blocks_workspace_bytes(int64_t num_blocks) {

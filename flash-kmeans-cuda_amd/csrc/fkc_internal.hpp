@@ -269,6 +269,20 @@ size_t kv4_attend_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int64_t T,
                                   int64_t R, int64_t max_seq);
 int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& a, void* ws,
                       size_t ws_bytes, hipStream_t s);
+// The same with capped, biased or masked scores; window 0 and null pointers:
+// without.
+struct Kv4Scores {
+  float softcap;  // 0: none
+  const float* slopes;
+  int64_t window;
+  const int32_t* starts;
+  const int32_t* prefix;
+};
+size_t kv4_attend_scored_workspace_bytes(const fkc_kv4_cache& c, int64_t H,
+                                         int64_t T, int64_t R, int64_t max_seq,
+                                         bool causal, const Kv4Scores& x);
+int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& a,
+                             const Kv4Scores& x, void* ws, hipStream_t s);
 // Pages: tables of R rows over block numbers, with the rows' lengths.
 struct Kv4Tables {
   const int32_t* tables;

@@ -62,6 +62,8 @@ SIGNATURES = {
     "fkc_kv4_read": (_int, [_vp, _vp, _i64, _vp, _vp, _vp]),
     "fkc_kv4_attend_workspace_bytes": (_sz, [_vp, _i64, _i64, _i64, _i64]),
     "fkc_kv4_attend": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "fkc_kv4_attend_scored_workspace_bytes": (_sz, [_vp, _i64, _i64, _i64, _i64, _int, _vp]),
+    "fkc_kv4_attend_scored": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _int, ctypes.c_float, _vp, _vp, _vp, _vp, _sz, _vp]),
     "fkc_free_blocks_workspace_bytes": (_sz, [_i64]),
     "fkc_free_blocks": (_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _sz, _vp]),
     "fkc_kv4_fork_workspace_bytes": (_sz, [_vp, _i64]),

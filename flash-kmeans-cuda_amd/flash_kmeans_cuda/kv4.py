@@ -256,23 +256,57 @@ def read(cache: Cache, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]
 
 
 class _NoGradient(torch.autograd.Function):
-    """Puts attend's results into the graph of its queries, so that a gradient
-    that would have to pass through them raises instead of being left out."""
+    """Puts attend's results into the graph of its queries (and slopes), so that
+    a gradient that would have to pass through them raises instead of being left
+    out."""
 
     @staticmethod
-    def forward(ctx, q, *results):
+    def forward(ctx, q, slopes, *results):
         ctx.mark_dirty(*results)
         return results
 
     @staticmethod
     def backward(ctx, *grads):
-        raise RuntimeError("kv4.attend has no gradient: detach q, or call it under no_grad")
+        raise RuntimeError("kv4.attend has no gradient: detach q and slopes, or call it under "
+                           "no_grad")
+
+
+class _CScores(ctypes.Structure):
+    """fkc_kv4_scores of include/fkc.h."""
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p),
+                ("window", ctypes.c_int64), ("starts", ctypes.c_void_p),
+                ("prefix_lens", ctypes.c_void_p)]
+
+
+def _scores(softcap, slopes, window, starts, prefix_lens, T, H, R, dev):
+    """(the C struct of attend's options, the tensors it points into)."""
+    if softcap is not None:
+        _require(0.0 < softcap < 3e38, f"softcap must be positive and finite, not {softcap}")
+    if window is not None:
+        _require(0 < window < 1 << 31, f"window must be at least 1, below 2^31, not {window}")
+    if slopes is not None:
+        _on_gpu("slopes", slopes, dev)
+        _require(slopes.dtype is torch.float32 and tuple(slopes.shape) == (H,),
+                 f"slopes must be ({H},) float32")
+        slopes = slopes.contiguous()
+    if starts is not None:
+        starts = _i32("starts", starts, 1, dev)
+        _require(starts.shape[0] == T, "starts must have one entry per row of q")
+    if prefix_lens is not None:
+        prefix_lens = _i32("prefix_lens", prefix_lens, 1, dev)
+        _require(prefix_lens.shape[0] == R, "prefix_lens must be as long as seq_lens")
+    c = _CScores(softcap or 0.0, _lib.ptr(slopes), window or 0, _lib.ptr(starts),
+                 _lib.ptr(prefix_lens))
+    return c, (slopes, starts, prefix_lens)
 
 
 def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.Tensor,
            cu_q: Optional[torch.Tensor] = None, *, causal: bool = True,
            sm_scale: Optional[float] = None, max_seq: Optional[int] = None,
-           out: Optional[torch.Tensor] = None, return_lse: bool = False
+           out: Optional[torch.Tensor] = None, return_lse: bool = False,
+           softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+           window: Optional[int] = None, starts: Optional[torch.Tensor] = None,
+           prefix_lens: Optional[torch.Tensor] = None
            ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Attention of q (T, H, D) over the cached tokens of R requests.
 
@@ -291,6 +325,16 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
     given, and with return_lse also log sum exp of each row's scores, fp32
     (T, H), -inf for rows that see nothing.  There is no gradient: going back
     through the result of a q that requires one raises RuntimeError.
+
+    Scores and masks of other models, any of them together, for a query at
+    position p of its request and a token at t:
+      softcap      a score z becomes softcap * tanh(z / softcap);
+      slopes       (H,) float32: slopes[h] * |p - t| is taken off it, after the cap;
+      window       no token more than window - 1 positions back is seen: t > p - window;
+      starts       (T,) int32, no token before starts[row] is seen: the first token of
+                   the query's document where several lie in one request;
+      prefix_lens  (R,) int32, with `causal` the first prefix_lens[r] tokens are seen by
+                   every query of the request (as far as window and starts let it).
     """
     q = _rows("q", q, 0, cache)
     dev = cache.device
@@ -317,6 +361,20 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
     if sm_scale is None:
         sm_scale = D ** -0.5
+    if not (softcap is None and slopes is None and window is None and starts is None
+            and prefix_lens is None):
+        scores, held = _scores(softcap, slopes, window, starts, prefix_lens, T, H, R, dev)
+        ref = ctypes.addressof(scores)
+        with _lib.on_device(q):
+            need = _lib.lib.fkc_kv4_attend_scored_workspace_bytes(cache._ref, H, T, R, max_seq,
+                                                                  int(causal), ref)
+            ws = _lib.workspace(need, dev) if need else None
+            _lib.check(_lib.lib.fkc_kv4_attend_scored(
+                cache._ref, q.data_ptr(), q.stride(0), q.stride(1), H, T, tables.data_ptr(),
+                stride, width, seq_lens.data_ptr(), _lib.ptr(cu_q), R, max_seq, int(causal),
+                sm_scale, ref, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need,
+                _lib.stream_of(q)), "attend")
+        return _outside_gradients(q, slopes, out, lse)
     with _lib.on_device(q):
         need = _lib.lib.fkc_kv4_attend_workspace_bytes(cache._ref, H, T, R, max_seq)
         ws = _lib.workspace(need, dev) if need else None
@@ -324,12 +382,18 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
             cache._ref, q.data_ptr(), q.stride(0), q.stride(1), H, T, tables.data_ptr(), stride,
             width, seq_lens.data_ptr(), _lib.ptr(cu_q), R, max_seq, int(causal), sm_scale,
             out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), need, _lib.stream_of(q)), "attend")
-    if q.requires_grad and torch.is_grad_enabled():
+    return _outside_gradients(q, None, out, lse)
+
+
+def _outside_gradients(q, slopes, out, lse):
+    """attend's results, in the graph of what requires a gradient."""
+    if (q.requires_grad or (slopes is not None and slopes.requires_grad)) \
+            and torch.is_grad_enabled():
         if lse is not None:
-            out, lse = _NoGradient.apply(q, out, lse)
+            out, lse = _NoGradient.apply(q, slopes, out, lse)
         else:
-            out, = _NoGradient.apply(q, out)
-    return (out, lse) if return_lse else out
+            out, = _NoGradient.apply(q, slopes, out)
+    return out if lse is None else (out, lse)
 
 
 def free_blocks(tables: torch.Tensor, seq_lens: torch.Tensor, block_size: int, num_blocks: int

@@ -456,6 +456,39 @@ FKC_CAPI int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
                             fkc_stream_t stream);
 
 /*
+ * The same attention with other scores and masks.  With p = seq_lens[r] - n + i
+ * the position of query i of n of request r, in row t of q,
+ *   z_t = softcap * tanh(sm_scale <q, k_t> / softcap)   (softcap 0: without)
+ *         - slopes[h] * |p - t|                         (slopes NULL: without)
+ * over the tokens first <= t < last,
+ *   last  = seq_lens[r], or if causal at most max(p + 1, prefix_lens[r]),
+ *   first = max(0, starts[row], p - window + 1)  (window 0, starts NULL: without).
+ * softcap > 0 and finite or 0; slopes (H) fp32, finite; window >= 0, below 2^31;
+ * starts (T) and prefix_lens (R) int32 of any values.  A row whose first is not
+ * below its last sees nothing.  Scores are fp32; the distance is exact below
+ * 2^24 and rounded beyond.  softcap at least 4 |sm_scale| keeps every finite
+ * score finite; with less, a key scale past 2^120 may overflow.
+ */
+typedef struct fkc_kv4_scores {
+  float softcap;
+  const float* slopes;
+  int64_t window;
+  const int32_t* starts;
+  const int32_t* prefix_lens;
+} fkc_kv4_scores;
+
+FKC_CAPI size_t fkc_kv4_attend_scored_workspace_bytes(
+    const fkc_kv4_cache* cache, int64_t H, int64_t T, int64_t R, int64_t max_seq,
+    int causal, const fkc_kv4_scores* scores);
+FKC_CAPI int fkc_kv4_attend_scored(
+    const fkc_kv4_cache* cache, const void* q, int64_t q_token_stride,
+    int64_t q_head_stride, int64_t H, int64_t T, const int32_t* tables,
+    int64_t table_stride, int64_t max_blocks, const int32_t* seq_lens,
+    const int32_t* cu_q, int64_t R, int64_t max_seq, int causal, float sm_scale,
+    const fkc_kv4_scores* scores, void* out, float* lse, void* workspace,
+    size_t workspace_bytes, fkc_stream_t stream);
+
+/*
  * Pages of the cache.  Row r of tables (R rows, table_stride apart, max_blocks
  * entries each) holds its first ceil(seq_lens[r] / block_size) entries, those
  * there are (negative lengths count as 0); entries outside the cache name no

@@ -1,0 +1,99 @@
+"""Attention with capped, biased or masked scores: its C entry points refuse
+what their kernels could not index, before anything reaches a device; and the
+reference's masks are checked one by one."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+import kv4_scored_ref as sref
+from test_kv4_cpu import FAKE, _cache
+
+
+def _scores(softcap=0.0, slopes=None, window=0, starts=None, prefix=None):
+    from flash_kmeans_cuda.kv4 import _CScores
+    return _CScores(softcap, slopes, window, starts, prefix)
+
+
+def _attend(scores, q=FAKE, ts=256, hs=64, H=4, T=3, tables=FAKE, stride=8, width=8, seq=FAKE,
+            cu=None, R=3, max_seq=128, out=FAKE, ws=None, nbytes=0, cache=None):
+    from flash_kmeans_cuda import _lib
+    c = cache or _cache()
+    rc = _lib.lib.fkc_kv4_attend_scored(
+        ctypes.addressof(c), q, ts, hs, H, T, tables, stride, width, seq, cu, R, max_seq, 1, 0.1,
+        ctypes.addressof(scores) if scores is not None else None, out, None, ws, nbytes, None)
+    return rc, _lib.last_error()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(softcap=-1.0), "softcap"), (dict(softcap=math.inf), "softcap"),
+    (dict(softcap=math.nan), "softcap"), (dict(window=-1), "window"),
+    (dict(window=1 << 31), "window")])
+def test_options_are_checked(kw, word):
+    from flash_kmeans_cuda import _lib
+    x, c = _scores(**kw), _cache()
+    rc, msg = _attend(x)
+    assert rc == 1 and word in msg
+    assert _lib.lib.fkc_kv4_attend_scored_workspace_bytes(
+        ctypes.addressof(c), 4, 3, 3, 128, 1, ctypes.addressof(x)) == 0
+    assert word in _lib.last_error()
+
+
+def test_null_options():
+    rc, msg = _attend(None)
+    assert rc == 1 and "null scores" in msg
+
+
+@pytest.mark.parametrize("scores", [dict(), dict(softcap=30.0), dict(window=5), dict(slopes=FAKE),
+                                    dict(starts=FAKE), dict(prefix=FAKE)])
+@pytest.mark.parametrize("kw,word", [
+    (dict(H=3), "multiple"), (dict(T=-1), "range"), (dict(max_seq=129), "longer"),
+    (dict(T=4), "T == R"), (dict(stride=7), "overlap"), (dict(q=None), "null"),
+    (dict(q=FAKE + 2), "aligned"), (dict(hs=63), "aligned"), (dict(out=None), "null"),
+    (dict(seq=None), "null"), (dict(tables=None), "null"), (dict(out=FAKE + 8), "aligned")])
+def test_refusals(scores, kw, word):
+    rc, msg = _attend(_scores(**scores), **kw)
+    assert rc == 1 and word in msg
+
+
+@pytest.mark.parametrize("scores", [dict(), dict(softcap=30.0), dict(slopes=FAKE, window=90000)])
+def test_workspace(scores):
+    from flash_kmeans_cuda import _lib
+    c, x = _cache(num_blocks=1 << 16), _scores(**scores)
+    need = _lib.lib.fkc_kv4_attend_scored_workspace_bytes(
+        ctypes.addressof(c), 4, 1, 1, 100000, 1, ctypes.addressof(x))
+    assert need > 0
+    kw = dict(T=1, R=1, max_seq=100000, width=6250, stride=6250, cache=c)
+    assert _attend(x, **kw)[0] == 2
+    rc, msg = _attend(x, ws=FAKE, nbytes=need - 1, **kw)
+    assert rc == 2 and "workspace" in msg
+    rc, msg = _attend(x, ws=FAKE + 16, nbytes=need, **kw)
+    assert rc == 2 and "aligned" in msg
+
+
+def test_reference_masks():
+    """Written out by hand: four queries at positions 2 .. 5 of six tokens."""
+    def rows(**kw):
+        return ["".join("x" if v else "." for v in r) for r in sref.seen(6, 4, **kw).tolist()]
+    assert rows() == ["xxx...", "xxxx..", "xxxxx.", "xxxxxx"]
+    assert rows(window=2) == [".xx...", "..xx..", "...xx.", "....xx"]
+    assert rows(window=2, causal=False) == [".xxxxx", "..xxxx", "...xxx", "....xx"]
+    assert rows(prefix=4) == ["xxxx..", "xxxx..", "xxxxx.", "xxxxxx"]
+    assert rows(prefix=4, window=3) == ["xxxx..", ".xxx..", "..xxx.", "...xxx"]
+    assert rows(starts=torch.tensor([0, 3, 3, 9])) == ["xxx...", "...x..", "...xx.", "......"]
+    assert sref.seen(1, 3).tolist() == [[False], [False], [True]]
+    assert sref.seen(1, 3, prefix=7).tolist() == [[True], [True], [True]]
+
+
+def test_reference_is_plain_attention_with_nothing_set():
+    import kv4_ref as ref
+    cache = ref.random_cache(4, 1, 16, 64, torch.float16, 1)
+    tables = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32)
+    q = torch.randn(6, 2, 64, generator=torch.Generator().manual_seed(1)).half()
+    a = ref.attend(q, cache, tables, [20, 31], [2, 4])
+    b = sref.attend(q, cache, tables, [20, 31], [2, 4])
+    assert torch.allclose(a[0], b[0], atol=1e-12) and torch.allclose(a[1], b[1], atol=1e-12)
