@@ -111,6 +111,9 @@ int tables_ok(const int32_t* tables, int64_t stride, int64_t max_blocks,
     return fail(FKC_ERR_INVALID, "%s: size out of range", what);
   if (stride < max_blocks)
     return fail(FKC_ERR_INVALID, "%s: rows of tables overlap", what);
+  // The kernels number the entries in 32 bits.
+  if (max_blocks && R >= (int64_t)UINT32_MAX / max_blocks)
+    return fail(FKC_ERR_UNSUPPORTED, "%s: 2^32 table entries and more", what);
   if (R && (!seq || (max_blocks && !tables)))
     return fail(FKC_ERR_INVALID, "%s: null pointer argument", what);
   return FKC_OK;
@@ -331,6 +334,8 @@ int fkc_kv4_fork(const fkc_kv4_cache* cache, const int32_t* tables, int64_t tabl
     return rc;
   if (F < 0 || F > kI32 || num_free < 0)
     return fail(FKC_ERR_INVALID, "kv4_fork: size out of range");
+  if (max_blocks && F >= (int64_t)UINT32_MAX / max_blocks)
+    return fail(FKC_ERR_UNSUPPORTED, "kv4_fork: 2^32 table entries and more");
   if (!taken || (F && (!parents || !new_seq || (max_blocks && !new_tables))) ||
       (num_free && !free_blocks))
     return fail(FKC_ERR_INVALID, "kv4_fork: null pointer argument");

@@ -14,7 +14,7 @@ namespace fkc {
 namespace {
 
 constexpr int PT = 256;          // threads per workgroup
-constexpr int CHUNK = 4096;      // blocks that a workgroup of the list counts
+constexpr int CHUNK = 1024;      // blocks that a workgroup lists
 constexpr int ENTRIES = 1024;    // table entries of a row per workgroup and turn
 
 struct Rows {
@@ -24,173 +24,314 @@ struct Rows {
   int64_t R;
   int width;
   uint32_t bs;
-  // Entries of row r that are held, and of these the ones that are full.
+  FastDiv by_width;
+  // Entries of row r that are held.
   __device__ inline int held(int64_t r) const {
     const uint32_t s = (uint32_t)max(seq[r], 0);
     return (int)min((s + bs - 1) / bs, (uint32_t)width);
   }
 };
 
-// ------------------------------------------------- which blocks are held
-
-__global__ void __launch_bounds__(PT)
-clear_kernel(uint32_t* __restrict__ p, int64_t words) {
-  for (int64_t i = (int64_t)blockIdx.x * PT + threadIdx.x; i < words;
-       i += (int64_t)gridDim.x * PT)
-    p[i] = 0;
+// Inclusive scan over the workgroup's T threads; *total: the sum.
+template <int T>
+__device__ inline int wg_scan(int v, int* s, int* total) {
+  int incl = wave_incl_scan(v);
+  __syncthreads();  // s is read
+  if ((threadIdx.x & 63) == 63) s[threadIdx.x >> 6] = incl;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) {
+    incl += w < (int)(threadIdx.x >> 6) ? s[w] : 0;
+    all += s[w];
+  }
+  *total = all;
+  return incl;
 }
 
-// A byte per block.  (Bytes rather than bits: stores of the same value need no
-// atomics.)
+// ------------------------------------------------- which blocks are held
+
+// -1 behind the free blocks, as many as are held; by the whole grid.
+template <bool FREE, int T>
+__device__ inline void finish(int64_t num_blocks, int all, int32_t* list, int32_t* total) {
+  if (FREE)
+    for (int64_t i = (int64_t)blockIdx.x * T + threadIdx.x; i < all; i += (int64_t)gridDim.x * T)
+      list[num_blocks - all + i] = -1;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *total = FREE ? (int)(num_blocks - all) : all;
+}
+
+// Small tables, one launch: every workgroup marks all of them in a bitmap of
+// its own, counts, and lists its part.  Bound by latency (64 rows of up to
+// 128 entries over 4700 blocks 5.4 us, the three launches below 9).  More entries
+// or blocks than this cost more time here than the launches that it saves.
+constexpr int ST = 1024, kSmallBlocks = 1 << 16, kSmallEntries = 1 << 15;
+template <bool FREE>
+__global__ void __launch_bounds__(ST)
+names_small_kernel(const Rows t, uint32_t num_blocks, int32_t* __restrict__ list,
+                   int32_t* __restrict__ number, int32_t* __restrict__ total) {
+  constexpr int PER = 2;  // words of 32 blocks per thread
+  static_assert(ST * PER * 32 == kSmallBlocks, "a bit for every block");
+  __shared__ uint32_t bits[ST * PER];
+  __shared__ int before[ST * PER];
+  __shared__ int s[ST / 64];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bits[threadIdx.x + i * ST] = 0;
+  __syncthreads();
+  const int n = (int)t.R * t.width;
+  for (int e0 = threadIdx.x; e0 < n; e0 += ST * 4) {
+    uint32_t b[4];
+    bool in[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = min(e0 + i * ST, n - 1);
+      const int r = (int)t.by_width.div(e), c = e - r * t.width;
+      b[i] = (uint32_t)t.tables[r * t.stride + c];
+      in[i] = c < t.held(r);  // (the last entry may be marked again)
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (in[i] && b[i] < num_blocks) atomicOr(&bits[b[i] / 32], 1u << (b[i] & 31));
+  }
+  __syncthreads();
+  int mine = 0, all;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) mine += __popc(bits[threadIdx.x * PER + i]);
+  int at = wg_scan<ST>(mine, s, &all) - mine;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    before[threadIdx.x * PER + i] = at;
+    at += __popc(bits[threadIdx.x * PER + i]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < CHUNK; i += ST) {
+    const uint32_t b = blockIdx.x * CHUNK + i;
+    if (b >= num_blocks) break;
+    const uint32_t w = bits[b / 32];
+    const int held = before[b / 32] + __popc(w & ((1u << (b & 31)) - 1));
+    const bool is = w >> (b & 31) & 1;
+    if (FREE) {
+      if (!is) list[b - held] = (int32_t)b;
+    } else if (is) {
+      list[held] = (int32_t)b;
+      number[b] = held;
+    }
+  }
+  finish<FREE, ST>(num_blocks, all, list, total);
+}
+
+// Larger ones: each held entry writes its number where its block is, whichever
+// comes last.  Nothing is cleared before: what stands there counts only if it is
+// the number of a held entry that names this block.
 __global__ void __launch_bounds__(PT)
-mark_kernel(const Rows t, uint32_t num_blocks, uint8_t* __restrict__ named) {
+mark_kernel(const Rows t, uint32_t num_blocks, uint32_t* __restrict__ entry) {
   const int parts = (t.width + ENTRIES - 1) / ENTRIES;
   for (int64_t u = blockIdx.x; u < t.R * parts; u += gridDim.x) {
-    const int64_t r = u / parts;
+    const int64_t r = parts == 1 ? u : u / parts;
     const int lo = (int)(u - r * parts) * ENTRIES, hi = min(t.held(r), lo + ENTRIES);
     for (int e = lo + threadIdx.x; e < hi; e += PT) {
       const uint32_t b = (uint32_t)t.tables[r * t.stride + e];
-      if (b < num_blocks) named[b] = 1;
+      if (b < num_blocks) entry[b] = (uint32_t)(r * t.width + e);
     }
   }
 }
 
-__device__ inline int wg_sum(int v, int* s) {
-  v = wave_sum_i(v);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
+__device__ inline bool named(const Rows& t, uint32_t b, uint32_t e) {
+  if (e >= (uint64_t)t.R * t.width) return false;
+  const uint32_t r = e >> 31 ? e / t.width : t.by_width.div(e);
+  const int c = (int)(e - r * (uint32_t)t.width);
+  return (uint32_t)t.tables[r * t.stride + c] == b && c < t.held(r);
+}
+
+// A wave's blocks, 64 at a time; masks holds a bit for each.
+constexpr int GROUPS = CHUNK / PT;
+
+__device__ inline int64_t first_of(int i) {
+  return (int64_t)blockIdx.x * CHUNK + ((threadIdx.x >> 6) * GROUPS + i) * 64;
+}
+
+__global__ void __launch_bounds__(PT)
+count_kernel(const Rows t, int64_t num_blocks, const uint32_t* __restrict__ entry,
+             uint64_t* __restrict__ masks, int32_t* __restrict__ counts) {
+  __shared__ int s[PT / 64];
+  const int lane = threadIdx.x & 63;
+  uint32_t e[GROUPS];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    const int64_t b = first_of(i) + lane;
+    e[i] = b < num_blocks ? entry[b] : 0xffffffffu;
+  }
+  bool is[GROUPS];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) is[i] = named(t, (uint32_t)(first_of(i) + lane), e[i]);
   int sum = 0;
 #pragma unroll
-  for (int w = 0; w < PT / 64; ++w) sum += s[w];
-  __syncthreads();
-  return sum;
-}
-
-// The named bytes of 16 blocks as a bit mask; those past the last count as not
-// named.
-__device__ inline uint32_t mask16(const uint8_t* named, int64_t b, int64_t num_blocks) {
-  uint32_t m = 0;
-  if (b < num_blocks) {  // (the bytes are padded to whole chunks)
-    const uint4 w = *reinterpret_cast<const uint4*>(named + b);
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m |= (x[i] * 0x10204080u >> 28) << (4 * i);
+  for (int i = 0; i < GROUPS; ++i) {
+    const uint64_t m = __ballot(is[i]);
+    sum += __popcll(m);
+    if (lane == 0) masks[first_of(i) / 64] = m;
   }
-  return m;
+  if (lane == 0) s[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < PT / 64; ++w) sum += s[w];
+    counts[blockIdx.x] = sum;
+  }
 }
 
-__global__ void __launch_bounds__(PT)
-count_kernel(const uint8_t* __restrict__ named, int64_t num_blocks, int32_t* __restrict__ counts) {
-  __shared__ int s[PT / 64];
-  const int64_t b = (int64_t)blockIdx.x * CHUNK + threadIdx.x * 16;
-  const int sum = wg_sum(__popc(mask16(named, b, num_blocks)), s);
-  if (threadIdx.x == 0) counts[blockIdx.x] = sum;
-}
-
-// Lists the free blocks, or the held ones and each one's place among them.
 template <bool FREE>
 __global__ void __launch_bounds__(PT)
-list_kernel(const uint8_t* __restrict__ named, int64_t num_blocks,
+list_kernel(int64_t num_blocks, const uint64_t* __restrict__ masks,
             const int32_t* __restrict__ counts, int32_t* __restrict__ list,
             int32_t* __restrict__ number, int32_t* __restrict__ total) {
   __shared__ int s[PT / 64];
-  const int t = threadIdx.x;
+  uint64_t m[GROUPS];
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    m[i] = masks[first_of(i) / 64];
+    mine += __popcll(m[i]);
+  }
   int below = 0, all = 0;
-  for (int i = t; i < (int)gridDim.x; i += PT) {
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += PT) {
     const int c = counts[i];
     all += c;
     below += i < (int)blockIdx.x ? c : 0;
   }
-  below = wg_sum(below, s);
-  all = wg_sum(all, s);
-  const int64_t b0 = (int64_t)blockIdx.x * CHUNK + t * 16;
-  const uint32_t m = mask16(named, b0, num_blocks);
-  const int mine = __popc(m);
-  int incl = wave_incl_scan(mine);
-  if ((t & 63) == 63) s[t >> 6] = incl;
-  __syncthreads();
-  for (int w = 0; w < t >> 6; ++w) incl += s[w];
-  int at = below + incl - mine;  // held blocks before mine
+  const int lane = threadIdx.x & 63;
+  int at, sum;
+  wg_scan<PT>(below, s, &below);
+  wg_scan<PT>(all, s, &all);
+  at = below + wg_scan<PT>(lane == 63 ? mine : 0, s, &sum) - (lane == 63 ? mine : 0);
+  at = __shfl(at, 63, 64);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t b = b0 + i;
-    if (b >= num_blocks) break;
-    const bool held = m >> i & 1;
+  for (int i = 0; i < GROUPS; ++i) {
+    const int64_t b = first_of(i) + lane;
+    const int held = at + (int)lanes_below(m[i]);
+    const bool is = m[i] >> lane & 1;
     if (FREE) {
-      if (!held) list[b - at] = (int32_t)b;
-    } else if (held) {
-      list[at] = (int32_t)b;
-      number[b] = at;
+      if (!is && b < num_blocks) list[b - held] = (int32_t)b;
+    } else if (is) {
+      list[held] = (int32_t)b;
+      number[b] = held;
     }
-    at += held;
+    at += __popcll(m[i]);
   }
-  if (FREE) {
-    // behind the free ones, as many as are held
-    for (int64_t i = (int64_t)blockIdx.x * PT + t; i < all; i += (int64_t)gridDim.x * PT)
-      list[num_blocks - all + i] = -1;
-  }
-  if (blockIdx.x == 0 && t == 0) *total = FREE ? (int)(num_blocks - all) : all;
+  finish<FREE, PT>(num_blocks, all, list, total);
 }
 
 // ------------------------------------------------- moving blocks
 
 // A block's codes and scales are four runs of 16-byte units.
+typedef uint32_t Unit __attribute__((ext_vector_type(4)));
 struct Store {
-  uint4* p[4];
+  Unit* p[4];
   __host__ __device__ explicit Store(const fkc_kv4_cache& c)
-      : p{(uint4*)c.k_codes, (uint4*)c.v_codes, (uint4*)c.k_scales, (uint4*)c.v_scales} {}
+      : p{(Unit*)c.k_codes, (Unit*)c.v_codes, (Unit*)c.k_scales, (Unit*)c.v_scales} {}
 };
 
-constexpr int PIECE = 4 * PT;  // units a workgroup copies at a time
+constexpr int LOADS = 2;             // units per thread at a time
+constexpr int PIECE = LOADS * PT;    // units a workgroup copies at a time
 
-// Piece `piece` of block sb to block db.  codes, scales: units of one run.
-__device__ inline void copy_piece(const Store& from, int64_t sb, const Store& to, int64_t db,
-                                  int64_t piece, int codes, int scales) {
-  const int all = 2 * (codes + scales);
-  uint4 v[4];
+// Blocks as pieces, dealt out to workgroups in turn.
+struct Pieces {
+  int codes, scales;  // units of one run
+  int per;            // pieces of a block
+  FastDiv by_per;
+  Pieces(const fkc_kv4_cache& c)
+      : codes((int)(c.heads * c.block_size * c.D / 32)),
+        scales((int)(c.heads * c.block_size / 8)),
+        per((2 * (codes + scales) + PIECE - 1) / PIECE),
+        by_per((uint32_t)per) {}
+};
+
+// Piece `piece` of block sb to block db.  Bound by memory: 465 MB moved by
+// compact_kernel take about 168 us, 5.5 TB/s counting both ways, where a large
+// library copy reaches 4.6.  The copies are not read here again: stored past the
+// caches they leave these to the loads (us a call without / with that, and with
+// loads past the caches too: 465 MB 204 / 182 / 176, 31.7 MB 23.2 / 11.7 / 15.0).
+// Units per thread at a time 2 / 4 / 8: 465 MB 177 / 182 / 221.
+__device__ inline void copy_piece(const Store& from, uint32_t sb, const Store& to, uint32_t db,
+                                  int piece, const Pieces& p) {
+  const int all = 2 * (p.codes + p.scales);
+  Unit v[LOADS];
+  auto place = [&](int i, int* run, int* units) {
+    const int u = piece * PIECE + i * PT + (int)threadIdx.x;
+    int in = u;
+    *run = 0;
+    *units = p.codes;
+    if (in >= p.codes) in -= p.codes, *run = 1;
+    if (u >= 2 * p.codes) {
+      in -= p.codes;
+      *run = 2;
+      *units = p.scales;
+      if (in >= p.scales) in -= p.scales, *run = 3;
+    }
+    return u < all ? in : -1;
+  };
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t u = piece * PIECE + i * PT + threadIdx.x;
-    if (u >= all) continue;
-    const int run = u < 2 * (int64_t)codes ? u >= codes : 2 + (u >= 2 * (int64_t)codes + scales);
-    const int64_t in = run < 2 ? u - run * (int64_t)codes
-                               : u - 2 * (int64_t)codes - (run - 2) * (int64_t)scales;
-    v[i] = from.p[run][sb * (run < 2 ? codes : scales) + in];
+  for (int i = 0; i < LOADS; ++i) {
+    int run, units;
+    const int in = place(i, &run, &units);
+    if (in >= 0) v[i] = from.p[run][(int64_t)sb * units + in];
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t u = piece * PIECE + i * PT + threadIdx.x;
-    if (u >= all) continue;
-    const int run = u < 2 * (int64_t)codes ? u >= codes : 2 + (u >= 2 * (int64_t)codes + scales);
-    const int64_t in = run < 2 ? u - run * (int64_t)codes
-                               : u - 2 * (int64_t)codes - (run - 2) * (int64_t)scales;
-    to.p[run][db * (run < 2 ? codes : scales) + in] = v[i];
+  for (int i = 0; i < LOADS; ++i) {
+    int run, units;
+    const int in = place(i, &run, &units);
+    if (in >= 0) __builtin_nontemporal_store(v[i], to.p[run] + (int64_t)db * units + in);
   }
 }
 
-// Blocks src[i] to dst[i] (null: i), i below n and *count (null: n).
+// f(block, piece) for the workgroup's pieces of n blocks; workgroup w of W.
+template <typename F>
+__device__ inline void for_pieces(const Pieces& p, int64_t n, uint32_t w, uint32_t W, F&& f) {
+  int64_t i = p.by_per.div(w);
+  int piece = (int)(w - (uint32_t)i * p.per);
+  const uint32_t di = p.by_per.div(W);
+  const int dp = (int)(W - di * p.per);
+  while (i < n) {
+    f(i, piece);
+    i += di;
+    piece += dp;
+    if (piece >= p.per) {
+      piece -= p.per;
+      ++i;
+    }
+  }
+}
+
+// Blocks src[i] to dst[i], i below n and *count (null: n).
 __global__ void __launch_bounds__(PT)
 copy_kernel(const Store from, uint32_t from_blocks, const Store to, uint32_t to_blocks,
             const int32_t* __restrict__ src, const int32_t* __restrict__ dst, int64_t n,
-            const int32_t* __restrict__ count, int codes, int scales) {
-  const int64_t pieces = (2 * ((int64_t)codes + scales) + PIECE - 1) / PIECE;
+            const int32_t* __restrict__ count, const Pieces p) {
   if (count != nullptr) n = min(n, (int64_t)*count);
-  for (int64_t u = blockIdx.x; u < n * pieces; u += gridDim.x) {
-    const int64_t i = u / pieces;
-    const uint32_t sb = (uint32_t)src[i], db = dst == nullptr ? (uint32_t)i : (uint32_t)dst[i];
-    if (sb < from_blocks && db < to_blocks)
-      copy_piece(from, sb, to, db, u - i * pieces, codes, scales);
-  }
+  for_pieces(p, n, blockIdx.x, gridDim.x, [&](int64_t i, int piece) {
+    const uint32_t sb = (uint32_t)src[i], db = (uint32_t)dst[i];
+    if (sb < from_blocks && db < to_blocks) copy_piece(from, sb, to, db, piece, p);
+  });
 }
 
-// Tables whose entries are the blocks' places among the held ones; -1 where a
-// row holds nothing, or `into` has no such block.
+// The first `movers` workgroups move the held blocks, list[i] to i; the others
+// write tables whose entries are the blocks' places among the held ones, -1 where
+// a row holds nothing, or `into` has no such block.
 __global__ void __launch_bounds__(PT)
-renumber_kernel(const Rows t, uint32_t num_blocks, const int32_t* __restrict__ number,
-                int into_blocks, int32_t* __restrict__ out) {
+compact_kernel(const Store from, const Store to, uint32_t to_blocks, const Rows t,
+               uint32_t num_blocks, const int32_t* __restrict__ list,
+               const int32_t* __restrict__ number, const int32_t* __restrict__ used,
+               int32_t* __restrict__ out, uint32_t movers, const Pieces p) {
+  if (blockIdx.x < movers) {
+    for_pieces(p, min(*used, (int)to_blocks), blockIdx.x, movers,
+               [&](int64_t i, int piece) {
+                 copy_piece(from, (uint32_t)list[i], to, (uint32_t)i, piece, p);
+               });
+    return;
+  }
   const int parts = (t.width + ENTRIES - 1) / ENTRIES;
-  for (int64_t u = blockIdx.x; u < t.R * parts; u += gridDim.x) {
-    const int64_t r = u / parts;
+  for (int64_t u = blockIdx.x - movers; u < t.R * parts; u += gridDim.x - movers) {
+    const int64_t r = parts == 1 ? u : u / parts;
     const int lo = (int)(u - r * parts) * ENTRIES, hi = min(t.width, lo + ENTRIES);
     const int held = t.held(r);
     for (int e = lo + threadIdx.x; e < hi; e += PT) {
@@ -198,7 +339,7 @@ renumber_kernel(const Rows t, uint32_t num_blocks, const int32_t* __restrict__ n
       if (e < held) {
         const uint32_t b = (uint32_t)t.tables[r * t.stride + e];
         if (b < num_blocks) v = number[b];
-        if (v >= into_blocks) v = -1;
+        if (v >= (int)to_blocks) v = -1;
       }
       out[r * t.width + e] = v;
     }
@@ -211,7 +352,7 @@ renumber_kernel(const Rows t, uint32_t num_blocks, const int32_t* __restrict__ n
 struct Child {
   int64_t row;  // -1: nothing
   int seq, whole;
-  int part;  // block that its last tokens share with nothing else's; -1: none
+  int part;  // the block that its last tokens are in, if that is not full; -1: none
 };
 
 __device__ inline Child child_of(const Rows& t, const int32_t* parents, int64_t j,
@@ -230,25 +371,27 @@ __device__ inline Child child_of(const Rows& t, const int32_t* parents, int64_t 
   return c;
 }
 
-// first[b], for the blocks that some child ends in, becomes the lowest such
-// child, or -1 where a child has b as a whole block.
-__global__ void __launch_bounds__(PT)
-fork_clear_kernel(const Rows t, const int32_t* __restrict__ parents, int64_t F,
-                  uint32_t num_blocks, int32_t* __restrict__ first) {
-  const int64_t j = (int64_t)blockIdx.x * PT + threadIdx.x;
-  if (j >= F) return;
-  const Child c = child_of(t, parents, j, num_blocks);
-  if (c.part >= 0) first[c.part] = INT32_MAX;
+// Whether e is the number (child, entry) of a whole entry that names block b.
+__device__ inline bool whole_entry(const Rows& t, const int32_t* parents, int64_t F, uint32_t b,
+                                   uint32_t e) {
+  if (e >= (uint64_t)F * t.width) return false;
+  const uint32_t j = e >> 31 ? e / t.width : t.by_width.div(e);
+  const int c = (int)(e - j * (uint32_t)t.width);
+  const int64_t r = parents[j];
+  return r >= 0 && r < t.R && (uint32_t)t.tables[r * t.stride + c] == b &&
+         c < (int)((uint32_t)max(t.seq[r], 0) / t.bs);
 }
 
-// A workgroup per child: its row of the new tables, its length, its marks.
+// A workgroup per child: its row of the new tables, its length, the block it
+// ends in; and where a block is, the number of some child's whole entry that
+// names it (nothing is cleared before, as for mark_kernel).
 __global__ void __launch_bounds__(PT)
 fork_mark_kernel(const Rows t, const int32_t* __restrict__ parents, int64_t F,
-                 uint32_t num_blocks, int32_t* __restrict__ first, int32_t* __restrict__ out,
-                 int32_t* __restrict__ out_seq) {
+                 uint32_t num_blocks, uint32_t* __restrict__ entry, int32_t* __restrict__ part,
+                 int32_t* __restrict__ out, int32_t* __restrict__ out_seq) {
   const int64_t j = blockIdx.x;
   const Child c = child_of(t, parents, j, num_blocks);
-  // Marks of a parent are made once, or nearly: by the first of the last 1024
+  // A parent's marks are made once, or nearly: by the first of the last 1024
   // children that go on from it.
   bool seen = false;
   for (int64_t i = max(j - 1024, (int64_t)0) + threadIdx.x; i < j; i += PT)
@@ -260,7 +403,7 @@ fork_mark_kernel(const Rows t, const int32_t* __restrict__ parents, int64_t F,
       const uint32_t b = (uint32_t)t.tables[c.row * t.stride + e];
       if (b < num_blocks) {
         v = (int32_t)b;
-        if (!seen) __hip_atomic_fetch_min(first + b, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!seen) entry[b] = (uint32_t)(j * t.width + e);
       }
     } else if (e == c.whole) {
       v = c.part;
@@ -269,45 +412,135 @@ fork_mark_kernel(const Rows t, const int32_t* __restrict__ parents, int64_t F,
   }
   if (threadIdx.x == 0) {
     out_seq[j] = c.seq;
-    if (c.part >= 0)
-      __hip_atomic_fetch_min(first + c.part, (int)j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    part[j] = c.part;
   }
 }
 
-// One workgroup: which children get a block of their own, in order.
+// Child j's new block b, the k-th of the free list.
+__device__ inline int32_t fresh_block(const int32_t* free_blocks, int64_t num_free, int64_t k,
+                                      uint32_t num_blocks) {
+  const int32_t b = k < num_free ? free_blocks[k] : -1;
+  return (uint32_t)b < num_blocks ? b : -1;
+}
+
+__device__ inline int64_t last_entry(const Rows& t, int64_t j, const int32_t* out_seq) {
+  return j * t.width + (uint32_t)out_seq[j] / t.bs;
+}
+
+// Up to FEW children: a workgroup per child and piece finds by itself which
+// children get a block of their own (those that another ends in, in LDS), and
+// copies.
+constexpr int FEW = 1024, SLOTS = 2 * FEW;
+__global__ void __launch_bounds__(PT)
+fork_few_kernel(const Rows t, const int32_t* __restrict__ parents, int F, uint32_t num_blocks,
+                const uint32_t* __restrict__ entry, const int32_t* __restrict__ part,
+                const int32_t* __restrict__ free_blocks, int64_t num_free,
+                int32_t* __restrict__ out, const int32_t* __restrict__ out_seq,
+                int32_t* __restrict__ taken, const Store store, const Pieces p) {
+  constexpr int PER = FEW / PT;
+  __shared__ int keys[SLOTS], lowest[SLOTS];
+  __shared__ int s[PT / 64];
+  const int j = (int)p.by_per.div(blockIdx.x), piece = (int)blockIdx.x - j * p.per;
+  int mine[PER];
+  const int own = part[j];
+  bool copies = false;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int k = i * PT + threadIdx.x;
+    mine[i] = k < F ? part[k] : -1;
+    copies |= k < j && mine[i] == own;
+  }
+  // Most children need no copy; the first workgroup counts them all the same.
+  if (blockIdx.x != 0) {
+    if (own < 0) return;
+    copies = __syncthreads_or(copies || (threadIdx.x == 0 &&
+                                         whole_entry(t, parents, F, own, entry[own])));
+    if (!copies) return;
+  }
+  bool whole[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    whole[i] = mine[i] >= 0 && whole_entry(t, parents, F, mine[i], entry[mine[i]]);
+  for (int i = threadIdx.x; i < SLOTS; i += PT) {
+    keys[i] = -1;
+    lowest[i] = INT32_MAX;
+  }
+  __syncthreads();
+  int slot[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (mine[i] < 0) continue;
+    // (at most half of the slots are ever taken: this ends)
+    int h = (int)((uint32_t)mine[i] * 2654435761u >> 21) & (SLOTS - 1);
+    for (;;) {
+      const int was = atomicCAS(&keys[h], -1, mine[i]);
+      if (was == -1 || was == mine[i]) break;
+      h = (h + 1) & (SLOTS - 1);
+    }
+    atomicMin(&lowest[h], i * PT + (int)threadIdx.x);
+    slot[i] = h;
+  }
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int k = i * PT + threadIdx.x;
+    const bool c = mine[i] >= 0 && (whole[i] || lowest[slot[i]] != k);
+    all += c;
+    before += c && k < j;
+  }
+  wg_scan<PT>(before, s, &before);
+  wg_scan<PT>(all, s, &all);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *taken = all;
+  if (blockIdx.x == 0) {  // does child 0 itself need one?
+    copies = __syncthreads_or(threadIdx.x == 0 && mine[0] >= 0 && whole[0]);
+    if (!copies) return;
+  }
+  const int32_t b = fresh_block(free_blocks, num_free, before, num_blocks);
+  if (piece == 0 && threadIdx.x == 0) out[last_entry(t, j, out_seq)] = b;
+  if (b >= 0) copy_piece(store, (uint32_t)own, store, (uint32_t)b, piece, p);
+}
+
+// Any number of children: one workgroup finds them, with the lowest child that
+// ends in a block in `first`.
 constexpr int FT = 1024;
 __global__ void __launch_bounds__(FT)
 fork_place_kernel(const Rows t, const int32_t* __restrict__ parents, int64_t F,
-                  uint32_t num_blocks, const int32_t* __restrict__ first,
+                  uint32_t num_blocks, const uint32_t* __restrict__ entry,
+                  const int32_t* __restrict__ part, int32_t* first,
                   const int32_t* __restrict__ free_blocks, int64_t num_free,
-                  int32_t* __restrict__ out, int32_t* __restrict__ src,
-                  int32_t* __restrict__ dst, int32_t* __restrict__ taken) {
+                  int32_t* __restrict__ out, const int32_t* __restrict__ out_seq,
+                  int32_t* __restrict__ dst, int32_t* __restrict__ src,
+                  int32_t* __restrict__ taken) {
   __shared__ int s[FT / 64];
+  // (Agent scope: what this workgroup's other waves wrote is past their caches.)
+  for (int64_t j = threadIdx.x; j < F; j += FT)
+    if (part[j] >= 0)
+      __hip_atomic_store(first + part[j], INT32_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __threadfence();
+  __syncthreads();
+  for (int64_t j = threadIdx.x; j < F; j += FT)
+    if (part[j] >= 0)
+      __hip_atomic_fetch_min(first + part[j], (int)j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __threadfence();
+  __syncthreads();
   int base = 0;
   for (int64_t j0 = 0; j0 < F; j0 += FT) {
     const int64_t j = j0 + threadIdx.x;
-    Child c{-1, 0, 0, -1};
-    if (j < F) c = child_of(t, parents, j, num_blocks);
-    const bool copy = c.part >= 0 && first[c.part] != (int)j;
-    int at = wave_incl_scan(copy);
-    if ((threadIdx.x & 63) == 63) s[threadIdx.x >> 6] = at;
-    __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < FT / 64; ++w) {
-      at += w < (int)(threadIdx.x >> 6) ? s[w] : 0;
-      all += s[w];
-    }
+    const int mine = j < F ? part[j] : -1;
+    const bool copy =
+        mine >= 0 && (__hip_atomic_load(first + mine, __ATOMIC_RELAXED,
+                                        __HIP_MEMORY_SCOPE_AGENT) != (int)j ||
+                      whole_entry(t, parents, F, mine, entry[mine]));
+    int all;
+    const int at = base + wg_scan<FT>(copy, s, &all) - 1;
     if (copy) {
-      at += base - 1;
-      int32_t b = at < num_free ? free_blocks[at] : -1;
-      if ((uint32_t)b >= num_blocks) b = -1;
-      src[at] = c.part;
+      const int32_t b = fresh_block(free_blocks, num_free, at, num_blocks);
+      src[at] = mine;
       dst[at] = b;
-      out[j * t.width + c.whole] = b;
+      out[last_entry(t, j, out_seq)] = b;
     }
     base += all;
-    __syncthreads();
   }
   if (threadIdx.x == 0) *taken = base;
 }
@@ -315,11 +548,13 @@ fork_place_kernel(const Rows t, const int32_t* __restrict__ parents, int64_t F,
 // ------------------------------------------------- workspaces, launches
 
 struct Names {
-  uint8_t* named;
+  uint32_t* entry;
+  uint64_t* masks;
   int32_t* counts;
   int64_t chunks;
   Names(Carve& w, int64_t num_blocks) : chunks((num_blocks + CHUNK - 1) / CHUNK) {
-    named = w.take<uint8_t>((size_t)chunks * CHUNK);
+    entry = w.take<uint32_t>((size_t)num_blocks);
+    masks = w.take<uint64_t>((size_t)chunks * CHUNK / 64);
     counts = w.take<int32_t>((size_t)chunks);
   }
 };
@@ -332,31 +567,36 @@ uint32_t grid_for(int64_t items, int per_cu) {
 int64_t row_parts(const Kv4Tables& t) { return t.R * ((t.max_blocks + ENTRIES - 1) / ENTRIES); }
 
 Rows rows_of(const Kv4Tables& t, int64_t bs) {
-  return Rows{t.tables, t.stride, t.seq, t.R, (int)t.max_blocks, (uint32_t)bs};
-}
-
-void launch_names(const Kv4Tables& t, int64_t bs, int64_t num_blocks, const Names& n,
-                  hipStream_t s) {
-  hipLaunchKernelGGL(clear_kernel, dim3(grid_for((n.chunks * CHUNK / 4 + PT - 1) / PT, 8)),
-                     dim3(PT), 0, s, (uint32_t*)n.named, n.chunks * CHUNK / 4);
-  if (row_parts(t) > 0)
-    hipLaunchKernelGGL(mark_kernel, dim3(grid_for(row_parts(t), 16)), dim3(PT), 0, s,
-                       rows_of(t, bs), (uint32_t)num_blocks, n.named);
-  hipLaunchKernelGGL(count_kernel, dim3((uint32_t)n.chunks), dim3(PT), 0, s, n.named, num_blocks,
-                     n.counts);
-}
-
-void launch_copy(const fkc_kv4_cache& from, const fkc_kv4_cache& to, const int32_t* src,
-                 const int32_t* dst, int64_t n, const int32_t* count, hipStream_t s) {
-  const int codes = (int)(from.heads * from.block_size * from.D / 32);
-  const int scales = (int)(from.heads * from.block_size / 8);
-  const int64_t pieces = (2 * ((int64_t)codes + scales) + PIECE - 1) / PIECE;
-  hipLaunchKernelGGL(copy_kernel, dim3(grid_for(n * pieces, 8)), dim3(PT), 0, s, Store(from),
-                     (uint32_t)from.num_blocks, Store(to), (uint32_t)to.num_blocks, src, dst, n,
-                     count, codes, scales);
+  return Rows{t.tables, t.stride, t.seq, t.R, (int)t.max_blocks, (uint32_t)bs,
+              FastDiv((uint32_t)t.max_blocks)};
 }
 
 __global__ void zero_kernel(int32_t* p) { *p = 0; }
+
+template <bool FREE>
+void launch_names(const Kv4Tables& t, int64_t bs, int64_t num_blocks, const Names& n,
+                  int32_t* list, int32_t* number, int32_t* total, hipStream_t s) {
+  if (num_blocks == 0) {
+    hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(1), 0, s, total);
+    return;
+  }
+  const Rows r = rows_of(t, bs);
+  const dim3 chunks((uint32_t)n.chunks);
+  if (num_blocks <= kSmallBlocks && t.R * t.max_blocks <= kSmallEntries) {
+    hipLaunchKernelGGL(names_small_kernel<FREE>, chunks, dim3(ST), 0, s, r, (uint32_t)num_blocks,
+                       list, number, total);
+    return;
+  }
+  if (row_parts(t) > 0)
+    hipLaunchKernelGGL(mark_kernel, dim3(grid_for(row_parts(t), 16)), dim3(PT), 0, s, r,
+                       (uint32_t)num_blocks, n.entry);
+  hipLaunchKernelGGL(count_kernel, chunks, dim3(PT), 0, s, r, num_blocks, n.entry, n.masks,
+                     n.counts);
+  hipLaunchKernelGGL(list_kernel<FREE>, chunks, dim3(PT), 0, s, num_blocks, n.masks, n.counts,
+                     list, number, total);
+}
+
+uint32_t copy_grid(int64_t blocks, const Pieces& p) { return grid_for(blocks * p.per, 8); }
 
 }  // namespace
 
@@ -369,14 +609,7 @@ size_t free_blocks_workspace_bytes(int64_t num_blocks) {
 int launch_free_blocks(const Kv4Tables& t, int64_t bs, int64_t num_blocks, int32_t* free_blocks,
                        int32_t* count, void* ws, hipStream_t s) {
   Carve w(ws);
-  const Names n(w, num_blocks);
-  if (num_blocks == 0) {
-    hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(1), 0, s, count);
-    return check_launch("free_blocks");
-  }
-  launch_names(t, bs, num_blocks, n, s);
-  hipLaunchKernelGGL(list_kernel<true>, dim3((uint32_t)n.chunks), dim3(PT), 0, s, n.named,
-                     num_blocks, n.counts, free_blocks, (int32_t*)nullptr, count);
+  launch_names<true>(t, bs, num_blocks, Names(w, num_blocks), free_blocks, nullptr, count, s);
   return check_launch("free_blocks");
 }
 
@@ -393,53 +626,62 @@ int launch_kv4_compact(const fkc_kv4_cache& c, const Kv4Tables& t, const fkc_kv4
   const Names n(w, c.num_blocks);
   int32_t* list = w.take<int32_t>((size_t)c.num_blocks * 2);
   int32_t* number = list + c.num_blocks;
-  if (c.num_blocks == 0) {
-    hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(1), 0, s, used);
-  } else {
-    launch_names(t, c.block_size, c.num_blocks, n, s);
-    hipLaunchKernelGGL(list_kernel<false>, dim3((uint32_t)n.chunks), dim3(PT), 0, s, n.named,
-                       c.num_blocks, n.counts, list, number, used);
-  }
-  if (row_parts(t) > 0)
-    hipLaunchKernelGGL(renumber_kernel, dim3(grid_for(row_parts(t), 16)), dim3(PT), 0, s,
-                       rows_of(t, c.block_size), (uint32_t)c.num_blocks, number,
-                       (int)into.num_blocks, new_tables);
+  launch_names<false>(t, c.block_size, c.num_blocks, n, list, number, used, s);
+  const Pieces p(c);
   const int64_t most = std::min(c.num_blocks, into.num_blocks);
-  if (most > 0) launch_copy(c, into, list, nullptr, most, used, s);
+  const uint32_t movers = most > 0 ? copy_grid(most, p) : 0;
+  const uint32_t writers = row_parts(t) > 0 ? grid_for(row_parts(t), 2) : 0;
+  if (movers + writers > 0)
+    hipLaunchKernelGGL(compact_kernel, dim3(movers + writers), dim3(PT), 0, s, Store(c),
+                       Store(into), (uint32_t)into.num_blocks, rows_of(t, c.block_size),
+                       (uint32_t)c.num_blocks, list, number, used, new_tables, movers, p);
   return check_launch("kv4_compact");
 }
 
 int launch_kv4_copy_blocks(const fkc_kv4_cache& c, const int32_t* src, const fkc_kv4_cache& into,
                            const int32_t* dst, int64_t n, hipStream_t s) {
-  launch_copy(c, into, src, dst, n, nullptr, s);
+  const Pieces p(c);
+  hipLaunchKernelGGL(copy_kernel, dim3(copy_grid(n, p)), dim3(PT), 0, s, Store(c),
+                     (uint32_t)c.num_blocks, Store(into), (uint32_t)into.num_blocks, src, dst, n,
+                     (const int32_t*)nullptr, p);
   return check_launch("kv4_copy_blocks");
 }
 
 size_t kv4_fork_workspace_bytes(const fkc_kv4_cache& c, int64_t F) {
   Carve w(nullptr);
-  w.take<int32_t>((size_t)c.num_blocks);
-  w.take<int32_t>((size_t)F * 2);
+  w.take<uint32_t>((size_t)c.num_blocks);
+  w.take<int32_t>((size_t)F);
+  if (F > FEW) w.take<int32_t>((size_t)F * 2 + (size_t)c.num_blocks);
   return w.used;
 }
 
 int launch_kv4_fork(const fkc_kv4_cache& c, const Kv4Tables& t, const int32_t* parents, int64_t F,
                     const int32_t* free_blocks, int64_t num_free, int32_t* new_tables,
                     int32_t* new_seq, int32_t* taken, void* ws, hipStream_t s) {
+  if (F == 0) {
+    hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(1), 0, s, taken);
+    return check_launch("kv4_fork");
+  }
   Carve w(ws);
-  int32_t* first = w.take<int32_t>((size_t)c.num_blocks);
-  int32_t* src = w.take<int32_t>((size_t)F * 2);
-  int32_t* dst = src + F;
+  uint32_t* entry = w.take<uint32_t>((size_t)c.num_blocks);
+  int32_t* part = w.take<int32_t>((size_t)F);
   const Rows r = rows_of(t, c.block_size);
   const uint32_t nb = (uint32_t)c.num_blocks;
-  if (F > 0) {
-    hipLaunchKernelGGL(fork_clear_kernel, dim3((uint32_t)((F + PT - 1) / PT)), dim3(PT), 0, s, r,
-                       parents, F, nb, first);
-    hipLaunchKernelGGL(fork_mark_kernel, dim3((uint32_t)F), dim3(PT), 0, s, r, parents, F, nb,
-                       first, new_tables, new_seq);
+  const Pieces p(c);
+  hipLaunchKernelGGL(fork_mark_kernel, dim3((uint32_t)F), dim3(PT), 0, s, r, parents, F, nb,
+                     entry, part, new_tables, new_seq);
+  if (F <= FEW) {
+    hipLaunchKernelGGL(fork_few_kernel, dim3((uint32_t)(F * p.per)), dim3(PT), 0, s, r, parents,
+                       (int)F, nb, entry, part, free_blocks, num_free, new_tables, new_seq, taken,
+                       Store(c), p);
+    return check_launch("kv4_fork");
   }
-  hipLaunchKernelGGL(fork_place_kernel, dim3(1), dim3(FT), 0, s, r, parents, F, nb, first,
-                     free_blocks, num_free, new_tables, src, dst, taken);
-  if (F > 0 && nb > 0) launch_copy(c, c, src, dst, F, taken, s);
+  int32_t* first = w.take<int32_t>((size_t)F * 2 + (size_t)c.num_blocks);
+  int32_t *src = first + c.num_blocks, *dst = src + F;
+  hipLaunchKernelGGL(fork_place_kernel, dim3(1), dim3(FT), 0, s, r, parents, F, nb, entry, part,
+                     first, free_blocks, num_free, new_tables, new_seq, dst, src, taken);
+  hipLaunchKernelGGL(copy_kernel, dim3(copy_grid(F, p)), dim3(PT), 0, s, Store(c), nb, Store(c),
+                     nb, src, dst, F, taken, p);
   return check_launch("kv4_fork");
 }
 

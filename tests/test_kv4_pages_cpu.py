@@ -28,7 +28,8 @@ def test_free_blocks_refusals():
     ok = [FAKE, 8, 8, FAKE, 3, 16, 40, FAKE, FAKE, FAKE, need, None]
     for at, value, code, word in (
             (0, None, 1, "null"), (1, 7, 1, "overlap"), (2, -1, 1, "range"), (3, None, 1, "null"),
-            (4, -1, 1, "range"), (4, 1 << 31, 1, "range"), (5, 0, 1, "range"),
+            (4, -1, 1, "range"), (4, 1 << 31, 1, "range"), (4, 1 << 29, 4, "2^32"),
+            (5, 0, 1, "range"),
             (5, (1 << 20) + 1, 1, "range"), (6, -1, 1, "range"), (6, 1 << 31, 1, "range"),
             (7, None, 1, "null"), (8, None, 1, "null"), (9, None, 2, "workspace"),
             (9, FAKE + 16, 2, "aligned"), (10, need - 1, 2, "workspace")):
@@ -46,6 +47,7 @@ def test_fork_refusals():
     for at, value, code, word in (
             (0, None, 1, "null cache"), (1, None, 1, "null"), (2, 7, 1, "overlap"),
             (3, -1, 1, "range"), (4, None, 1, "null"), (5, -1, 1, "range"), (6, None, 1, "null"),
+            (5, 1 << 29, 4, "2^32"), (7, 1 << 29, 4, "2^32"),
             (7, -1, 1, "range"), (8, None, 1, "null"), (9, -1, 1, "range"), (10, None, 1, "null"),
             (11, None, 1, "null"), (12, None, 1, "null"), (13, None, 2, "workspace"),
             (13, FAKE + 8, 2, "aligned"), (14, need - 1, 2, "workspace")):
