@@ -289,9 +289,13 @@ struct MState : State<DT, D, NT> {
   using S::o;
   static constexpr int ND = S::ND;
   __device__ inline float base2(int y, float zscale) const {
-    if constexpr (MODE == kMask) return S::base2(y, zscale);
-    return DT == FKC_F16 ? m[y] - 14.f : __builtin_amdgcn_fmed3f(m[y], kLowest, -kLowest);
+    if constexpr (DT == FKC_F16) return m[y] - kLead;
+    return __builtin_amdgcn_fmed3f(MODE == kMask ? m[y] * zscale : m[y], kLowest, -kLowest);
   }
+  // What m may lag behind the largest score (powers of two) before everything is
+  // made relative to a new one; fp16: 2^kLead is the largest weight times scale
+  // without a lag, so 2^14 with it.
+  static constexpr float kLag = DT == FKC_F16 ? 6.f : 8.f, kLead = 8.f;
   // tok: this lane's first token.  zscale: of the mode's first step.
   __device__ inline void weights(f32x4 (&s)[NT][2], const uint2 (&kw)[2], const uint2 (&vw)[2],
                                  bool masked, int base0, int base1, int tok,
@@ -367,7 +371,7 @@ struct MState : State<DT, D, NT> {
                                           : z[j][i] + ve[j][i];
           top = fmaxf(top, v);
         }
-      if (__any(top > m[y])) {
+      if (__any(DT == FKC_F16 || MODE != kMask ? top > m[y] + kLag : (top - m[y]) * zscale > kLag)) {
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float nm = fmaxf(m[y], top);

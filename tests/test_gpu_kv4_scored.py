@@ -311,16 +311,22 @@ def test_rows_of_no_request_beside_cut_ones(kv4, dtype, D, G):
 
 def test_the_options_of_nothing_are_none(kv4):
     """A cap far above every score, slopes of 0, a window of everything, no
-    documents and no prefix: the answer without options, within rounding."""
+    documents and no prefix: the answer without options.  Not its bits: a weight
+    is rounded to the type relative to a maximum, which may lag here and does not
+    there, and w 2^-a rounded times 2^a is w rounded only for whole a.  Both are
+    within the bound of one rounding of each weight and of the result, which is
+    what the reference's tolerance counts, so they are within twice that of each
+    other."""
     seq, nq = [300, 700], [300, 5]
     cache, tables, g = _setup(seq, 16, 2, 128, BF16, 3)
     q = torch.randn(sum(nq), 8, 128, generator=g).to(BF16)
     dev = kv4.Cache(*(t.cuda() for t in cache))
     args = q.cuda(), dev, tables.cuda(), i32(seq), i32([0, 300, 305])
-    want = kv4.attend(*args)
+    want = kv4.attend(*args).cpu().double()
+    tol = sref.attend(q, cache, tables, seq, nq)[2]
     zero = torch.zeros(305, dtype=torch.int32, device="cuda")
     for kw in (dict(window=10 ** 6), dict(starts=zero), dict(prefix_lens=zero[:2])):
-        assert torch.equal(kv4.attend(*args, **kw), want)
+        assert bool(((kv4.attend(*args, **kw).cpu().double() - want).abs() <= 2 * tol).all())
     for kw in (dict(softcap=1e6), dict(slopes=torch.zeros(8, device="cuda"))):
         _check(kv4, cache, tables, q, seq, nq, **{k: v.cpu() if isinstance(v, torch.Tensor) else v
                                                   for k, v in kw.items()})
