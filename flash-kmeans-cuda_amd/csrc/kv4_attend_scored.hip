@@ -279,8 +279,19 @@ struct Columns {
   }
 };
 
-// As State (kv4_tile.hpp), with scores as above.  kMask keeps scores before their
-// scale zscale, as there; the others have them in powers of two.
+// fp16: what a value scale adds to the maximum: its exponent, rounded up; zero
+// counts as 2^-60.
+__device__ inline float exponent_of(float scale) {
+  return fmaxf((float)(int)(__float_as_uint(fabsf(scale)) >> 23) - 126.f, -60.f);
+}
+
+// As State (kv4_tile.hpp), with scores as above, in the steps that a kernel may
+// put between its products.  What stands for a score z in powers of two:
+//   kMask  z / zscale,
+//   kCap   r = 1 / (1 + e^2x), with z = cap2 / 2 - cap2 r (hidden: r = infinity),
+//   kBias  z - shift, one shift per column and tile,
+// so that the last multiplication is the one that the weight's exponent needs
+// anyway.
 template <int DT, int D, int NT, int MODE>
 struct MState : State<DT, D, NT> {
   typedef State<DT, D, NT> S;
@@ -288,20 +299,20 @@ struct MState : State<DT, D, NT> {
   using S::m;
   using S::o;
   static constexpr int ND = S::ND;
-  __device__ inline float base2(int y, float zscale) const {
-    if constexpr (DT == FKC_F16) return m[y] - kLead;
-    return __builtin_amdgcn_fmed3f(MODE == kMask ? m[y] * zscale : m[y], kLowest, -kLowest);
-  }
   // What m may lag behind the largest score (powers of two) before everything is
   // made relative to a new one; fp16: 2^kLead is the largest weight times scale
   // without a lag, so 2^14 with it.
   static constexpr float kLag = DT == FKC_F16 ? 6.f : 8.f, kLead = 8.f;
-  // tok: this lane's first token.  zscale: of the mode's first step.
-  __device__ inline void weights(f32x4 (&s)[NT][2], const uint2 (&kw)[2], const uint2 (&vw)[2],
-                                 bool masked, int base0, int base1, int tok,
-                                 const Columns<MODE, NT>& c, float zscale, float cap2,
-                                 u32x4 (&pf)[NT]) {
-    float ks[2][4], vs[2][4];
+  static constexpr float kHidden = MODE == kCap ? INFINITY : -INFINITY;
+  // Of the tile at hand: the keys' scales, times the first step's factor but for
+  // kMask, the values', and (fp16) exponent_of these.
+  f32x4 ks[2], vs[2], ve[DT == FKC_F16 ? 2 : 1];
+  float shift[MODE == kBias ? NT : 1];
+  __device__ inline float base2(int y, float zscale) const {
+    if constexpr (DT == FKC_F16) return m[y] - kLead;
+    return __builtin_amdgcn_fmed3f(MODE == kMask ? m[y] * zscale : m[y], kLowest, -kLowest);
+  }
+  __device__ inline void scales(const uint2 (&kw)[2], const uint2 (&vw)[2], float zscale) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -310,71 +321,117 @@ struct MState : State<DT, D, NT> {
         ks[j][i] = from16<DT>((i & 1) ? kx >> 16 : kx & 0xffffu);
         vs[j][i] = from16<DT>((i & 1) ? vx >> 16 : vx & 0xffffu);
         if constexpr (MODE != kMask) ks[j][i] *= zscale;
+        if constexpr (DT == FKC_F16) ve[j][i] = exponent_of(vs[j][i]);
       }
-    if (masked) {  // what lies past the requests' tokens is anything
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((j ? base1 : base0) < 0 || tok + 16 * j + i >= c.hi) vs[j][i] = 0.f;
-          rare(vs[j][i]);
-        }
-    }
-    float ve[2][4];  // fp16: the value scales' exponents; zero counts as 2^-60
-    if constexpr (DT == FKC_F16) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          ve[j][i] = fmaxf((float)(int)(__float_as_uint(fabsf(vs[j][i])) >> 23) - 126.f, -60.f);
-    }
+  }
+  // Products to scores, in place.  tok: this lane's first token, first: the tile's.
+  __device__ inline void score(f32x4 (&z)[NT][2], int tok, int first,
+                               const Columns<MODE, NT>& c, float cap2) {
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
-      float z[2][4], top = kLowest;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z[j][i] = s[y][j][i] * ks[j][i];
+        for (int i = 0; i < 4; ++i) z[y][j][i] *= ks[j][i];
       if (MODE == kCap || (MODE == kBias && cap2 != 0.f)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            z[j][i] = __builtin_fmaf(
-                -cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[j][i])), 0.5f * cap2);
-      }
-      if constexpr (MODE == kBias) {
-        const float away = (float)(c.pos[y] - tok);  // rounded past 2^24 only
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            z[j][i] = __builtin_fmaf(-c.slope[y], fabsf(away - (float)(16 * j + i)), z[j][i]);
-      }
-      if (masked) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int x = tok + 16 * j + i;
-            if ((j ? base1 : base0) < 0 || x < c.first[y] || x >= c.last[y])
-              z[j][i] = -INFINITY;
-            rare(z[j][i]);
+            const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[y][j][i]));
+            z[y][j][i] = MODE == kCap ? r : __builtin_fmaf(-cap2, r, 0.5f * cap2);
           }
       }
+      if constexpr (MODE == kBias) {
+        // Before all of the tile or behind it a column's distances rise or fall by
+        // one from token to token.
+        const int away = c.pos[y] - tok;  // (exact in fp32 below 2^24)
+        if (!__any(c.pos[y] > first && c.pos[y] < first + 31)) {
+          const float per = c.pos[y] > first ? c.slope[y] : -c.slope[y];
+          shift[y] = -per * (float)away;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              z[y][j][i] = __builtin_fmaf(per, (float)(16 * j + i), z[y][j][i]);
+        } else {
+          shift[y] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              z[y][j][i] =
+                  __builtin_fmaf(-c.slope[y], fabsf((float)(away - 16 * j - i)), z[y][j][i]);
+        }
+      }
+    }
+  }
+  // For tiles that some column does not see all of.
+  __device__ inline void mask(f32x4 (&z)[NT][2], int base0, int base1, int tok,
+                              const Columns<MODE, NT>& c) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = tok + 16 * j + i;
+#pragma unroll
+        for (int y = 0; y < NT; ++y) {
+          float v = z[y][j][i];
+          if ((j ? base1 : base0) < 0 || x < c.first[y] || x >= c.last[y]) v = kHidden;
+          rare(v);
+          z[y][j][i] = v;
+        }
+      }
+  }
+  // And their values' scales: 0 for what no column sees, which may be anything.
+  // Returns whether one is not finite all the same, so that its product with a
+  // hidden column's weight, 0, would not be 0.
+  __device__ inline bool mask_values(int base0, int base1, int tok, const Columns<MODE, NT>& c) {
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int x = tok + 16 * j + i;
+        float s = vs[j][i];
+        if ((j ? base1 : base0) < 0 || x >= c.hi || x < c.lo) s = 0.f;
+        rare(s);
+        vs[j][i] = s;
+        odd |= !(fabsf(s) < INFINITY);
+      }
+    return __any(odd);
+  }
+  // The maxima, and what follows from new ones.
+  __device__ inline void settle(const f32x4 (&z)[NT][2], float zscale, float cap2) {
+    float top[NT];
+    bool more = false;
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      float t = DT != FKC_F16 && MODE == kCap ? INFINITY : -INFINITY;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = DT != FKC_F16   ? z[j][i]
-                          : MODE == kMask ? __builtin_fmaf(z[j][i], zscale, ve[j][i])
-                                          : z[j][i] + ve[j][i];
-          top = fmaxf(top, v);
+          const float v = z[y][j][i];
+          if constexpr (DT != FKC_F16)
+            t = MODE == kCap ? fminf(t, v) : fmaxf(t, v);
+          else
+            t = fmaxf(t, MODE == kMask  ? __builtin_fmaf(v, zscale, ve[j][i])
+                         : MODE == kCap ? __builtin_fmaf(-cap2, v, ve[j][i])
+                                        : v + ve[j][i]);
         }
-      if (__any(DT == FKC_F16 || MODE != kMask ? top > m[y] + kLag : (top - m[y]) * zscale > kLag)) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float nm = fmaxf(m[y], top);
+      if constexpr (MODE == kCap)
+        t = DT != FKC_F16 ? __builtin_fmaf(-cap2, t, 0.5f * cap2) : t + 0.5f * cap2;
+      if constexpr (MODE == kBias) t += shift[y];
+      top[y] = t;
+      more |= DT == FKC_F16 || MODE != kMask ? t > m[y] + kLag : (t - m[y]) * zscale > kLag;
+    }
+    if (__any(more)) {
+#pragma unroll
+      for (int y = 0; y < NT; ++y) {
+        float t = fmaxf(top[y], __shfl_xor(top[y], 16, 64));
+        t = fmaxf(t, __shfl_xor(t, 32, 64));
+        const float nm = fmaxf(m[y], t);
         const float f = __builtin_amdgcn_exp2f(
             DT == FKC_F16 || MODE != kMask ? m[y] - nm : (m[y] - nm) * zscale);
         m[y] = nm;
@@ -382,29 +439,54 @@ struct MState : State<DT, D, NT> {
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[y][d] *= f;
       }
-      const float mz = base2(y, zscale);
+    }
+  }
+  // What the exponent of a weight is: one operation from what stands for z.
+  __device__ inline float exponent(float v, float base, float zscale, float cap2) const {
+    return MODE == kMask  ? __builtin_fmaf(v, zscale, base)
+           : MODE == kCap ? __builtin_fmaf(-cap2, v, base)
+                          : v + base;
+  }
+  __device__ inline float base_of(int y, float zscale, float cap2) const {
+    const float b = -base2(y, zscale);
+    return MODE == kCap ? 0.5f * cap2 + b : MODE == kBias ? shift[y] + b : b;
+  }
+  // Scores to weights, packed as the second product reads them.
+  __device__ inline void weigh(const f32x4 (&z)[NT][2], float zscale, float cap2,
+                               u32x4 (&pf)[NT]) {
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      const float base = base_of(y, zscale, cap2);
       float w[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(
-              MODE == kMask ? __builtin_fmaf(z[j][i], zscale, -mz) : z[j][i] - mz);
+          const float p = __builtin_amdgcn_exp2f(exponent(z[y][j][i], base, zscale, cap2));
           l[y] += p;
           w[j][i] = p * vs[j][i];
         }
-      if (masked) {  // a scale that is not finite counts where it is seen
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            w[j][i] = z[j][i] == -INFINITY ? 0.f : w[j][i];
-            rare(w[j][i]);
-          }
-      }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         pf[y][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
+    }
+  }
+  // After mask's true: the weights once more, 0 for what is hidden.
+  __device__ inline void weigh_odd(const f32x4 (&z)[NT][2], float zscale, float cap2,
+                                   u32x4 (&pf)[NT]) {
+#pragma unroll
+    for (int y = 0; y < NT; ++y) {
+      const float base = base_of(y, zscale, cap2);
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = z[y][e >> 2][e & 3];
+        w[e] = __builtin_amdgcn_exp2f(exponent(v, base, zscale, cap2)) * vs[e >> 2][e & 3];
+        w[e] = v == kHidden ? 0.f : w[e];
+        rare(w[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pf[y][e] = pack2<DT>(w[2 * e], w[2 * e + 1]);
     }
   }
 };
@@ -529,8 +611,17 @@ kv4_masked_split_kernel(const MArgs margs) {
       load_scales<D>(a, nbase, lanes, cur);
       u32x4 pf[NT];
       const int tok = t0 + it * 32;
-      st.weights(s, kw, vw, tok + 32 > cols.to || tok < cols.from || (base[0] | base[1]) < 0,
-                 base[0], base[1], tok + 4 * g, cols, zscale, cap2, pf);
+      const bool masked = tok + 32 > cols.to || tok < cols.from || (base[0] | base[1]) < 0;
+      st.scales(kw, vw, zscale);
+      st.score(s, tok + 4 * g, tok, cols, cap2);
+      bool odd = false;
+      if (masked) {
+        st.mask(s, base[0], base[1], tok + 4 * g, cols);
+        odd = st.mask_values(base[0], base[1], tok + 4 * g, cols);
+      }
+      st.settle(s, zscale, cap2);
+      st.weigh(s, zscale, cap2, pf);
+      if (odd) st.weigh_odd(s, zscale, cap2, pf);
       // Features 2 b and 2 b + 1 of the lane's row, two tokens a dword.
 #pragma unroll
       for (int v = 0; v < (ND + 7) / 8; ++v) {
@@ -628,25 +719,64 @@ kv4_masked_split_kernel(const MArgs margs) {
   }
 }
 
-template <int DT, int D, int NT, int TT, int MODE>
-__global__ void __launch_bounds__(512, 2)
+// The wide form, for prompts: every wave has a tile of 16 columns of its own, and
+// all of a workgroup's go over the same tokens.  These are looked up once for
+// all: each wave turns its share of the codes into the fragments of both
+// products, laid out so that a fragment is read by 64 lanes in a row (16 bytes
+// each, no bank conflict), in one of two buffers; while a stage of G groups of
+// 32 tokens is computed on, the next one is filled into the other.
+//
+// Feature row n of fragment d of the second product is feature 32 (d / 2) + 2 n +
+// d % 2: the two codes of one byte go to two fragments, and 16 lanes read 16
+// bytes of a token.
+template <int D>
+struct Wide {
+  static constexpr int WAVES = D == 256 ? 12 : 16, PER_SIMD = WAVES / 4;
+  static constexpr int COLS = 16 * WAVES, THREADS = WAVES * 64;
+  static constexpr int KS = D / 32, ND = D / 16;
+  static constexpr int G = 256 / D;            // groups of a stage
+  static constexpr int GROUP = 32 * D * 2;     // bytes of a group's keys or values
+  static constexpr int BUF = 2 * G * GROUP;    // keys, then values
+  // Scales of a stage in fp32: keys', values', and (fp16) exponent_of these, per
+  // group.
+  static constexpr int SCALES = 3 * 32 * 4;
+  static constexpr int kBuffers = kTable, kScales = kBuffers + 2 * BUF,
+                       kShares = kScales + 2 * G * SCALES;
+  // Of a stage's 16 key fragments the first waves fill KEYS each, of its eight
+  // pairs of value fragments the others one each.
+  static constexpr int KEYS = 16 / (WAVES - 8), KEY_WAVES = WAVES - 8;
+  static_assert(G * 2 * KS == 16 && G * ND / 2 == 8 && KS % KEYS == 0, "a stage");
+};
+
+// fill_table (kv4_tile.hpp) by THREADS threads, any multiple of 256.
+template <int THREADS>
+__device__ inline void fill_table_any(const Args& a, int hc, char* lds, int tid) {
+  constexpr int UNITS = kTable / 16, TURNS = (UNITS + THREADS - 1) / THREADS;
+  const uint16_t* lv = ((tid & 8) ? a.v_levels : a.k_levels) + hc * 16;
+  const uint32_t low = lv[tid / 16 % 16];
+  uint32_t high[TURNS];
+#pragma unroll
+  for (int r = 0; r < TURNS; ++r) high[r] = lv[min((r * THREADS + tid) / 256, 15)];
+#pragma unroll
+  for (int r = 0; r < TURNS; ++r) {
+    const uint32_t w = high[r] << 16 | low;
+    if (r * THREADS + tid < UNITS)
+      *reinterpret_cast<u32x4*>(lds + (r * THREADS + tid) * 16) = u32x4{w, w, w, w};
+  }
+}
+
+template <int DT, int D, int MODE>
+__global__ void __launch_bounds__(Wide<D>::THREADS, Wide<D>::PER_SIMD)
 kv4_masked_wide_kernel(const MArgs margs) {
-  constexpr int WAVES = 8, COLS = 16 * NT * WAVES, THREADS = WAVES * 64;
-  constexpr int KS = D / 32, ND = D / 16, HALVES = TT / 16, GROUPS = TT / 32;
-  constexpr int KPW = HALVES * KS / WAVES;  // key fragments a wave fills
-  constexpr int VW = GROUPS * ND / 2;       // waves that fill two value fragments
-  static_assert(KPW >= 1 && KS % KPW == 0 && VW <= WAVES, "a wave fills within one half");
-  constexpr int KBYTES = TT * D * 2, BUF = 2 * KBYTES;
-  typedef int Groups __attribute__((ext_vector_type(HALVES)));
+  typedef Wide<D> L;
+  constexpr int G = L::G, COLS = L::COLS, THREADS = L::THREADS, KS = L::KS, ND = L::ND, NT = 1;
   const Args& args = margs.a;
   extern __shared__ __align__(16) char lds[];
-  int* s_pre = reinterpret_cast<int*>(lds + kTable + 2 * BUF);
+  int* s_pre = reinterpret_cast<int*>(lds + L::kShares);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kj = wave * KPW / KS, kc0 = wave * KPW % KS;  // its half, first step
-  const int vg = wave % VW / (ND / 2), vu = wave % (ND / 2);  // its group, fragment pair
   int table = -1;  // head whose table is in LDS
-  typedef MWalk<COLS, THREADS, TT> W;
+  typedef MWalk<COLS, THREADS, 32 * G> W;
   W k = args.whole ? W() : W(arguments(), s_pre);
   if (!(args.whole ? k.whole(arguments()) : k.next(arguments()))) return;
   for (;;) {
@@ -658,8 +788,8 @@ kv4_masked_wide_kernel(const MArgs margs) {
     const uint32_t loff = (uint32_t)(lane & 31) * 4;
     const MTile& t = k.t;
     const int ncols = t.nq * a.G;
-    const int col0 = t.col0 + wave * 16 * NT;  // the wave's columns, in the request
-    const int t0 = k.from, t1 = k.to, tiles = (max(t1 - t0, 0) + TT - 1) / TT;
+    const int col0 = t.col0 + wave * 16;  // the wave's columns, in the request
+    const int t0 = k.from, t1 = k.to, groups = (max(t1 - t0, 0) + 31) / 32;
 
     // The arguments that every tile needs, in scalar registers (left to itself
     // the compiler reads them again at each use, and waits).
@@ -674,68 +804,88 @@ kv4_masked_wide_kernel(const MArgs margs) {
     asm volatile("" : "+s"(k_codes), "+s"(v_codes), "+s"(k_scales), "+s"(v_scales));
     asm volatile("" : "+s"(bs), "+s"(bs_m), "+s"(num_blocks), "+s"(bs_sh), "+s"(heads),
                  "+s"(zscale), "+s"(cap2));
-    const Const32 blocks = (Const32)(a.tables + (int64_t)t.req * a.table_stride);
-    // 16-slot groups of a tile's halves over all heads, -1 where there is none.
-    auto find_groups = [&](int tile, Groups& base) {
-#pragma unroll
-      for (int j = 0; j < HALVES; ++j) {
-        const uint32_t tok = t0 + tile * TT + 16 * j;
-        const uint32_t at = __umulhi(tok, bs_m) >> bs_sh;  // (block sizes are 16 at least)
-        const uint32_t b = (int)tok < t1 ? (uint32_t)blocks[at] : 0xffffffffu;
-        base[j] = b < num_blocks ? (int)((b * heads + k.head) * (bs / 16) + (tok - at * bs) / 16)
-                                 : -1;
-      }
+    const int32_t* blocks = a.tables + (int64_t)t.req * a.table_stride;
+    // 16-slot groups of the item's halves (of 16 tokens) over all heads, -1 where
+    // there is none.  A lane has one of 64 halves, so that none is loaded in the
+    // loop's way (scalar loads would be waited for with every LDS read).
+    auto load_halves = [&](int part) {
+      const int tok = t0 + (part * 64 + lane) * 16;
+      const uint32_t at = __umulhi((uint32_t)tok, bs_m) >> bs_sh;  // (block sizes are 16 at least)
+      const uint32_t b = tok < t1 ? (uint32_t)blocks[at] : 0xffffffffu;
+      return b < num_blocks
+                 ? (int)((b * heads + k.head) * (bs / 16) + ((uint32_t)tok - at * bs) / 16)
+                 : -1;
     };
-    uint32_t kcode[KPW], vcode[8];
-    uint2 ks[HALVES], vs[HALVES];
-    auto pick = [](const Groups& base, int j) {
-      int v = base[0];
-#pragma unroll
-      for (int i = 1; i < HALVES; ++i) v = j == i ? base[i] : v;
-      return (int64_t)max(v, 0);  // a missing half reads slot 0
+    int part = 0, halves = load_halves(0), more_halves = load_halves(1);
+    // Half x, of this part or the next.  (Both are read, and by all lanes' leave: a
+    // choice between the registers would be made for the active lanes only.)
+    auto half = [&](int x) {
+      const int a = __builtin_amdgcn_readlane(halves, x & 63);
+      const int b = __builtin_amdgcn_readlane(more_halves, x & 63);
+      return x >> 6 == part ? a : b;
     };
-    auto load_tile = [&](const Groups& base) {
-      const Global kp = k_codes + pick(base, kj) * (16 * D / 2);
+    // What the wave fills: key fragments (half kj of the stage, from step kc0 on),
+    // or a pair of value fragments.
+    const bool keys = wave < L::KEY_WAVES;
+    const int kj = wave * L::KEYS / KS, kc0 = wave * L::KEYS % KS;
+    const int pair = wave - L::KEY_WAVES, vg = pair / (ND / 2), vu = pair % (ND / 2);
+    uint32_t code[8];
+    auto load_codes = [&](int i0) {  // of the stage from group i0 on
+      if (keys) {
+        const Global kp = k_codes + (int64_t)max(half(2 * i0 + kj), 0) * (16 * D / 2);
 #pragma unroll
-      for (int e = 0; e < KPW; ++e)
-        kcode[e] = at<uint32_t>(kp, n * (D / 2) + g * (D / 8) + (kc0 + e) * 4);
-      // (waves without value fragments load those of others)
-      {
+        for (int e = 0; e < L::KEYS; ++e)
+          code[e] = at<uint32_t>(kp, n * (D / 2) + g * (D / 8) + (kc0 + e) * 4);
+      } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const Global vp = v_codes + pick(base, 2 * vg + j) * (16 * D / 2);
+          const Global vp = v_codes + (int64_t)max(half(2 * (i0 + vg) + j), 0) * (16 * D / 2);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            vcode[4 * j + i] = at<uint8_t>(vp, (4 * g + i) * (D / 2) + 16 * vu + n);
+            code[4 * j + i] = at<uint8_t>(vp, (4 * g + i) * (D / 2) + 16 * vu + n);
         }
       }
     };
-    auto load_scales = [&](const Groups& base, int j) {
-      const int64_t row = (int64_t)max(base[j], 0) * 32;  // bytes
-      ks[j] = at<uint2>(k_scales + row, 8 * g);
-      vs[j] = at<uint2>(v_scales + row, 8 * g);
-    };
-    auto fill_buffer = [&](int tile) {
-      char* buf = lds + kTable + (tile & 1) * BUF + lane * 16;
+    auto fill = [&](int buffer) {
+      char* buf = lds + L::kBuffers + buffer * L::BUF + lane * 16;
+      if (keys) {
 #pragma unroll
-      for (int e = 0; e < KPW; ++e) {
-        u32x4 f;
+        for (int e = 0; e < L::KEYS; ++e) {
+          u32x4 f;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) f[b] = lookup<0>(kcode[e], b, loff);
-        *reinterpret_cast<u32x4*>(buf + (kj * KS + kc0 + e) * 1024) = f;
-      }
-      if (wave < VW) {
+          for (int b = 0; b < 4; ++b) f[b] = lookup<0>(code[e], b, loff);
+          *reinterpret_cast<u32x4*>(buf + (kj * KS + kc0 + e) * 1024) = f;
+        }
+      } else {
         u32x4 even, odd;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t b0 = vcode[2 * c], b1 = vcode[2 * c + 1];
-          even[c] = lookup<128>((b0 & 15u) | (b1 << 4 & 0xf0u), 0, loff);
-          odd[c] = lookup<128>(b0 >> 4 | (b1 & 0xf0u), 0, loff);
+        for (int c = 0; c < 4; ++c) {  // (a look-up takes its byte alone)
+          even[c] = lookup<128>((code[2 * c] & 15u) | code[2 * c + 1] << 4, 0, loff);
+          odd[c] = lookup<128>(code[2 * c] >> 4 | (code[2 * c + 1] & 0xf0u), 0, loff);
         }
-        char* vb = buf + KBYTES + (vg * ND + 2 * vu) * 1024;
+        char* vb = buf + G * L::GROUP + 2 * pair * 1024;
         *reinterpret_cast<u32x4*>(vb) = even;
         *reinterpret_cast<u32x4*>(vb + 1024) = odd;
       }
+    };
+    // The first G waves also have a group's scales, a lane one of a key (the first
+    // 32) or of a value.
+    uint32_t scale = 0;
+    auto load_scale = [&](int i0) {
+      if (wave >= G) return;
+      const int base0 = half(2 * (i0 + wave)), base1 = half(2 * (i0 + wave) + 1);
+      const int base = (lane & 16) ? base1 : base0;
+      const Global from = lane < 32 ? k_scales : v_scales;
+      scale = *(const uint16_t __attribute__((address_space(1)))*)(
+          from + (int64_t)max(base, 0) * 32 + 2 * n);
+    };
+    auto fill_scale = [&](int buffer) {
+      if (wave >= G) return;
+      float* to = reinterpret_cast<float*>(lds + L::kScales + (buffer * G + wave) * L::SCALES);
+      float v = from16<DT>(scale);
+      if (MODE != kMask && lane < 32) v *= zscale;
+      to[lane] = v;
+      if (DT == FKC_F16 && lane >= 32) to[32 + lane] = exponent_of(v);
     };
     auto column = [&](const Args& a, int y, int& row, int& head, int& i) {
       const int col = col0 + 16 * y + n;
@@ -744,13 +894,9 @@ kv4_masked_wide_kernel(const MArgs margs) {
       head = k.head * a.G + (min(col, ncols - 1) - i * a.G);
     };
 
-    Groups base, nbase;  // of this tile and the next
-    find_groups(0, base);
-    find_groups(1, nbase);
-    if (tiles > 0) {
-      load_tile(base);
-#pragma unroll
-      for (int j = 0; j < HALVES; ++j) load_scales(base, j);
+    if (groups > 0) {
+      load_codes(0);
+      load_scale(0);
     }
     Columns<MODE, NT> cols;
     cols.clear();
@@ -768,59 +914,84 @@ kv4_masked_wide_kernel(const MArgs margs) {
                    a.qsign;
     }
     cols.reduce();
+    // The wave's groups g0 .. g1 - 1 of the item's.
+    int g0 = INT32_MAX, g1 = INT32_MAX;
+    if (max(cols.lo, t0) < min(cols.hi, t1)) {
+      g0 = (max(cols.lo, t0) - t0) / 32;
+      g1 = (min(cols.hi, t1) - t0 + 31) / 32;
+    }
     if (table != k.head) {  // (every look-up of the last item was before its last barrier)
       table = k.head;
-      fill_table<THREADS>(a, k.head, lds, tid);
+      fill_table_any<THREADS>(a, k.head, lds, tid);
       lds_barrier();
     }
-    if (tiles > 0) fill_buffer(0);
-    if (tiles > 0) load_tile(nbase);
-    lds_barrier();
 
     MState<DT, D, NT, MODE> st;
     st.clear();
-    for (int tile = 0; tile < tiles; ++tile) {
-      Groups after;
-      if (tile + 1 < tiles) fill_buffer(tile + 1);
-      find_groups(tile + 2, after);
-      // Past the last tile slot 0's codes, unused: a load that may or may not be
-      // on its way would have to be waited for with every older one.
-      load_tile(after);
-      const char* buf = lds + kTable + (tile & 1) * BUF + lane * 16;
-      auto group = [&](auto H) {
-        constexpr int h = H.value;
-        const int tok = t0 + tile * TT + 32 * h;
-        const uint2 kw[2] = {ks[2 * h], ks[2 * h + 1]}, vw[2] = {vs[2 * h], vs[2 * h + 1]};
-        load_scales(nbase, 2 * h);
-        load_scales(nbase, 2 * h + 1);
-        if (tok >= cols.hi || tok + 32 <= cols.lo) return;  // none of the wave's columns sees them
-        f32x4 s[NT][2];
-#pragma unroll
-        for (int c = 0; c < KS; ++c)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const u32x4 kf =
-                *reinterpret_cast<const u32x4*>(buf + ((2 * h + j) * KS + c) * 1024);
-#pragma unroll
-            for (int y = 0; y < NT; ++y)
-              s[y][j] = mfma<DT>(kf, qf[y][c], c ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
-          }
-        u32x4 pf[NT];
-        st.weights(s, kw, vw,
-                   tok + 32 > cols.to || tok < cols.from || (base[2 * h] | base[2 * h + 1]) < 0,
-                   base[2 * h], base[2 * h + 1], tok + 4 * g, cols, zscale, cap2, pf);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const u32x4 vf = *reinterpret_cast<const u32x4*>(buf + KBYTES + (h * ND + d) * 1024);
-#pragma unroll
-          for (int y = 0; y < NT; ++y) st.o[y][d] = mfma<DT>(vf, pf[y], st.o[y][d]);
-        }
-      };
-      group(std::integral_constant<int, 0>{});
-      if constexpr (GROUPS > 1) group(std::integral_constant<int, 1>{});
-      base = nbase;
-      nbase = after;
+    if (groups > 0) {
+      fill(0);
+      fill_scale(0);
+      load_codes(G);
+      load_scale(G);
       lds_barrier();
+      for (int i0 = 0; i0 < groups; i0 += G) {
+        const int buffer = i0 / G & 1;
+        fill(buffer ^ 1);
+        fill_scale(buffer ^ 1);
+        load_codes(i0 + 2 * G);
+        load_scale(i0 + 2 * G);
+        const char* buf = lds + L::kBuffers + buffer * L::BUF + lane * 16;
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          const int i = i0 + h;
+          if (i < g0 || i >= g1) continue;  // none of the wave's columns sees them
+          const int tok = t0 + i * 32;
+          const f32x4* sc = reinterpret_cast<const f32x4*>(
+              lds + L::kScales + (buffer * G + h) * L::SCALES) + g;
+          f32x4 z[NT][2];
+#pragma unroll
+          for (int c = 0; c < KS; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const u32x4 kf =
+                  *reinterpret_cast<const u32x4*>(buf + ((2 * h + j) * KS + c) * 1024);
+#pragma unroll
+              for (int y = 0; y < NT; ++y)
+                z[y][j] = mfma<DT>(kf, qf[y][c], c ? z[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
+            }
+          const int base0 = half(2 * i), base1 = half(2 * i + 1);
+          const bool masked = tok + 32 > cols.to || tok < cols.from || (base0 | base1) < 0;
+          st.ks[0] = sc[0];
+          st.ks[1] = sc[4];
+          st.score(z, tok + 4 * g, tok, cols, cap2);
+          if (masked) st.mask(z, base0, base1, tok + 4 * g, cols);
+          if constexpr (DT == FKC_F16) {
+            st.ve[0] = sc[16];
+            st.ve[1] = sc[20];
+          }
+          st.settle(z, zscale, cap2);
+          st.vs[0] = sc[8];
+          st.vs[1] = sc[12];
+          bool odd = false;
+          if (masked) odd = st.mask_values(base0, base1, tok + 4 * g, cols);
+          u32x4 pf[NT];
+          st.weigh(z, zscale, cap2, pf);
+          if (odd) st.weigh_odd(z, zscale, cap2, pf);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) {
+            const u32x4 vf =
+                *reinterpret_cast<const u32x4*>(buf + G * L::GROUP + (h * ND + d) * 1024);
+#pragma unroll
+            for (int y = 0; y < NT; ++y) st.o[y][d] = mfma<DT>(vf, pf[y], st.o[y][d]);
+          }
+        }
+        if ((2 * (i0 + G)) >> 6 != part) {
+          ++part;
+          halves = more_halves;
+          more_halves = load_halves(part + 1);
+        }
+        lds_barrier();
+      }
     }
 
     st.join_lanes();
@@ -844,7 +1015,7 @@ kv4_masked_wide_kernel(const MArgs margs) {
           }
           if (g == 0 && a.lse != nullptr) a.lse[at] = log_sum(st.base2(y, zscale), st.l[y]);
         } else {
-          const int64_t at = k.slot() * COLS + wave * 16 * NT + 16 * y + n;
+          const int64_t at = k.slot() * COLS + wave * 16 + 16 * y + n;
 #pragma unroll
           for (int u = 0; u < ND / 2; ++u)
 #pragma unroll
@@ -878,9 +1049,8 @@ struct Plan {
   size_t part_rows() const { return (size_t)wgs * 2 * cols(); }
 };
 
-constexpr int kWide = 8;  // waves of the wide form
-constexpr int wide_tiles(int D) { return D == 256 ? 1 : 2; }
-constexpr int wide_tokens(int D) { return D == 256 ? 32 : 64; }
+constexpr int wide_waves(int D) { return D == 256 ? 12 : 16; }
+constexpr int wide_tokens(int D) { return 32 * (256 / D); }
 constexpr int waves_of(int D) { return D == 256 ? 4 : 8; }
 
 // reach: tokens that one query sees at most (max_seq, or the window).
@@ -890,8 +1060,8 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
   const int64_t G = H / c.heads;
   const int64_t avg = R > 0 ? T * G / R : 0;
   p.wide = avg > (c.D == 256 ? 224 : 448);
-  p.nt = p.wide ? wide_tiles((int)c.D) : c.D < 256 && avg > 64 ? 2 : 1;
-  p.waves = p.wide ? kWide : p.nt == 2 ? 4 : waves_of((int)c.D);
+  p.nt = p.wide ? 1 : c.D < 256 && avg > 64 ? 2 : 1;
+  p.waves = p.wide ? wide_waves((int)c.D) : p.nt == 2 ? 4 : waves_of((int)c.D);
   const int64_t cols = p.cols();
   p.tiles_per_req = (int)((G + cols - 1) / cols);
   p.ntiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
@@ -938,10 +1108,10 @@ int launch_split(const MArgs& m, const Plan& p, hipStream_t s) {
 template <int DT, int D, int MODE>
 int launch_wide(const MArgs& m, const Plan& p, hipStream_t s) {
   static std::atomic<uint64_t> set{0};
-  constexpr int NT = wide_tiles(D), TT = wide_tokens(D), COLS = 16 * NT * kWide;
-  return launch<DT, D, COLS, TT, kWide * 64>(
-      &kv4_masked_wide_kernel<DT, D, NT, TT, MODE>, set,
-      kTable + 2 * (TT * D * 4) + MWalk<COLS, kWide * 64, 1>::kInts * 4, m, p, s);
+  typedef Wide<D> L;
+  return launch<DT, D, L::COLS, 32 * L::G, L::THREADS>(
+      &kv4_masked_wide_kernel<DT, D, MODE>, set,
+      L::kShares + MWalk<L::COLS, L::THREADS, 1>::kInts * 4, m, p, s);
 }
 
 template <int DT, int D, int MODE>
