@@ -90,9 +90,9 @@ __device__ inline void find_range(const MArgs& m, MTile& t) {
   t.lo &= ~15;  // codes are loaded by groups of 16 slots
 }
 
-// Weighs the tiles: granules of GR tokens and kItem more for what a tile costs by
+// Weighs the tiles: granules of GR tokens and ITEM more for what a tile costs by
 // itself, kIdle where it sees nothing.  One wave per tile.
-template <int COLS, int GR>
+template <int COLS, int GR, int ITEM>
 __global__ void __launch_bounds__(256)
 kv4_tiles_kernel(const MArgs m) {
   const int tile = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -101,7 +101,7 @@ kv4_tiles_kernel(const MArgs m) {
   int w = 0;
   if (find_tile<COLS>(m.a, tile, t)) {
     find_range<COLS>(m, t);
-    w = t.hi > t.lo ? kItem + (t.hi - t.lo + GR - 1) / GR : kIdle;
+    w = t.hi > t.lo ? ITEM + (t.hi - t.lo + GR - 1) / GR : kIdle;
   }
   if ((threadIdx.x & 63) != 0) return;
   m.weights[tile] = w;
@@ -112,7 +112,7 @@ kv4_tiles_kernel(const MArgs m) {
 // The tiles' weights over all heads are cut into equal shares, one per
 // workgroup, wherever the cuts fall; an item (a tile under one head) that is cut
 // is joined afterwards.
-template <int COLS, int THREADS, int GR>
+template <int COLS, int THREADS, int GR, int ITEM>
 struct MWalk {
   int64_t u = 0, u_end = 0, share = 1;
   int tile = 0, at = 0, hc = 0;  // where the share goes on
@@ -188,7 +188,7 @@ struct MWalk {
       const int end = (int)min((int64_t)n, at + (u_end - u));
       u += end - at;
       auto token = [&](int place) {
-        return place == n ? t.hi : min(t.lo + max(place - kItem, 0) * GR, t.hi);
+        return place == n ? t.hi : min(t.lo + max(place - ITEM, 0) * GR, t.hi);
       };
       from = token(at);
       to = token(end);
@@ -279,10 +279,10 @@ struct Columns {
   }
 };
 
-// fp16: what a value scale adds to the maximum: its exponent, rounded up; zero
-// counts as 2^-60.
+// fp16: what a value scale adds to the maximum, its logarithm; zero counts as 2^-60,
+// infinity as 2^129.
 __device__ inline float exponent_of(float scale) {
-  return fmaxf((float)(int)(__float_as_uint(fabsf(scale)) >> 23) - 126.f, -60.f);
+  return __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(fabsf(scale)), -60.f, 129.f);
 }
 
 // As State (kv4_tile.hpp), with scores as above, in the steps that a kernel may
@@ -366,35 +366,45 @@ struct MState : State<DT, D, NT> {
       }
     }
   }
-  // For tiles that some column does not see all of.
-  __device__ inline void mask(f32x4 (&z)[NT][2], int base0, int base1, int tok,
+  // For tiles that some column does not see all of; there: a bit for each half that
+  // has a block.
+  __device__ inline void mask(f32x4 (&z)[NT][2], int there, int tok,
                               const Columns<MODE, NT>& c) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int y = 0; y < NT; ++y) {
+      // (one comparison for both ends: what is before the first wraps)
+      const uint32_t at = (uint32_t)(tok - c.first[y]);
+      const uint32_t len = (uint32_t)max(c.last[y] - c.first[y], 0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int x = tok + 16 * j + i;
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int y = 0; y < NT; ++y) {
+        for (int i = 0; i < 4; ++i) {
           float v = z[y][j][i];
-          if ((j ? base1 : base0) < 0 || x < c.first[y] || x >= c.last[y]) v = kHidden;
+          if (at + (16 * j + i) >= len) v = kHidden;
           rare(v);
           z[y][j][i] = v;
         }
-      }
+    }
+    if (there != 3) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (!(there >> j & 1))
+#pragma unroll
+          for (int y = 0; y < NT; ++y) z[y][j] = f32x4{kHidden, kHidden, kHidden, kHidden};
+    }
   }
   // And their values' scales: 0 for what no column sees, which may be anything.
   // Returns whether one is not finite all the same, so that its product with a
   // hidden column's weight, 0, would not be 0.
-  __device__ inline bool mask_values(int base0, int base1, int tok, const Columns<MODE, NT>& c) {
+  __device__ inline bool mask_values(int there, int tok, const Columns<MODE, NT>& c) {
     bool odd = false;
+    const uint32_t at = (uint32_t)(tok - c.lo), len = (uint32_t)max(c.hi - c.lo, 0);
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int x = tok + 16 * j + i;
         float s = vs[j][i];
-        if ((j ? base1 : base0) < 0 || x >= c.hi || x < c.lo) s = 0.f;
+        if (at + (16 * j + i) >= len || !(there >> j & 1)) s = 0.f;
         rare(s);
         vs[j][i] = s;
         odd |= !(fabsf(s) < INFINITY);
@@ -457,18 +467,18 @@ struct MState : State<DT, D, NT> {
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
       const float base = base_of(y, zscale, cap2);
-      float w[2][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j) {
+        float w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float p = __builtin_amdgcn_exp2f(exponent(z[y][j][i], base, zscale, cap2));
           l[y] += p;
-          w[j][i] = p * vs[j][i];
+          w[i] = p * vs[j][i];
         }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        pf[y][e] = pack2<DT>(w[e >> 1][2 * (e & 1)], w[e >> 1][2 * (e & 1) + 1]);
+        pf[y][2 * j] = pack2<DT>(w[0], w[1]);
+        pf[y][2 * j + 1] = pack2<DT>(w[2], w[3]);
+      }
     }
   }
   // After mask's true: the weights once more, 0 for what is hidden.
@@ -477,16 +487,19 @@ struct MState : State<DT, D, NT> {
 #pragma unroll
     for (int y = 0; y < NT; ++y) {
       const float base = base_of(y, zscale, cap2);
-      float w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = z[y][e >> 2][e & 3];
-        w[e] = __builtin_amdgcn_exp2f(exponent(v, base, zscale, cap2)) * vs[e >> 2][e & 3];
-        w[e] = v == kHidden ? 0.f : w[e];
-        rare(w[e]);
+      for (int j = 0; j < 2; ++j) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = z[y][j][i];
+          w[i] = __builtin_amdgcn_exp2f(exponent(v, base, zscale, cap2)) * vs[j][i];
+          w[i] = v == kHidden ? 0.f : w[i];
+          rare(w[i]);
+        }
+        pf[y][2 * j] = pack2<DT>(w[0], w[1]);
+        pf[y][2 * j + 1] = pack2<DT>(w[2], w[3]);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf[y][e] = pack2<DT>(w[2 * e], w[2 * e + 1]);
     }
   }
 };
@@ -505,7 +518,7 @@ kv4_masked_split_kernel(const MArgs margs) {
   int* s_pre = reinterpret_cast<int*>(lds + kTable + kJoin);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  typedef MWalk<COLS, THREADS, UNIT> W;
+  typedef MWalk<COLS, THREADS, UNIT, kItem> W;
   W k = args.whole ? W() : W(arguments(), s_pre);
   if (!(args.whole ? k.whole(arguments()) : k.next(arguments()))) return;
   for (;;) {
@@ -543,6 +556,13 @@ kv4_masked_split_kernel(const MArgs margs) {
       }
     };
     int blk[2], base[2], nbase[2];
+    // What is loaded where there is no block, or no tile any more: what the wave
+    // loaded last, not slot 0, the same for every workgroup.
+    int from[2] = {0, 0};
+    auto loads = [&](const int (&b)[2]) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) from[j] = b[j] >= 0 ? b[j] : from[j];
+    };
     load_blocks(wave, blk);
 
     // Query and head of a column of the tile's; row -1 past the last.
@@ -574,10 +594,11 @@ kv4_masked_split_kernel(const MArgs margs) {
     const Lane<D> lanes(n, g);
     Codes<D> cur;
     groups(wave, blk, base);
+    loads(base);
     if (wave < ntile) {
-      load_keys<D>(a, base, lanes, cur);
-      load_scales<D>(a, base, lanes, cur);
-      load_values<D>(a, base, lanes, cur);
+      load_keys<D>(a, from, lanes, cur);
+      load_scales<D>(a, from, lanes, cur);
+      load_values<D>(a, from, lanes, cur);
     }
     load_blocks(wave + WAVES, blk);
     fill_table<THREADS>(a, k.head, lds, tid);
@@ -592,6 +613,7 @@ kv4_masked_split_kernel(const MArgs margs) {
     // latency.
     for (int it = wave; it < ntile; it += WAVES) {
       groups(it + WAVES, blk, nbase);
+      loads(nbase);
       load_blocks(it + 2 * WAVES, blk);
 
       f32x4 s[NT][2];
@@ -606,9 +628,9 @@ kv4_masked_split_kernel(const MArgs margs) {
           for (int y = 0; y < NT; ++y)
             s[y][j] = mfma<DT>(kf, qf[y][c], c ? s[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
         }
-      load_keys<D>(a, nbase, lanes, cur);
+      load_keys<D>(a, from, lanes, cur);
       const uint2 kw[2] = {cur.ks[0], cur.ks[1]}, vw[2] = {cur.vs[0], cur.vs[1]};
-      load_scales<D>(a, nbase, lanes, cur);
+      load_scales<D>(a, from, lanes, cur);
       u32x4 pf[NT];
       const int tok = t0 + it * 32;
       const bool masked = tok + 32 > cols.to || tok < cols.from || (base[0] | base[1]) < 0;
@@ -616,8 +638,9 @@ kv4_masked_split_kernel(const MArgs margs) {
       st.score(s, tok + 4 * g, tok, cols, cap2);
       bool odd = false;
       if (masked) {
-        st.mask(s, base[0], base[1], tok + 4 * g, cols);
-        odd = st.mask_values(base[0], base[1], tok + 4 * g, cols);
+        const int there = (base[0] >= 0) + 2 * (base[1] >= 0);
+        st.mask(s, there, tok + 4 * g, cols);
+        odd = st.mask_values(there, tok + 4 * g, cols);
       }
       st.settle(s, zscale, cap2);
       st.weigh(s, zscale, cap2, pf);
@@ -645,7 +668,7 @@ kv4_masked_split_kernel(const MArgs margs) {
           }
         }
       }
-      load_values<D>(a, nbase, lanes, cur);
+      load_values<D>(a, from, lanes, cur);
       base[0] = nbase[0];
       base[1] = nbase[1];
     }
@@ -724,7 +747,7 @@ kv4_masked_split_kernel(const MArgs margs) {
 // all: each wave turns its share of the codes into the fragments of both
 // products, laid out so that a fragment is read by 64 lanes in a row (16 bytes
 // each, no bank conflict), in one of two buffers; while a stage of G groups of
-// 32 tokens is computed on, the next one is filled into the other.
+// two halves of 16 tokens is computed on, the next one is filled into the other.
 //
 // Feature row n of fragment d of the second product is feature 32 (d / 2) + 2 n +
 // d % 2: the two codes of one byte go to two fragments, and 16 lanes read 16
@@ -735,17 +758,19 @@ struct Wide {
   static constexpr int COLS = 16 * WAVES, THREADS = WAVES * 64;
   static constexpr int KS = D / 32, ND = D / 16;
   static constexpr int G = 256 / D;            // groups of a stage
-  static constexpr int GROUP = 32 * D * 2;     // bytes of a group's keys or values
-  static constexpr int BUF = 2 * G * GROUP;    // keys, then values
-  // Scales of a stage in fp32: keys', values', and (fp16) exponent_of these, per
-  // group.
+  // Groups that an item costs by itself.
+  static constexpr int ITEM = D == 64 ? 10 : 6;
+  static constexpr int RUN = G * 32 * D * 2;  // bytes of a stage's keys or values
+  static constexpr int BUF = 2 * RUN;             // keys, then values
+  // Scales of a stage in fp32, per group: keys', values', and (fp16)
+  // exponent_of these.
   static constexpr int SCALES = 3 * 32 * 4;
   static constexpr int kBuffers = kTable, kScales = kBuffers + 2 * BUF,
                        kShares = kScales + 2 * G * SCALES;
-  // Of a stage's 16 key fragments the first waves fill KEYS each, of its eight
-  // pairs of value fragments the others one each.
-  static constexpr int KEYS = 16 / (WAVES - 8), KEY_WAVES = WAVES - 8;
-  static_assert(G * 2 * KS == 16 && G * ND / 2 == 8 && KS % KEYS == 0, "a stage");
+  // Eight waves fill two of a stage's 16 key fragments each, eight a pair of its 16
+  // value fragments; where there are no sixteen, the same.
+  static constexpr int VALUES_FROM = WAVES == 16 ? 8 : 0;
+  static_assert(G * 2 * KS == 16 && G * ND == 16, "a stage");
 };
 
 // fill_table (kv4_tile.hpp) by THREADS threads, any multiple of 256.
@@ -769,14 +794,15 @@ template <int DT, int D, int MODE>
 __global__ void __launch_bounds__(Wide<D>::THREADS, Wide<D>::PER_SIMD)
 kv4_masked_wide_kernel(const MArgs margs) {
   typedef Wide<D> L;
-  constexpr int G = L::G, COLS = L::COLS, THREADS = L::THREADS, KS = L::KS, ND = L::ND, NT = 1;
+  constexpr int G = L::G, COLS = L::COLS, THREADS = L::THREADS;
+  constexpr int KS = L::KS, ND = L::ND, NT = 1;
   const Args& args = margs.a;
   extern __shared__ __align__(16) char lds[];
   int* s_pre = reinterpret_cast<int*>(lds + L::kShares);
 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int table = -1;  // head whose table is in LDS
-  typedef MWalk<COLS, THREADS, 32 * G> W;
+  typedef MWalk<COLS, THREADS, 32, L::ITEM> W;
   W k = args.whole ? W() : W(arguments(), s_pre);
   if (!(args.whole ? k.whole(arguments()) : k.next(arguments()))) return;
   for (;;) {
@@ -817,75 +843,77 @@ kv4_masked_wide_kernel(const MArgs margs) {
                  : -1;
     };
     int part = 0, halves = load_halves(0), more_halves = load_halves(1);
-    // Half x, of this part or the next.  (Both are read, and by all lanes' leave: a
-    // choice between the registers would be made for the active lanes only.)
+    // Half x, of this part or the next; past the item's end its last one, which is
+    // at hand.  (Called where all lanes go the same way only: the registers are read
+    // whatever lanes are active.)
     auto half = [&](int x) {
-      const int a = __builtin_amdgcn_readlane(halves, x & 63);
-      const int b = __builtin_amdgcn_readlane(more_halves, x & 63);
-      return x >> 6 == part ? a : b;
+      x = min(x, 2 * groups - 1);
+      if (x >> 6 != part) return __builtin_amdgcn_readlane(more_halves, x & 63);
+      return __builtin_amdgcn_readlane(halves, x & 63);
     };
-    // What the wave fills: key fragments (half kj of the stage, from step kc0 on),
-    // or a pair of value fragments.
-    const bool keys = wave < L::KEY_WAVES;
-    const int kj = wave * L::KEYS / KS, kc0 = wave * L::KEYS % KS;
-    const int pair = wave - L::KEY_WAVES, vg = pair / (ND / 2), vu = pair % (ND / 2);
-    uint32_t code[8];
-    auto load_codes = [&](int i0) {  // of the stage from group i0 on
+    // What the wave fills: key fragments of half kj of the stage, from step kc0 on; a
+    // pair of value fragments of group vg.  The first G waves also have a group's
+    // scales, a lane one of a key (the first 32) or of a value.
+    constexpr int VAT = L::VALUES_FROM ? 0 : 2;  // place of the values' codes
+    const bool keys = wave < 8, values = wave >= L::VALUES_FROM && wave < L::VALUES_FROM + 8;
+    const int kj = wave * 2 / KS, kc0 = wave * 2 % KS;
+    const int pair = wave - L::VALUES_FROM, vg = pair / (ND / 2), vu = pair % (ND / 2);
+    uint32_t code[8 + VAT], scale = 0;
+    auto load = [&](int x0) {  // of the stage from half x0 on
       if (keys) {
-        const Global kp = k_codes + (int64_t)max(half(2 * i0 + kj), 0) * (16 * D / 2);
+        const Global kp = k_codes + (int64_t)max(half(x0 + kj), 0) * (16 * D / 2);
 #pragma unroll
-        for (int e = 0; e < L::KEYS; ++e)
+        for (int e = 0; e < 2; ++e)
           code[e] = at<uint32_t>(kp, n * (D / 2) + g * (D / 8) + (kc0 + e) * 4);
-      } else {
+      }
+      if (values) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const Global vp = v_codes + (int64_t)max(half(2 * (i0 + vg) + j), 0) * (16 * D / 2);
+          const Global vp = v_codes + (int64_t)max(half(x0 + 2 * vg + j), 0) * (16 * D / 2);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            code[4 * j + i] = at<uint8_t>(vp, (4 * g + i) * (D / 2) + 16 * vu + n);
+            code[VAT + 4 * j + i] = at<uint8_t>(vp, (4 * g + i) * (D / 2) + 16 * vu + n);
         }
+      }
+      if (wave < G) {
+        const int base0 = half(x0 + 2 * wave), base1 = half(x0 + 2 * wave + 1);
+        const int base = max((lane & 16) ? base1 : base0, 0);
+        const Global from = lane < 32 ? k_scales : v_scales;
+        scale = *(const uint16_t __attribute__((address_space(1)))*)(from + (int64_t)base * 32 +
+                                                                     2 * n);
       }
     };
     auto fill = [&](int buffer) {
       char* buf = lds + L::kBuffers + buffer * L::BUF + lane * 16;
       if (keys) {
 #pragma unroll
-        for (int e = 0; e < L::KEYS; ++e) {
+        for (int e = 0; e < 2; ++e) {
           u32x4 f;
 #pragma unroll
           for (int b = 0; b < 4; ++b) f[b] = lookup<0>(code[e], b, loff);
           *reinterpret_cast<u32x4*>(buf + (kj * KS + kc0 + e) * 1024) = f;
         }
-      } else {
+      }
+      if (values) {
         u32x4 even, odd;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {  // (a look-up takes its byte alone)
-          even[c] = lookup<128>((code[2 * c] & 15u) | code[2 * c + 1] << 4, 0, loff);
-          odd[c] = lookup<128>(code[2 * c] >> 4 | (code[2 * c + 1] & 0xf0u), 0, loff);
+          const uint32_t b0 = code[VAT + 2 * c], b1 = code[VAT + 2 * c + 1];
+          even[c] = lookup<128>((b0 & 15u) | b1 << 4, 0, loff);
+          odd[c] = lookup<128>(b0 >> 4 | (b1 & 0xf0u), 0, loff);
         }
-        char* vb = buf + G * L::GROUP + 2 * pair * 1024;
+        char* vb = buf + L::RUN + 2 * pair * 1024;
         *reinterpret_cast<u32x4*>(vb) = even;
         *reinterpret_cast<u32x4*>(vb + 1024) = odd;
       }
-    };
-    // The first G waves also have a group's scales, a lane one of a key (the first
-    // 32) or of a value.
-    uint32_t scale = 0;
-    auto load_scale = [&](int i0) {
-      if (wave >= G) return;
-      const int base0 = half(2 * (i0 + wave)), base1 = half(2 * (i0 + wave) + 1);
-      const int base = (lane & 16) ? base1 : base0;
-      const Global from = lane < 32 ? k_scales : v_scales;
-      scale = *(const uint16_t __attribute__((address_space(1)))*)(
-          from + (int64_t)max(base, 0) * 32 + 2 * n);
-    };
-    auto fill_scale = [&](int buffer) {
-      if (wave >= G) return;
-      float* to = reinterpret_cast<float*>(lds + L::kScales + (buffer * G + wave) * L::SCALES);
-      float v = from16<DT>(scale);
-      if (MODE != kMask && lane < 32) v *= zscale;
-      to[lane] = v;
-      if (DT == FKC_F16 && lane >= 32) to[32 + lane] = exponent_of(v);
+      if (wave < G) {
+        float* to =
+            reinterpret_cast<float*>(lds + L::kScales + (buffer * G + wave) * L::SCALES);
+        float v = from16<DT>(scale);
+        if (MODE != kMask && lane < 32) v *= zscale;
+        to[lane] = v;
+        if (DT == FKC_F16 && lane >= 32) to[32 + lane] = exponent_of(v);
+      }
     };
     auto column = [&](const Args& a, int y, int& row, int& head, int& i) {
       const int col = col0 + 16 * y + n;
@@ -894,10 +922,7 @@ kv4_masked_wide_kernel(const MArgs margs) {
       head = k.head * a.G + (min(col, ncols - 1) - i * a.G);
     };
 
-    if (groups > 0) {
-      load_codes(0);
-      load_scale(0);
-    }
+    if (groups > 0) load(0);
     Columns<MODE, NT> cols;
     cols.clear();
     u32x4 qf[NT][KS];
@@ -930,16 +955,12 @@ kv4_masked_wide_kernel(const MArgs margs) {
     st.clear();
     if (groups > 0) {
       fill(0);
-      fill_scale(0);
-      load_codes(G);
-      load_scale(G);
+      load(2 * G);
       lds_barrier();
-      for (int i0 = 0; i0 < groups; i0 += G) {
-        const int buffer = i0 / G & 1;
+      uint64_t there = __ballot(halves >= 0);  // a bit for each half of the part
+      for (int i0 = 0, buffer = 0; i0 < groups; i0 += G, buffer ^= 1) {
         fill(buffer ^ 1);
-        fill_scale(buffer ^ 1);
-        load_codes(i0 + 2 * G);
-        load_scale(i0 + 2 * G);
+        load(2 * i0 + 4 * G);
         const char* buf = lds + L::kBuffers + buffer * L::BUF + lane * 16;
 #pragma unroll
         for (int h = 0; h < G; ++h) {
@@ -959,12 +980,12 @@ kv4_masked_wide_kernel(const MArgs margs) {
               for (int y = 0; y < NT; ++y)
                 z[y][j] = mfma<DT>(kf, qf[y][c], c ? z[y][j] : f32x4{0.f, 0.f, 0.f, 0.f});
             }
-          const int base0 = half(2 * i), base1 = half(2 * i + 1);
-          const bool masked = tok + 32 > cols.to || tok < cols.from || (base0 | base1) < 0;
+          const int both = (int)(there >> (2 * i & 63)) & 3;
+          const bool masked = tok + 32 > cols.to || tok < cols.from || both != 3;
           st.ks[0] = sc[0];
           st.ks[1] = sc[4];
           st.score(z, tok + 4 * g, tok, cols, cap2);
-          if (masked) st.mask(z, base0, base1, tok + 4 * g, cols);
+          if (masked) st.mask(z, both, tok + 4 * g, cols);
           if constexpr (DT == FKC_F16) {
             st.ve[0] = sc[16];
             st.ve[1] = sc[20];
@@ -973,14 +994,13 @@ kv4_masked_wide_kernel(const MArgs margs) {
           st.vs[0] = sc[8];
           st.vs[1] = sc[12];
           bool odd = false;
-          if (masked) odd = st.mask_values(base0, base1, tok + 4 * g, cols);
+          if (masked) odd = st.mask_values(both, tok + 4 * g, cols);
           u32x4 pf[NT];
           st.weigh(z, zscale, cap2, pf);
           if (odd) st.weigh_odd(z, zscale, cap2, pf);
 #pragma unroll
           for (int d = 0; d < ND; ++d) {
-            const u32x4 vf =
-                *reinterpret_cast<const u32x4*>(buf + G * L::GROUP + (h * ND + d) * 1024);
+            const u32x4 vf = *reinterpret_cast<const u32x4*>(buf + L::RUN + (h * ND + d) * 1024);
 #pragma unroll
             for (int y = 0; y < NT; ++y) st.o[y][d] = mfma<DT>(vf, pf[y], st.o[y][d]);
           }
@@ -988,6 +1008,7 @@ kv4_masked_wide_kernel(const MArgs margs) {
         if ((2 * (i0 + G)) >> 6 != part) {
           ++part;
           halves = more_halves;
+          there = __ballot(halves >= 0);
           more_halves = load_halves(part + 1);
         }
         lds_barrier();
@@ -1050,7 +1071,6 @@ struct Plan {
 };
 
 constexpr int wide_waves(int D) { return D == 256 ? 12 : 16; }
-constexpr int wide_tokens(int D) { return 32 * (256 / D); }
 constexpr int waves_of(int D) { return D == 256 ? 4 : 8; }
 
 // reach: tokens that one query sees at most (max_seq, or the window).
@@ -1071,7 +1091,7 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
   return p;
 }
 
-template <int DT, int D, int COLS, int GR, int THREADS, typename K>
+template <int DT, int D, int COLS, int GR, int ITEM, int THREADS, typename K>
 int launch(K kernel, std::atomic<uint64_t>& set, int bytes, const MArgs& m, const Plan& p,
            hipStream_t s) {
   // The attribute stays with the kernel: once per device is enough.
@@ -1085,7 +1105,7 @@ int launch(K kernel, std::atomic<uint64_t>& set, int bytes, const MArgs& m, cons
     set.fetch_or(bit, std::memory_order_relaxed);
   }
   if (!p.whole)
-    hipLaunchKernelGGL((kv4_tiles_kernel<COLS, GR>), dim3((uint32_t)((p.ntiles + 3) / 4)),
+    hipLaunchKernelGGL((kv4_tiles_kernel<COLS, GR, ITEM>), dim3((uint32_t)((p.ntiles + 3) / 4)),
                        dim3(256), 0, s, m);
   hipLaunchKernelGGL(kernel, dim3((uint32_t)p.wgs), dim3(THREADS), bytes, s, m);
   if (int rc = check_launch("kv4_attend")) return rc;
@@ -1100,18 +1120,18 @@ int launch(K kernel, std::atomic<uint64_t>& set, int bytes, const MArgs& m, cons
 template <int DT, int D, int NT, int WAVES, int MODE>
 int launch_split(const MArgs& m, const Plan& p, hipStream_t s) {
   static std::atomic<uint64_t> set{0};
-  return launch<DT, D, 16 * NT, WAVES * 32, WAVES * 64>(
+  return launch<DT, D, 16 * NT, WAVES * 32, kItem, WAVES * 64>(
       &kv4_masked_split_kernel<DT, D, NT, WAVES, MODE>, set,
-      kTable + kJoin + MWalk<16 * NT, WAVES * 64, 1>::kInts * 4, m, p, s);
+      kTable + kJoin + MWalk<16 * NT, WAVES * 64, 1, 0>::kInts * 4, m, p, s);
 }
 
 template <int DT, int D, int MODE>
 int launch_wide(const MArgs& m, const Plan& p, hipStream_t s) {
   static std::atomic<uint64_t> set{0};
   typedef Wide<D> L;
-  return launch<DT, D, L::COLS, 32 * L::G, L::THREADS>(
+  return launch<DT, D, L::COLS, 32, L::ITEM, L::THREADS>(
       &kv4_masked_wide_kernel<DT, D, MODE>, set,
-      L::kShares + MWalk<L::COLS, L::THREADS, 1>::kInts * 4, m, p, s);
+      L::kShares + MWalk<L::COLS, L::THREADS, 1, 0>::kInts * 4, m, p, s);
 }
 
 template <int DT, int D, int MODE>
@@ -1157,8 +1177,11 @@ int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const K
                            x.cu_q != nullptr);
   const int G = (int)(x.H / c.heads);
   // Weights of a head's items are summed in 32 bits.
-  const int64_t gr = p.wide ? wide_tokens((int)c.D) : 32 * p.waves;
-  if (p.wgs > INT32_MAX || p.ntiles > INT32_MAX / (x.max_seq / gr + 2 + kItem))
+  constexpr int kMostItem = 10;
+  static_assert(kItem <= kMostItem && Wide<64>::ITEM <= kMostItem &&
+                Wide<128>::ITEM <= kMostItem && Wide<256>::ITEM <= kMostItem, "");
+  const int64_t gr = p.wide ? 32 : 32 * p.waves;
+  if (p.wgs > INT32_MAX || p.ntiles > INT32_MAX / (x.max_seq / gr + 2 + kMostItem))
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   // (of scores times 0 the masked ones would be NaN)
   const double scale = std::max(std::fabs((double)x.sm_scale) * 1.4426950408889634, 1e-30);
