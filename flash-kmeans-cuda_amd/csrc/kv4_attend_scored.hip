@@ -90,8 +90,25 @@ __device__ inline void find_range(const MArgs& m, MTile& t) {
   t.lo &= ~15;  // codes are loaded by groups of 16 slots
 }
 
+// The range of a single token's tile, by one lane.
+template <int COLS>
+__device__ inline bool find_single(const MArgs& m, int tile, MTile& t) {
+  if (!find_tile<COLS>(m.a, tile, t)) return false;
+  t.prefix = m.prefix != nullptr ? m.prefix[t.req] : 0;
+  const Bounds b = bounds(m, t, 0);
+  t.lo = b.first < b.last ? b.first & ~15 : 0;
+  t.hi = b.first < b.last ? b.last : 0;
+  return true;
+}
+
+template <int GR, int ITEM>
+__device__ inline int weight_of(const MTile& t) {
+  return t.hi > t.lo ? ITEM + (t.hi - t.lo + GR - 1) / GR : kIdle;
+}
+
 // Weighs the tiles: granules of GR tokens and ITEM more for what a tile costs by
-// itself, kIdle where it sees nothing.  One wave per tile.
+// itself, kIdle where it sees nothing.  One wave per tile.  (Single tokens' tiles
+// are weighed by the workgroups that share them: one load or two each.)
 template <int COLS, int GR, int ITEM>
 __global__ void __launch_bounds__(256)
 kv4_tiles_kernel(const MArgs m) {
@@ -101,7 +118,7 @@ kv4_tiles_kernel(const MArgs m) {
   int w = 0;
   if (find_tile<COLS>(m.a, tile, t)) {
     find_range<COLS>(m, t);
-    w = t.hi > t.lo ? ITEM + (t.hi - t.lo + GR - 1) / GR : kIdle;
+    w = weight_of<GR, ITEM>(t);
   }
   if ((threadIdx.x & 63) != 0) return;
   m.weights[tile] = w;
@@ -123,13 +140,18 @@ struct MWalk {
   static constexpr int kInts = THREADS + (THREADS / 64 + 3) / 4 * 4;
 
   __device__ inline MWalk() {}
+  __device__ inline int weigh(const MArgs& m, int i) const {
+    if (m.a.cu_q != nullptr) return m.weights[i];
+    MTile x;
+    return find_single<COLS>(m, i, x) ? weight_of<GR, ITEM>(x) : 0;
+  }
   __device__ inline MWalk(const MArgs& m, int* s_pre) {
     int* s_wave = s_pre + THREADS;
     const int per = (m.ntiles + THREADS - 1) / THREADS;
     int sum = 0;
     for (int i = 0; i < per; ++i) {
       const int x = threadIdx.x * per + i;
-      if (x < m.ntiles) sum += m.weights[x];
+      if (x < m.ntiles) sum += weigh(m, x);
     }
     const int incl = wave_incl_scan(sum);
     if ((threadIdx.x & 63) == 63) s_wave[threadIdx.x >> 6] = incl;
@@ -158,7 +180,7 @@ struct MWalk {
     place -= __builtin_amdgcn_readfirstlane(s_pre[j]);
     tile = j * per;
     for (;; ++tile) {
-      const int w = __builtin_amdgcn_readfirstlane(m.weights[tile]);
+      const int w = __builtin_amdgcn_readfirstlane(weigh(m, tile));
       if (place < w) break;
       place -= w;
     }
@@ -170,20 +192,23 @@ struct MWalk {
         tile = 0;
         ++hc;
       }
-      const int n = __builtin_amdgcn_readfirstlane(m.weights[tile]);
+      int n;
+      if (m.a.cu_q == nullptr) {
+        n = find_single<COLS>(m, tile, t) ? weight_of<GR, ITEM>(t) : 0;
+      } else {
+        n = m.weights[tile];
+        const int4 x = m.tiles[2 * tile], y = m.tiles[2 * tile + 1];
+        t.req = x.x, t.row0 = x.y, t.nq = x.z, t.col0 = x.w;
+        t.end = y.x, t.prefix = y.y, t.lo = y.z, t.hi = y.w;
+      }
+      auto scalar = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
+      scalar(n);
       if (n == 0) {
         ++tile;
         continue;
       }
-      const int4 x = m.tiles[2 * tile], y = m.tiles[2 * tile + 1];
-      t.req = __builtin_amdgcn_readfirstlane(x.x);
-      t.row0 = __builtin_amdgcn_readfirstlane(x.y);
-      t.nq = __builtin_amdgcn_readfirstlane(x.z);
-      t.col0 = __builtin_amdgcn_readfirstlane(x.w);
-      t.end = __builtin_amdgcn_readfirstlane(y.x);
-      t.prefix = __builtin_amdgcn_readfirstlane(y.y);
-      t.lo = __builtin_amdgcn_readfirstlane(y.z);
-      t.hi = __builtin_amdgcn_readfirstlane(y.w);
+      scalar(t.req), scalar(t.row0), scalar(t.nq), scalar(t.end), scalar(t.col0);
+      scalar(t.prefix), scalar(t.lo), scalar(t.hi);
       head = hc;
       const int end = (int)min((int64_t)n, at + (u_end - u));
       u += end - at;
@@ -1104,7 +1129,7 @@ int launch(K kernel, std::atomic<uint64_t>& set, int bytes, const MArgs& m, cons
       return fail(FKC_ERR_LAUNCH, "kv4_attend: %d bytes of LDS refused", bytes);
     set.fetch_or(bit, std::memory_order_relaxed);
   }
-  if (!p.whole)
+  if (!p.whole && m.a.cu_q != nullptr)
     hipLaunchKernelGGL((kv4_tiles_kernel<COLS, GR, ITEM>), dim3((uint32_t)((p.ntiles + 3) / 4)),
                        dim3(256), 0, s, m);
   hipLaunchKernelGGL(kernel, dim3((uint32_t)p.wgs), dim3(THREADS), bytes, s, m);

@@ -252,11 +252,11 @@ struct Pieces {
 // caches they leave these to the loads (us a call without / with that, and with
 // loads past the caches too: 465 MB 204 / 182 / 176, 31.7 MB 23.2 / 11.7 / 15.0).
 // Units per thread at a time 2 / 4 / 8: 465 MB 177 / 182 / 221.
-__device__ inline void copy_piece(const Store& from, uint32_t sb, const Store& to, uint32_t db,
-                                  int piece, const Pieces& p) {
-  const int all = 2 * (p.codes + p.scales);
+struct Piece {
   Unit v[LOADS];
-  auto place = [&](int i, int* run, int* units) {
+  int piece;
+  // Run, units of it in a block and unit of the i-th one, -1 past the block.
+  __device__ inline int place(const Pieces& p, int i, int* run, int* units) const {
     const int u = piece * PIECE + i * PT + (int)threadIdx.x;
     int in = u;
     *run = 0;
@@ -268,20 +268,33 @@ __device__ inline void copy_piece(const Store& from, uint32_t sb, const Store& t
       *units = p.scales;
       if (in >= p.scales) in -= p.scales, *run = 3;
     }
-    return u < all ? in : -1;
-  };
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    int run, units;
-    const int in = place(i, &run, &units);
-    if (in >= 0) v[i] = from.p[run][(int64_t)sb * units + in];
+    return u < 2 * (p.codes + p.scales) ? in : -1;
   }
+  // Nothing is loaded of a block below 0.
+  __device__ inline Piece(const Store& from, int block, int piece_, const Pieces& p)
+      : piece(piece_) {
+    if (block < 0) return;
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    int run, units;
-    const int in = place(i, &run, &units);
-    if (in >= 0) __builtin_nontemporal_store(v[i], to.p[run] + (int64_t)db * units + in);
+    for (int i = 0; i < LOADS; ++i) {
+      int run, units;
+      const int in = place(p, i, &run, &units);
+      if (in >= 0) v[i] = from.p[run][(int64_t)block * units + in];
+    }
   }
+  __device__ inline void store(const Store& to, uint32_t block, const Pieces& p) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int run, units;
+      const int in = place(p, i, &run, &units);
+      if (in >= 0)
+        __builtin_nontemporal_store(v[i], to.p[run] + (int64_t)block * units + in);
+    }
+  }
+};
+
+__device__ inline void copy_piece(const Store& from, uint32_t sb, const Store& to, uint32_t db,
+                                  int piece, const Pieces& p) {
+  Piece(from, (int)sb, piece, p).store(to, db, p);
 }
 
 // f(block, piece) for the workgroup's pieces of n blocks; workgroup w of W.
@@ -443,6 +456,8 @@ fork_few_kernel(const Rows t, const int32_t* __restrict__ parents, int F, uint32
   const int j = (int)p.by_per.div(blockIdx.x), piece = (int)blockIdx.x - j * p.per;
   int mine[PER];
   const int own = part[j];
+  // On its way while it is found out whether and where to it is copied.
+  const Piece data(store, own, piece, p);
   bool copies = false;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -498,7 +513,7 @@ fork_few_kernel(const Rows t, const int32_t* __restrict__ parents, int F, uint32
   }
   const int32_t b = fresh_block(free_blocks, num_free, before, num_blocks);
   if (piece == 0 && threadIdx.x == 0) out[last_entry(t, j, out_seq)] = b;
-  if (b >= 0) copy_piece(store, (uint32_t)own, store, (uint32_t)b, piece, p);
+  if (b >= 0) data.store(store, (uint32_t)b, p);
 }
 
 // Any number of children: one workgroup finds them, with the lowest child that
