@@ -267,10 +267,8 @@ struct Columns {
   // seen by any.
   int from, to, lo, hi;
   __device__ inline void clear() {
-    from = lo = 0;
-    to = INT32_MAX;
-    hi = 0;
-    lo = INT32_MAX;
+    from = hi = 0;
+    to = lo = INT32_MAX;
   }
   __device__ inline void set(const MArgs& m, const MTile& t, int y, bool ok, int i, int h) {
     const Bounds b = bounds(m, t, i);
@@ -632,8 +630,8 @@ kv4_masked_split_kernel(const MArgs margs) {
     MState<DT, D, NT, MODE> st;
     st.clear();
     // What a tile has used up is fetched for the next one at once, after the last
-    // tile slot 0's (a load that may or may not be on its way would have to be
-    // waited for with every older one), into the same registers: with a second
+    // tile its own again (a load that may or may not be on its way would have to
+    // be waited for with every older one), into the same registers: with a second
     // set of them four waves a SIMD do not fit, and it is they that hide the loads'
     // latency.
     for (int it = wave; it < ntile; it += WAVES) {
@@ -782,11 +780,11 @@ struct Wide {
   static constexpr int WAVES = D == 256 ? 12 : 16, PER_SIMD = WAVES / 4;
   static constexpr int COLS = 16 * WAVES, THREADS = WAVES * 64;
   static constexpr int KS = D / 32, ND = D / 16;
-  static constexpr int G = 256 / D;            // groups of a stage
+  static constexpr int G = 256 / D;           // groups of a stage
   // Groups that an item costs by itself.
   static constexpr int ITEM = D == 64 ? 10 : 6;
   static constexpr int RUN = G * 32 * D * 2;  // bytes of a stage's keys or values
-  static constexpr int BUF = 2 * RUN;             // keys, then values
+  static constexpr int BUF = 2 * RUN;         // keys, then values
   // Scales of a stage in fp32, per group: keys', values', and (fp16)
   // exponent_of these.
   static constexpr int SCALES = 3 * 32 * 4;
@@ -1223,7 +1221,8 @@ int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const K
           (int)p.ntiles, 0.f, 0.f, nullptr, nullptr};
   if (sc.softcap > 0.f) {
     m.cap2 = (float)(2 * 1.4426950408889634 * sc.softcap);
-    m.cap_scale = (float)std::min(2 * scale / sc.softcap, 3e38);
+    // (a product of it with a key's scale stays finite for these up to 2^28)
+    m.cap_scale = (float)std::min(2 * scale / sc.softcap, 0x1p100);
   }
   if (!p.whole) {
     const Scratch w(ws, c, p);

@@ -229,7 +229,8 @@ def test_many_children_and_rows(kv4):
 # ------------------------------------------------------------ a run of them
 
 class _Loop:
-    """A server's step over one cache: free list, tables, append, attend."""
+    """A server's step over one cache: free list, tables, append, attention of a
+    model that caps its scores and looks back over a window."""
 
     def __init__(self, kv4, cache, requests, width):
         self.kv4, self.cache = kv4, cache
@@ -246,7 +247,8 @@ class _Loop:
         slots, cu, _ = self.kv4.block_tables(self.seq, new, self.tables, free,
                                              self.cache.block_size, len(k))
         self.kv4.append(self.cache, k, v, slots)
-        return self.kv4.attend(q, self.cache, self.tables, self.seq, cu, return_lse=True)
+        return self.kv4.attend(q, self.cache, self.tables, self.seq, cu, return_lse=True,
+                               softcap=30.0, window=50)
 
     def fork(self, parents):
         self.tables, self.seq, _ = self.kv4.fork(self.cache, self.tables, self.seq, i32(parents),
@@ -279,7 +281,8 @@ def test_a_server_that_forks_and_moves(kv4, dtype, D, bs):
         check.step(n, vectors(int(n.sum()), H * G), torch.cat([r[0] for r in rows]),
                    torch.cat([r[1] for r in rows]))
         cu = i32(np.cumsum([0] + new).tolist())
-        want = kv4.attend(q, check.cache, check.tables, n, cu, return_lse=True)
+        want = kv4.attend(q, check.cache, check.tables, n, cu, return_lse=True, softcap=30.0,
+                          window=50)
         assert torch.equal(loop.seq, n)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         mine = kv4.read(loop.cache, _slots(loop, rows))

@@ -281,6 +281,50 @@ def test_scores_that_are_not_numbers_show(kv4, dtype, nq):
         assert torch.equal(out.cpu()[~sees], clean[~sees])
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nq", [1, 240])
+def test_rows_that_see_nothing_ignore_their_query(kv4, dtype, nq):
+    """Padding may hold NaN and infinities: such rows are 0 and -inf, and their
+    neighbours what they are without them."""
+    seq = [300, 80]
+    cache, tables, g = _setup(seq, 16, 2, 64, dtype, 14)
+    q = torch.randn(2 * nq, 4, 64, generator=g).to(dtype)
+    starts = torch.zeros(2 * nq, dtype=torch.int32)
+    starts[::3] = 301
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    for kw in dict(), dict(softcap=20.0), dict(slopes=_slopes(4), window=60):
+        clean = _check(kv4, cache, tables, q, seq, [nq] * 2, starts=starts, **kw)
+        bad = q.clone()
+        bad[::3, :, ::2] = math.nan
+        bad[::3, :, 1::2] = math.inf
+        out, lse = kv4.attend(bad.cuda(), dev, tables.cuda(), i32(seq), i32([0, nq, 2 * nq]),
+                              return_lse=True, starts=starts.cuda(), **_gpu(kw))
+        assert torch.equal(out, clean)
+        assert bool((lse[::3] == -math.inf).all())
+
+
+def test_blocks_past_32_bits(kv4):
+    """Codes beyond 4 GiB into the cache give what they give near its start, bit
+    for bit, in both forms."""
+    H, D, bs, nb = 16, 256, 128, 18000
+    host, tables, g = _setup([2 * bs] * 2, bs, H, D, F16, 3, spare=0)
+    far = kv4.Cache.empty(nb, bs, D, host[4].cuda(), host[5].cuda(), F16)
+    assert far.k_codes.numel() > 2 ** 32
+    near = kv4.Cache(*(t.cuda() for t in host))
+    at = i32([nb - 1, 5, nb - 3, nb - 2])
+    kv4.copy_blocks(near, i32([0, 1, 2, 3]), far, at)
+    moved = at[tables.long().cuda()]
+    for nq in 1, 20:
+        q = torch.randn(2 * nq, 2 * H, D, generator=g).to(F16).cuda()
+        q = q if nq == 1 else q.repeat(8, 1, 1)  # (enough columns for the form of prompts)
+        m = q.shape[0] // 2
+        for kw in (dict(softcap=20.0), dict(slopes=_slopes(2 * H).cuda(), window=100),
+                   dict(prefix_lens=i32([50, 256]))):
+            args = i32([250, 2 * bs]), i32([0, m, 2 * m])
+            assert torch.equal(kv4.attend(q, far, moved, *args, **kw),
+                               kv4.attend(q, near, tables.cuda(), *args, **kw))
+
+
 @pytest.mark.parametrize("ragged", [False, True])
 @pytest.mark.parametrize("long", [40, 2600])
 def test_many_requests(kv4, ragged, long):
