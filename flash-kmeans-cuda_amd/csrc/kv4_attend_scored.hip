@@ -9,9 +9,10 @@
 // tokens [lo, hi) in which what lies before some row's first or behind some row's
 // last token is masked element by element.
 //
-// A tile is computed as in kv4_attend.hip.  The tanh is 1 - 2 / (1 + e^2x): one
-// exponential, one reciprocal, and nothing to tell apart for small or large x.
-// Scores are in powers of two from there on, so a weight is 2^(z - m).
+// A tile's products are those of kv4_attend.hip.  The tanh is 1 - 2 / (1 + e^2x):
+// one exponential, one reciprocal, and nothing to tell apart for small or large x;
+// off by a few units in the last place of 1, which a cap of 50 makes 1e-5 of a
+// score.  Scores are in powers of two from there on, so a weight is 2^(z - m).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -128,7 +129,9 @@ kv4_tiles_kernel(const MArgs m) {
 
 // The tiles' weights over all heads are cut into equal shares, one per
 // workgroup, wherever the cuts fall; an item (a tile under one head) that is cut
-// is joined afterwards.
+// is joined afterwards.  (Weights of a sum in closed form, as kv4_attend.hip has
+// them, do not know where documents begin; every workgroup adds up all of them
+// instead, about 1 us.)
 template <int COLS, int THREADS, int GR, int ITEM>
 struct MWalk {
   int64_t u = 0, u_end = 0, share = 1;
@@ -535,6 +538,18 @@ struct MState : State<DT, D, NT> {
 
 __device__ inline const MArgs& arguments() { return arguments_as<MArgs>(); }
 
+// The split form, for few columns, as in kv4_attend.hip: the waves of a workgroup
+// share NT tiles of 16 columns and take 32 tokens each in turn, are joined in LDS at
+// the end of an item, and cut items by a second kernel.
+//
+// Bound by memory where contexts are long: one query of each of 64 ragged requests
+// that look back over 4096 tokens, 435 MB of bf16 cache (D = 256, 8 heads of 2
+// capped), takes 92 us, 4.7 TB/s, where a large copy moves 4.6 and reading alone
+// 6.4.  Drafts of 2 to 7 tokens under slopes (fp16, D = 128, 4 heads of 8, contexts of
+// 300 to 65536, 175 MB) take 76 us: tiles of 16 columns look the same codes up 2.75
+// times, 128 look-ups a tile of 32 tokens, beside ~230 vector and 16 matrix
+// operations.  (Two tiles a wave look up half as often with half the waves: the
+// same.)
 template <int DT, int D, int NT, int WAVES, int MODE>
 __global__ void __launch_bounds__(WAVES * 64, WAVES / 2)
 kv4_masked_split_kernel(const MArgs margs) {
@@ -778,6 +793,22 @@ kv4_masked_split_kernel(const MArgs margs) {
 // each, no bank conflict), in one of two buffers; while a stage of G groups of
 // two halves of 16 tokens is computed on, the next one is filled into the other.
 //
+// Bound by the vector unit and the matrix cores one after the other: of four waves
+// a SIMD 64 vector operations take 310 ns, 16 exponentials 233, 16 products 476, the
+// first two together 543, the first and the last 696, all 862.  A group's 256
+// capped columns (D = 128) are 16 products, 24 exponentials and reciprocals and
+// ~95 others a wave, 1.3 us by that sum, and take 1.6: ragged prompts of 900 to 5600
+// tokens, 32 heads of 128 columns, bf16, 650 us (0.59 PFLOP/s).  Prefixes with
+// slopes, D = 256, 2000 to 5000 tokens, 659 us (0.55 PFLOP/s); documents of 700
+// tokens in requests of 9000 and 16000, fp16, D = 64, 163 us, a third of it what an
+// item costs by itself, the rest waves whose columns see nothing of a stage beside
+// others' that do.  What was measured (us): two waves a SIMD of two tiles each with
+// the scores of one group beside the weights of the last 770 (capped), with three
+// and four waves a SIMD of one tile 751, without each wave converting the scales
+// and with one operation less a weight 673, items weighed right 650.  Steps of 64
+// tokens a wave are no faster (D = 64), or spill (D = 128); nor is an item's first
+// stage loaded and filled during the last one's.
+//
 // Feature row n of fragment d of the second product is feature 32 (d / 2) + 2 n +
 // d % 2: the two codes of one byte go to two fragments, and 16 lanes read 16
 // bytes of a token.
@@ -787,7 +818,8 @@ struct Wide {
   static constexpr int COLS = 16 * WAVES, THREADS = WAVES * 64;
   static constexpr int KS = D / 32, ND = D / 16;
   static constexpr int G = 256 / D;           // groups of a stage
-  // Groups that an item costs by itself.
+  // Groups that an item costs by itself (us with 4 / 6 / 9: capped prompts 668 / 650 /
+  // 666, prefixes 693 / 690 / 692; documents with 7 / 10: 187 / 182).
   static constexpr int ITEM = D == 64 ? 10 : 6;
   static constexpr int RUN = G * 32 * D * 2;  // bytes of a stage's keys or values
   static constexpr int BUF = 2 * RUN;         // keys, then values

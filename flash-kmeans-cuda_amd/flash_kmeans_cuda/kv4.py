@@ -19,7 +19,12 @@ them new:
     out = kv4.attend(q, cache, tables, seq_lens, cu_new)
 
 `tables` is updated in place.  Lengths, tables and slots stay on the GPU:
-nothing here waits for it.
+nothing here waits for it.  Blocks that no row holds any more come back with
+
+    free, count = kv4.free_blocks(tables, seq_lens, block_size, num_blocks)
+
+`fork` makes rows that go on from others' tokens and share their blocks,
+`compact` moves the held blocks into another cache, `copy_blocks` single ones.
 
 The cache holds codes, which have no gradient: `append` and `read` take and give
 values only, and going back through `attend` raises.
