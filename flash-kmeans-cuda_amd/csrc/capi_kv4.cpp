@@ -90,8 +90,9 @@ int attend_ok(const fkc_kv4_cache& c, const Kv4Attend& a, int64_t max_blocks) {
 
 int scores_ok(const fkc_kv4_scores* x, const char* what) {
   if (!x) return fail(FKC_ERR_INVALID, "%s: null scores", what);
-  if (!(x->softcap >= 0.f && x->softcap <= std::numeric_limits<float>::max()))
-    return fail(FKC_ERR_INVALID, "%s: softcap is not a positive finite number", what);
+  // (beyond these factors of it leave fp32's range)
+  if (x->softcap != 0.f && !(x->softcap >= 1e-30f && x->softcap <= 1e30f))
+    return fail(FKC_ERR_INVALID, "%s: softcap is not between 1e-30 and 1e30", what);
   if (x->window < 0 || x->window > kI32)
     return fail(FKC_ERR_INVALID, "%s: window out of range", what);
   return FKC_OK;

@@ -11,8 +11,9 @@
 //
 // A tile's products are those of kv4_attend.hip.  The tanh is 1 - 2 / (1 + e^2x):
 // one exponential, one reciprocal, and nothing to tell apart for small or large x;
-// off by a few units in the last place of 1, which a cap of 50 makes 1e-5 of a
-// score.  Scores are in powers of two from there on, so a weight is 2^(z - m).
+// off by a few units in the last place of 1, which a cap of 50 makes 5e-5 of a
+// score at most (large caps: sharp_tanh).  Scores are in powers of two from there
+// on, so a weight is 2^(z - m).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -29,7 +30,10 @@ namespace {
 // What is done to a score between the products.
 constexpr int kMask = 0;  // nothing
 constexpr int kCap = 1;   // the cap
-constexpr int kBias = 2;  // the distance, and the cap where cap2 is not 0
+constexpr int kBias = 2;  // the distance
+constexpr int kBoth = 3;  // the cap, by sharp_tanh, and the distance
+constexpr bool capped(int mode) { return mode == kCap || mode == kBoth; }
+constexpr bool biased(int mode) { return mode >= kBias; }
 
 struct MArgs {
   Args a;
@@ -264,8 +268,8 @@ struct MWalk {
 template <int MODE, int NT>
 struct Columns {
   int first[NT], last[NT];
-  int pos[MODE == kBias ? NT : 1];
-  float slope[MODE == kBias ? NT : 1];  // in powers of two
+  int pos[biased(MODE) ? NT : 1];
+  float slope[biased(MODE) ? NT : 1];  // in powers of two
   // Every token from .. to - 1 is seen by all columns; none outside lo .. hi is
   // seen by any.
   int from, to, lo, hi;
@@ -277,9 +281,9 @@ struct Columns {
     const Bounds b = bounds(m, t, i);
     first[y] = ok ? b.first : 0;
     last[y] = ok ? b.last : 0;
-    if constexpr (MODE == kBias) {
+    if constexpr (biased(MODE)) {
       pos[y] = t.end - t.nq + i;
-      slope[y] = m.slopes[h] * kLog2e;
+      slope[y] = m.slopes != nullptr ? m.slopes[h] * kLog2e : 0.f;
     }
     if (!ok) return;  // computed along, and dropped
     from = max(from, b.first);
@@ -311,11 +315,24 @@ __device__ inline float exponent_of(float scale) {
   return __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(fabsf(scale)), -60.f, 129.f);
 }
 
+// tanh x of e = 2 log2(e) x within 2^-18 of itself: for |x| < 0.35 the series, whose
+// first term left out is 2^-22 of it, and 1 - 2 / (1 + 2^e), off by 2^-20 of 1,
+// beyond.
+__device__ inline float sharp_tanh(float e) {
+  const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
+  const float x = e * 0.34657359f, xx = x * x;
+  float p = __builtin_fmaf(xx, 62.f / 2835, -17.f / 315);
+  p = __builtin_fmaf(p, xx, 2.f / 15);
+  p = __builtin_fmaf(p, xx, -1.f / 3);
+  p = __builtin_fmaf(p * xx, x, x);
+  return fabsf(e) < 1.f ? p : __builtin_fmaf(-2.f, r, 1.f);
+}
+
 // As State (kv4_tile.hpp), with scores as above, in the steps that a kernel may
 // put between its products.  What stands for a score z in powers of two:
 //   kMask  z / zscale,
 //   kCap   r = 1 / (1 + e^2x), with z = cap2 / 2 - cap2 r (hidden: r = infinity),
-//   kBias  z - shift, one shift per column and tile,
+//   kBias, kBoth  z - shift, one shift per column and tile,
 // so that the last multiplication is the one that the weight's exponent needs
 // anyway.
 template <int DT, int D, int NT, int MODE, bool LAG>
@@ -339,7 +356,7 @@ struct MState : State<DT, D, NT> {
   // Of the tile at hand: the keys' scales, times the first step's factor but for
   // kMask, the values', and (fp16) exponent_of these.
   f32x4 ks[2], vs[2], ve[DT == FKC_F16 ? 2 : 1];
-  float shift[MODE == kBias ? NT : 1];
+  float shift[biased(MODE) ? NT : 1];
   __device__ inline float base2(int y, float zscale) const {
     if constexpr (DT == FKC_F16) return m[y] - kLead;
     return __builtin_amdgcn_fmed3f(MODE == kMask ? m[y] * zscale : m[y], kLowest, -kLowest);
@@ -365,16 +382,18 @@ struct MState : State<DT, D, NT> {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[y][j][i] *= ks[j][i];
-      if (MODE == kCap || (MODE == kBias && cap2 != 0.f)) {
+      if constexpr (capped(MODE)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[y][j][i]));
-            z[y][j][i] = MODE == kCap ? r : __builtin_fmaf(-cap2, r, 0.5f * cap2);
+            const float e = z[y][j][i];
+            z[y][j][i] = MODE == kCap
+                             ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e))
+                             : 0.5f * cap2 * sharp_tanh(e);
           }
       }
-      if constexpr (MODE == kBias) {
+      if constexpr (biased(MODE)) {
         // Before all of the tile or behind it a column's distances rise or fall by
         // one from token to token.
         const int away = c.pos[y] - tok;  // (exact in fp32 below 2^24)
@@ -464,7 +483,7 @@ struct MState : State<DT, D, NT> {
         }
       if constexpr (MODE == kCap)
         t = DT != FKC_F16 ? __builtin_fmaf(-cap2, t, 0.5f * cap2) : t + 0.5f * cap2;
-      if constexpr (MODE == kBias) t += shift[y];
+      if constexpr (biased(MODE)) t += shift[y];
       top[y] = t;
       more |= DT == FKC_F16 || MODE != kMask ? t > m[y] + kLag : (t - m[y]) * zscale > kLag;
     }
@@ -491,7 +510,7 @@ struct MState : State<DT, D, NT> {
   }
   __device__ inline float base_of(int y, float zscale, float cap2) const {
     const float b = -base2(y, zscale);
-    return MODE == kCap ? 0.5f * cap2 + b : MODE == kBias ? shift[y] + b : b;
+    return MODE == kCap ? 0.5f * cap2 + b : biased(MODE) ? shift[y] + b : b;
   }
   // Scores to weights, packed as the second product reads them.
   __device__ inline void weigh(const f32x4 (&z)[NT][2], float zscale, float cap2,
@@ -632,8 +651,7 @@ kv4_masked_split_kernel(const MArgs margs) {
                    a.qsign;
     }
     cols.reduce();
-    const float zscale = MODE == kCap || (MODE == kBias && ma.cap2 != 0.f) ? ma.cap_scale
-                                                                         : a.zscale;
+    const float zscale = capped(MODE) ? ma.cap_scale : a.zscale;
     const float cap2 = ma.cap2;
     const Lane<D> lanes(n, g);
     Codes<D> cur;
@@ -886,7 +904,7 @@ kv4_masked_wide_kernel(const MArgs margs) {
     Global k_scales = (Global)a.k_scales, v_scales = (Global)a.v_scales;
     uint32_t bs = a.bs.d, bs_m = a.bs.m, num_blocks = a.num_blocks;
     int bs_sh = a.bs.sh, heads = a.heads;
-    float zscale = MODE == kCap || (MODE == kBias && ma.cap2 != 0.f) ? ma.cap_scale : a.zscale;
+    float zscale = capped(MODE) ? ma.cap_scale : a.zscale;
     float cap2 = ma.cap2;
     asm volatile("" : "+s"(k_codes), "+s"(v_codes), "+s"(k_scales), "+s"(v_scales));
     asm volatile("" : "+s"(bs), "+s"(bs_m), "+s"(num_blocks), "+s"(bs_sh), "+s"(heads),
@@ -1232,6 +1250,11 @@ size_t kv4_attend_scored_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int6
   return p.whole ? 0 : Scratch(nullptr, c, p).bytes;
 }
 
+// Caps above this take kBoth, with slopes of 0: kCap's tanh is off by 2^-20 of the cap,
+// 2^-12 of a weight here, half of a step of fp16.  Prompts capped at 50 take 660 us
+// with kCap and 953 with kBoth, single tokens 13.4 and 14.6.
+constexpr float kSharp = 256.f;
+
 int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const Kv4Scores& sc,
                              void* ws, hipStream_t s) {
   const Plan p = make_plan(c, x.H, x.T, x.R, x.max_seq, reach_of(x.max_seq, sc, x.causal),
@@ -1272,6 +1295,8 @@ int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const K
   }
   return kv4_by_shape(c.dtype, c.D, [&](auto dt, auto d) {
     constexpr int DT = dt.value, DD = d.value;
+    if (sc.softcap > (sc.slopes != nullptr ? 0.f : kSharp))
+      return launch_mode<DT, DD, kBoth>(m, p, s);
     if (sc.slopes != nullptr) return launch_mode<DT, DD, kBias>(m, p, s);
     if (sc.softcap > 0.f) return launch_mode<DT, DD, kCap>(m, p, s);
     return launch_mode<DT, DD, kMask>(m, p, s);

@@ -286,7 +286,7 @@ class _CScores(ctypes.Structure):
 def _scores(softcap, slopes, window, starts, prefix_lens, T, H, R, dev):
     """(the C struct of attend's options, the tensors it points into)."""
     if softcap is not None:
-        _require(0.0 < softcap < 3e38, f"softcap must be positive and finite, not {softcap}")
+        _require(1e-30 <= softcap <= 1e30, f"softcap must be within 1e-30 .. 1e30, not {softcap}")
     if window is not None:
         _require(0 < window < 1 << 31, f"window must be at least 1, below 2^31, not {window}")
     if slopes is not None:
@@ -333,7 +333,7 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
 
     Scores and masks of other models, any of them together, for a query at
     position p of its request and a token at t:
-      softcap      a score z becomes softcap * tanh(z / softcap);
+      softcap      a score z becomes softcap * tanh(z / softcap), 1e-30 <= softcap <= 1e30;
       slopes       (H,) float32: slopes[h] * |p - t| is taken off it, after the cap;
       window       no token more than window - 1 positions back is seen: t > p - window;
       starts       (T,) int32, no token before starts[row] is seen: the first token of

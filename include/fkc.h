@@ -463,7 +463,7 @@ FKC_CAPI int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
  * over the tokens first <= t < last,
  *   last  = seq_lens[r], or if causal at most max(p + 1, prefix_lens[r]),
  *   first = max(0, starts[row], p - window + 1)  (window 0, starts NULL: without).
- * softcap > 0 and finite or 0; slopes (H) fp32, finite; window >= 0, below 2^31;
+ * softcap 0 or 1e-30 to 1e30; slopes (H) fp32, finite; window >= 0, below 2^31;
  * starts (T) and prefix_lens (R) int32 of any values.  A row whose first is not
  * below its last sees nothing.  Scores are fp32; the distance is exact below
  * 2^24 and rounded beyond.  With a softcap or slopes a key's scale times

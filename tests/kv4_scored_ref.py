@@ -34,6 +34,9 @@ def attend(q, cache, tables, seq, nq, causal=True, sm_scale=None, max_seq=None, 
       last place (2^-23) each, of sums that are rounded to 2^-24: the reciprocal,
       at most 1, is off by 2^-22 and a quarter of the exponential's error, twice
       the cap times that below                                  cap 2^-20
+      and for caps above 256 at most                               |z| 2^-18:
+      where tanh is below 1/3 its series, 2^-22 of it left out and five
+      roundings, and above that the same 2^-20 of the cap
       the distance's product, its sum and the difference to the maximum:
                                                               |bias| 2^-22
       the score itself, rounded in powers of two                  |z| 2^-22
@@ -76,7 +79,7 @@ def attend(q, cache, tables, seq, nq, causal=True, sm_scale=None, max_seq=None, 
                 e = (D + 12) * 2.0 ** -24 * abs(sm_scale) * (qq.abs() @ k.abs().T)
                 if softcap is not None:
                     z = softcap * torch.tanh(z / softcap)
-                    e = e + softcap * 2.0 ** -20
+                    e = e + (softcap * 2.0 ** -20 if softcap <= 256 else z.abs() * 2.0 ** -18)
                 if slopes is not None:
                     bias = float(slopes[g]) * away
                     z = z - bias

@@ -376,6 +376,46 @@ def test_the_options_of_nothing_are_none(kv4):
                                                   for k, v in kw.items()})
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("nq", [1, 6, 260])
+@pytest.mark.parametrize("softcap", [1e-30, 1e-9, 256.0, 257.0, 3e4, 1e9, 1e30])
+def test_caps_of_any_size(kv4, dtype, nq, softcap):
+    """Caps far below every score, where all weights are alike, to far above,
+    where they are those without a cap."""
+    seq = [400, 257]
+    cache, tables, g = _setup(seq, 32, 2, 64, dtype, 11)
+    cache[2][tables[0, :5].long()] *= 20
+    q = (3 * torch.randn(2 * nq, 8, 64, generator=g)).to(dtype)
+    for scale in None, -2.0:
+        _check(kv4, cache, tables, q, seq, [nq] * 2, sm_scale=scale, softcap=softcap)
+    _check(kv4, cache, tables, q, seq, [nq] * 2, softcap=softcap, slopes=_slopes(8), window=300)
+
+
+def test_rows_of_nothing(kv4):
+    """Queries of no request, requests of no tokens, tables without entries, no
+    query at all; slopes in steps."""
+    seq = [40, 60]
+    cache, tables, g = _setup(seq, 16, 2, 64, F16, 7)
+    dev, t = kv4.Cache(*(x.cuda() for x in cache)), tables.cuda()
+    q = torch.randn(5, 8, 64, generator=g).to(F16).cuda()
+    none = i32([])
+    slopes = torch.zeros(8, 3, device="cuda")
+    slopes[:, 1] = _slopes(8).cuda()
+    strided = slopes[:, 1]
+    for kw in dict(softcap=9.0), dict(slopes=strided), dict(window=20), dict(softcap=1e4):
+        for args in ((t[:0], none, i32([0])), (t[:0, :0], none, i32([0])),
+                     (t[:, :0], i32(seq), i32([0, 2, 5])), (t, i32([0, -3]), i32([0, 2, 5]))):
+            out, lse = kv4.attend(q, dev, *args, return_lse=True, **kw)
+            assert not bool(out.any()) and bool((lse == -math.inf).all())
+        out = kv4.attend(q, dev, t, i32(seq), i32([0, 2, 5]), max_seq=0, **kw)
+        assert not bool(out.any())
+        out, lse = kv4.attend(q[:0], dev, t, i32(seq), i32([0, 0, 0]), return_lse=True, **kw)
+        assert out.shape == (0, 8, 64) and lse.shape == (0, 8)
+    args = q, dev, t, i32(seq), i32([0, 2, 5])
+    assert torch.equal(kv4.attend(*args, slopes=strided),
+                       kv4.attend(*args, slopes=strided.contiguous()))
+
+
 def test_offsets_that_do_not_ascend_end(kv4):
     """Nonsense offsets stay in range, and what they do not name is written as
     it is without them."""
@@ -463,6 +503,8 @@ def test_gradients_raise(kv4):
 @pytest.mark.parametrize("kw,word", [
     (dict(softcap=0.0), "softcap"), (dict(softcap=-1.0), "softcap"),
     (dict(softcap=math.inf), "softcap"), (dict(softcap=math.nan), "softcap"),
+    (dict(softcap=1e-50), "softcap"), (dict(softcap=9e-31), "softcap"),
+    (dict(softcap=2e30), "softcap"),
     (dict(window=0), "window"), (dict(window=-1), "window"), (dict(window=1 << 31), "window"),
     (dict(slopes=torch.zeros(4)), None), (dict(slopes="half"), "float32"),
     (dict(slopes="short"), "float32"), (dict(starts="long"), "int32"),

@@ -31,7 +31,8 @@ def _attend(scores, q=FAKE, ts=256, hs=64, H=4, T=3, tables=FAKE, stride=8, widt
 
 @pytest.mark.parametrize("kw,word", [
     (dict(softcap=-1.0), "softcap"), (dict(softcap=math.inf), "softcap"),
-    (dict(softcap=math.nan), "softcap"), (dict(window=-1), "window"),
+    (dict(softcap=math.nan), "softcap"), (dict(softcap=1e-31), "softcap"),
+    (dict(softcap=1e31), "softcap"), (dict(window=-1), "window"),
     (dict(window=1 << 31), "window")])
 def test_options_are_checked(kw, word):
     from flash_kmeans_cuda import _lib
