@@ -337,6 +337,8 @@ int fkc_kv4_fork(const fkc_kv4_cache* cache, const int32_t* tables, int64_t tabl
     return fail(FKC_ERR_INVALID, "kv4_fork: size out of range");
   if (max_blocks && F >= (int64_t)UINT32_MAX / max_blocks)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_fork: 2^32 table entries and more");
+  // (a workgroup of 256 for each, and a launch has less than 2^32 threads)
+  if (F >= 1 << 24) return fail(FKC_ERR_UNSUPPORTED, "kv4_fork: 2^24 children and more");
   if (!taken || (F && (!parents || !new_seq || (max_blocks && !new_tables))) ||
       (num_free && !free_blocks))
     return fail(FKC_ERR_INVALID, "kv4_fork: null pointer argument");

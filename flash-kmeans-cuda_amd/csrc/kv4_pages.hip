@@ -615,6 +615,9 @@ void launch_names(const Kv4Tables& t, int64_t bs, int64_t num_blocks, const Name
                      list, number, total);
 }
 
+// (a launch has less than 2^32 threads: huge blocks are left to copy_kernel's loop)
+bool few(int64_t F, const Pieces& p) { return F <= FEW && F * p.per < (int64_t)1 << 23; }
+
 uint32_t copy_grid(int64_t blocks, const Pieces& p) { return grid_for(blocks * p.per, 8); }
 
 }  // namespace
@@ -670,7 +673,7 @@ size_t kv4_fork_workspace_bytes(const fkc_kv4_cache& c, int64_t F) {
   Carve w(nullptr);
   w.take<uint32_t>((size_t)c.num_blocks);
   w.take<int32_t>((size_t)F);
-  if (F > FEW) w.take<int32_t>((size_t)F * 2 + (size_t)c.num_blocks);
+  if (!few(F, Pieces(c))) w.take<int32_t>((size_t)F * 2 + (size_t)c.num_blocks);
   return w.used;
 }
 
@@ -689,7 +692,7 @@ int launch_kv4_fork(const fkc_kv4_cache& c, const Kv4Tables& t, const int32_t* p
   const Pieces p(c);
   hipLaunchKernelGGL(fork_mark_kernel, dim3((uint32_t)F), dim3(PT), 0, s, r, parents, F, nb,
                      entry, part, new_tables, new_seq);
-  if (F <= FEW) {
+  if (few(F, p)) {
     hipLaunchKernelGGL(fork_few_kernel, dim3((uint32_t)(F * p.per)), dim3(PT), 0, s, r, parents,
                        (int)F, nb, entry, part, free_blocks, num_free, new_tables, new_seq, taken,
                        Store(c), p);

@@ -112,6 +112,46 @@ def test_fork_of_every_block_size(kv4, dtype, heads, D, bs):
     _check_fork(kv4, 4, 3, bs, 30, 9, D + bs, heads=heads, D=D, dtype=dtype)
 
 
+def test_forks_of_huge_blocks(kv4):
+    """More pieces of blocks than a launch has workgroups of them."""
+    bs, nb, F = 1 << 18, 4, 1000
+    codes = [torch.randint(0, 256, (nb, 8, bs, 32), dtype=torch.uint8, device="cuda")
+             for _ in range(2)]
+    scales = [torch.rand(nb, 8, bs, device="cuda").to(F16) for _ in range(2)]
+    levels = [torch.rand(8, 16, device="cuda").to(F16) for _ in range(2)]
+    cache = kv4.Cache(*codes, *scales, *levels)
+    before = [t.clone() for t in codes + scales]
+    tables, seq = np.array([[1, 0]], np.int32), np.array([bs + 5], np.int32)
+    want, want_seq, taken, copies = pages.fork(tables, seq, [0] * F, [3], bs, nb)
+    new, new_seq, n = kv4.fork(cache, i32(tables.tolist()), i32(seq.tolist()), i32([0] * F),
+                               i32([3]))
+    assert n.tolist() == [taken] and copies == [(0, 3)]
+    assert np.array_equal(new.cpu().numpy(), want)
+    assert np.array_equal(new_seq.cpu().numpy(), want_seq)
+    for t, old in zip(codes + scales, before):
+        assert torch.equal(t[:3], old[:3]) and torch.equal(t[3], old[0])
+
+
+def test_pages_of_nothing(kv4):
+    """Tables without rows or without entries, an empty cache, parents that are
+    no rows."""
+    for nb in 0, 20:
+        _, cache = _cache(kv4, nb, 2, 16, 64, F16, 3)
+        _, into = _cache(kv4, 5, 2, 16, 64, F16, 4)
+        for tables, seq in (([], []), ([[]] * 3, [40, 0, 5]), ([[1, 2], [3, -1]], [0, -9])):
+            width = 2 if len(tables) == 2 else 0
+            t = torch.tensor(tables, dtype=torch.int32, device="cuda").reshape(len(seq), width)
+            free, count = kv4.free_blocks(t, i32(seq), 16, nb)
+            assert free.tolist() == list(range(nb)) and count.tolist() == [nb]
+            new, new_seq, taken = kv4.fork(cache, t, i32(seq), i32([-1, 5, 0]), i32([9]))
+            assert new.shape == (3, width) and bool((new == -1).all()) and taken.tolist() == [0]
+            assert new_seq.tolist() == [0, 0, max(seq[0], 0) if seq else 0]
+            new, used = kv4.compact(cache, t, i32(seq), into)
+            assert new.shape == t.shape and bool((new == -1).all()) and used.tolist() == [0]
+        kv4.copy_blocks(cache, i32([0, 1]), into, i32([-1, 7]))
+    torch.cuda.synchronize()
+
+
 def test_fork_keeps_and_copies(kv4):
     """Two children of one parent; a parent that two rows share the last block
     of; one whose last block is another's whole one; no child at all."""

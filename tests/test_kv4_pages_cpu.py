@@ -47,7 +47,7 @@ def test_fork_refusals():
     for at, value, code, word in (
             (0, None, 1, "null cache"), (1, None, 1, "null"), (2, 7, 1, "overlap"),
             (3, -1, 1, "range"), (4, None, 1, "null"), (5, -1, 1, "range"), (6, None, 1, "null"),
-            (5, 1 << 29, 4, "2^32"), (7, 1 << 29, 4, "2^32"),
+            (5, 1 << 29, 4, "2^32"), (7, 1 << 29, 4, "2^32"), (7, 1 << 24, 4, "2^24"),
             (7, -1, 1, "range"), (8, None, 1, "null"), (9, -1, 1, "range"), (10, None, 1, "null"),
             (11, None, 1, "null"), (12, None, 1, "null"), (13, None, 2, "workspace"),
             (13, FAKE + 8, 2, "aligned"), (14, need - 1, 2, "workspace")):
