@@ -1251,7 +1251,7 @@ size_t kv4_attend_scored_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int6
 }
 
 // Caps above this take kBoth, with slopes of 0: kCap's tanh is off by 2^-20 of the cap,
-// 2^-12 of a weight here, half of a step of fp16.  Prompts capped at 50 take 660 us
+// 2^-12 of a weight here, half of a step of fp16.  Prompts capped at 30 take 660 us
 // with kCap and 953 with kBoth, single tokens 13.4 and 14.6.
 constexpr float kSharp = 256.f;
 
