@@ -30,7 +30,7 @@ namespace {
 // What is done to a score between the products.
 constexpr int kMask = 0;  // nothing
 constexpr int kCap = 1;   // the cap
-constexpr int kBias = 2;  // the distance
+constexpr int kBias = 2;  // the distance; in the wide form the cap too, if there is one
 constexpr int kBoth = 3;  // the cap, by sharp_tanh, and the distance
 constexpr bool capped(int mode) { return mode == kCap || mode == kBoth; }
 constexpr bool biased(int mode) { return mode >= kBias; }
@@ -382,7 +382,9 @@ struct MState : State<DT, D, NT> {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[y][j][i] *= ks[j][i];
-      if constexpr (capped(MODE)) {
+      // (LAG: the wide form, where asking as it runs is the faster way: prefixes under
+      // slopes 699 us, without the question 737.  Drafts 93.4, with it 94.9.)
+      if (capped(MODE) || (LAG && MODE == kBias && cap2 != 0.f)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -904,7 +906,7 @@ kv4_masked_wide_kernel(const MArgs margs) {
     Global k_scales = (Global)a.k_scales, v_scales = (Global)a.v_scales;
     uint32_t bs = a.bs.d, bs_m = a.bs.m, num_blocks = a.num_blocks;
     int bs_sh = a.bs.sh, heads = a.heads;
-    float zscale = capped(MODE) ? ma.cap_scale : a.zscale;
+    float zscale = capped(MODE) || (MODE == kBias && ma.cap2 != 0.f) ? ma.cap_scale : a.zscale;
     float cap2 = ma.cap2;
     asm volatile("" : "+s"(k_codes), "+s"(v_codes), "+s"(k_scales), "+s"(v_scales));
     asm volatile("" : "+s"(bs), "+s"(bs_m), "+s"(num_blocks), "+s"(bs_sh), "+s"(heads),
@@ -1215,7 +1217,7 @@ int launch_wide(const MArgs& m, const Plan& p, hipStream_t s) {
 
 template <int DT, int D, int MODE>
 int launch_mode(const MArgs& m, const Plan& p, hipStream_t s) {
-  if (p.wide) return launch_wide<DT, D, MODE>(m, p, s);
+  if (p.wide) return launch_wide<DT, D, MODE == kBoth ? kBias : MODE>(m, p, s);
   if constexpr (D < 256)
     if (p.nt == 2) return launch_split<DT, D, 2, 4, MODE>(m, p, s);
   return launch_split<DT, D, 1, waves_of(D), MODE>(m, p, s);
@@ -1252,7 +1254,7 @@ size_t kv4_attend_scored_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int6
 
 // Caps above this take kBoth, with slopes of 0: kCap's tanh is off by 2^-20 of the cap,
 // 2^-12 of a weight here, half of a step of fp16.  Prompts capped at 30 take 660 us
-// with kCap and 953 with kBoth, single tokens 13.4 and 14.6.
+// with kCap and 953 with the series, single tokens 13.4 and 14.6.
 constexpr float kSharp = 256.f;
 
 int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const Kv4Scores& sc,
