@@ -163,15 +163,16 @@ class Cache:
     def empty(cls, num_blocks: int, block_size: int, head_dim: int, k_levels: torch.Tensor,
               v_levels: torch.Tensor, dtype: torch.dtype) -> "Cache":
         """A cache of num_blocks blocks on the levels' device.  The levels
-        (heads, 16), of any floating dtype, are rounded to `dtype`; what the
-        blocks hold before it is stored is never used."""
+        (heads, 16), of any floating dtype, are copied, rounded to `dtype`; what
+        the blocks hold before it is stored is never used."""
         heads, dev = k_levels.shape[0], k_levels.device
         codes = [torch.empty((num_blocks, heads, block_size, head_dim // 2), dtype=torch.uint8,
                              device=dev) for _ in range(2)]
         scales = [torch.empty((num_blocks, heads, block_size), dtype=dtype, device=dev)
                   for _ in range(2)]
-        return cls(*codes, *scales, k_levels.to(dtype).contiguous(),
-                   v_levels.to(dtype).contiguous())
+        levels = [t.to(dtype, copy=True, memory_format=torch.contiguous_format)
+                  for t in (k_levels, v_levels)]
+        return cls(*codes, *scales, *levels)
 
 
 def learn_levels(sample: torch.Tensor, max_iters: int = 25, tol: float = 1e-5) -> torch.Tensor:

@@ -169,6 +169,33 @@ def test_a_cache_keeps_its_tensors(kv4):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("given", [F16, BF16, torch.float32])
+def test_an_empty_cache_has_levels_of_its_own(kv4, dtype, given):
+    """Cache.empty copies the levels whatever their dtype, so one tensor may be
+    given for keys and values, and writing it, or one of the cache's, changes
+    no other."""
+    lv = ref.random_levels(2, BF16, 0).to(given).cuda()
+    want = lv.to(dtype).clone()
+    c = kv4.Cache.empty(4, 16, 64, lv, lv, dtype)
+    x = torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    kv4.append(c, x, x, i32([0, 1, 2]))
+    before = kv4.read(c, i32([0, 1, 2]))
+    old = lv.clone()
+    lv.zero_()
+    assert torch.equal(c.k_levels, want) and torch.equal(c.v_levels, want)
+    for a, b in zip(kv4.read(c, i32([0, 1, 2])), before):
+        assert torch.equal(a, b)
+    lv.copy_(old)
+    c.k_levels.zero_()
+    assert torch.equal(c.v_levels, want) and torch.equal(lv, old)
+    # a slice that does not begin at 16 bytes, a transposed one
+    wide = torch.zeros(16, 3, dtype=given, device="cuda")
+    wide[:, 1:] = lv.t()
+    c = kv4.Cache.empty(4, 16, 64, wide[:, 1:].t(), wide[:, 1:].t(), dtype)
+    assert torch.equal(c.k_levels, want) and c.k_levels.is_contiguous()
+
+
 # ------------------------------------------------------------ gradients
 
 def test_a_gradient_through_the_cache_is_refused(kv4):
