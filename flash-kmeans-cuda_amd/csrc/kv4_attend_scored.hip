@@ -335,23 +335,20 @@ __device__ inline float sharp_tanh(float e) {
 //   kBias, kBoth  z - shift, one shift per column and tile,
 // so that the last multiplication is the one that the weight's exponent needs
 // anyway.
-template <int DT, int D, int NT, int MODE, bool LAG>
+template <int DT, int D, int NT, int MODE, bool WIDE>
 struct MState : State<DT, D, NT> {
   typedef State<DT, D, NT> S;
   using S::l;
   using S::m;
   using S::o;
   static constexpr int ND = S::ND;
-  // What m may lag behind the largest score (powers of two) before everything is
-  // made relative to a new one; fp16: 2^kLead is the largest weight times scale
-  // without a lag, so 2^14 with it.  A lag spares most of the scaling (with 1024
-  // columns a CU some column has a new maximum in most groups of the first
-  // thousand tokens): capped prompts 656 us instead of 690, documents 179 instead
-  // of 188, single tokens and drafts the same, which have none.  It costs what the
-  // largest weight, no longer 1, is rounded by: capped prompts of large scores are
-  // 2.0e-3 off 64-bit results instead of 1.8e-3, the result's own rounding making 1.7e-3.
-  static constexpr float kLag = !LAG ? 0.f : DT == FKC_F16 ? 6.f : 8.f;
-  static constexpr float kLead = LAG ? 8.f : 14.f;
+  // m is the largest score so far, so the largest weight is 1 and its product with
+  // its scale is exact (fp16: the largest product is 2^kLead).  A maximum left
+  // behind by up to 2^8 (fp16 2^6) spares most of the scaling, capped prompts 658 us
+  // instead of 690, documents 181 instead of 188, and rounds the largest product
+  // too: capped prompts 2.05e-3 off the plain form instead of 0.99e-3, documents
+  // 2.5e-4 instead of 1.6e-4.
+  static constexpr float kLead = 14.f;
   static constexpr float kHidden = MODE == kCap ? INFINITY : -INFINITY;
   // Of the tile at hand: the keys' scales, times the first step's factor but for
   // kMask, the values', and (fp16) exponent_of these.
@@ -382,9 +379,9 @@ struct MState : State<DT, D, NT> {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[y][j][i] *= ks[j][i];
-      // (LAG: the wide form, where asking as it runs is the faster way: prefixes under
+      // (WIDE: the wide form, where asking as it runs is the faster way: prefixes under
       // slopes 699 us, without the question 737.  Drafts 93.4, with it 94.9.)
-      if (capped(MODE) || (LAG && MODE == kBias && cap2 != 0.f)) {
+      if (capped(MODE) || (WIDE && MODE == kBias && cap2 != 0.f)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -487,7 +484,7 @@ struct MState : State<DT, D, NT> {
         t = DT != FKC_F16 ? __builtin_fmaf(-cap2, t, 0.5f * cap2) : t + 0.5f * cap2;
       if constexpr (biased(MODE)) t += shift[y];
       top[y] = t;
-      more |= DT == FKC_F16 || MODE != kMask ? t > m[y] + kLag : (t - m[y]) * zscale > kLag;
+      more |= t > m[y];
     }
     if (__any(more)) {
 #pragma unroll

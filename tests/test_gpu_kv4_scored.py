@@ -376,6 +376,74 @@ def test_the_options_of_nothing_are_none(kv4):
                                                   for k, v in kw.items()})
 
 
+@pytest.mark.parametrize("nq", [[300, 5], [1, 1], [40, 40]])
+def test_the_options_of_nothing_give_the_bits_of_none(kv4, nq):
+    """bf16, where both kernels make weights relative to the largest score: a
+    window of everything, no documents, no prefix leave the same operations in
+    the same order."""
+    seq = [300, 700]
+    cache, tables, g = _setup(seq, 16, 2, 128, BF16, 3)
+    q = torch.randn(sum(nq), 8, 128, generator=g).to(BF16)
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    args = q.cuda(), dev, tables.cuda(), i32(seq), i32([0, nq[0], sum(nq)])
+    want, want_lse = kv4.attend(*args, return_lse=True)
+    zero = torch.zeros(sum(nq), dtype=torch.int32, device="cuda")
+    for kw in (dict(window=10 ** 6), dict(starts=zero), dict(prefix_lens=zero[:2])):
+        out, lse = kv4.attend(*args, return_lse=True, **kw)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("nq", [1, 128])
+@pytest.mark.parametrize("kw", [dict(window=10 ** 6), dict(softcap=50.0), dict(softcap=1000.0),
+                                dict(slopes=None)], ids=str)
+def test_the_largest_weight_is_not_rounded(kv4, dtype, D, nq, kw):
+    """One token, late, scores up to 6 powers of two above all others, and only
+    it has a value.  Weights are relative to the largest, whose weight is 1 to
+    2^-20 whatever came before it: times its scale, a number of the type, it is
+    exact, and what is left of the reference's bound is the result's one rounding
+    and the scores' errors.  (fp16: relative to the largest weight times scale,
+    which is 2^14 then.  A token whose score is D lower and whose scale is more
+    than e^D times as large has the larger one; the late token's is 2^14 times
+    any number below 1 then, and rounded like every other: such rows keep the
+    reference's bound.)"""
+    n, late, H, G = 400, 300, 2, 4
+    cache, tables, g = _setup([n], 16, H, D, dtype, D + nq)
+    k_codes, v_codes, k_scales, v_scales, k_levels, v_levels = cache
+    k_codes[:] = k_codes[:1, :, :1]
+    v_levels[:, 0] = 0
+    at = tables[0, late // 16], slice(None), late % 16
+    value = v_codes[at].clone()
+    v_codes[:] = 0  # of level 0
+    v_codes[at] = value
+    k_scales[:] = 1.0
+    k_scales[at] = 1.5
+    both = torch.stack((k_codes[0, :, 0] & 15, k_codes[0, :, 0] >> 4), -1).flatten(-2).long()
+    key = k_levels.float().gather(1, both)  # the same for all tokens of a head
+    score = 0.5 + 7.5 * torch.rand(nq, H, G, 1, generator=g)  # of every other token
+    q = (score * (key * D ** 0.5 / key.square().sum(-1, keepdim=True))[:, None])
+    q = q.reshape(nq, H * G, D).to(dtype)
+    if "slopes" in kw:
+        kw = dict(slopes=torch.full((H * G,), 1e-4))
+    want, want_lse, tol, lse_tol = sref.attend(q, cache, tables, [n], [nq], causal=False, **kw)
+    exact = torch.ones(nq, H, G, 1, dtype=torch.bool)
+    if dtype is F16:
+        cap = kw.get("softcap", math.inf)
+        above = [cap * torch.tanh(z / cap) if cap < math.inf else z for z in (1.5 * score, score)]
+        scale = v_scales[tables[0, :n // 16].long()].float()  # (blocks, heads, slots)
+        lead = scale.amax((0, 2)).log() - v_scales[at].float().log()
+        exact = above[0] - above[1] > lead.view(H, 1, 1) + 0.05  # (0.05: q is rounded)
+        assert nq == 1 or exact.float().mean() > 0.5
+    tol = tol - 1.01 * sref.ref.UNIT[dtype] * want.abs() * exact.reshape(nq, H * G, 1)
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    got, lse = kv4.attend(q.cuda(), dev, tables.cuda(), i32([n]), i32([0, nq]), causal=False,
+                          return_lse=True, **_gpu(kw))
+    err = (got.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"out off by {float((err / tol).max()):.3g}"
+    assert bool(((lse.cpu().double() - want_lse).abs() <= lse_tol).all())
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("nq", [1, 6, 260])
 @pytest.mark.parametrize("softcap", [1e-30, 1e-9, 256.0, 257.0, 3e4, 1e9, 1e30])
