@@ -756,7 +756,8 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
   const int64_t cols = p.cols();
   p.tiles_per_req = (int)((G + cols - 1) / cols);
   const int64_t tiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
-  p.whole = max_seq <= (p.wide ? kWideWhole * 32 : kWhole * 32 * p.waves);
+  p.whole = max_seq <= (p.wide ? kWideWhole * 32 : kWhole * 32 * p.waves) &&
+            tiles * c.heads < kMostThreads / (64 * p.waves);
   p.wgs = p.whole ? tiles * c.heads : (p.wide ? 1 : 2) * (int64_t)device_shape().cus;
   return p;
 }
@@ -821,7 +822,7 @@ int launch_kv4_attend(const fkc_kv4_cache& c, const Kv4Attend& x, void* ws, size
   // Weights of a head's items are summed in 32 bits.
   const int64_t most =
       kv4_most_weight(p.cols(), p.wide ? wide_tokens((int)c.D) : 32 * p.waves, G, x.max_seq);
-  if (p.wgs > INT32_MAX || x.T * G / p.cols() + x.R + 1 > INT32_MAX / most)
+  if (x.T * G / p.cols() + x.R + 1 > INT32_MAX / most)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   Args a{(const uint16_t*)x.q.p, x.q.token_stride, x.q.head_stride,
          (const uint8_t*)c.k_codes, (const uint8_t*)c.v_codes,

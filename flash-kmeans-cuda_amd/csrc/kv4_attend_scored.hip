@@ -1164,7 +1164,8 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
   p.tiles_per_req = (int)((G + cols - 1) / cols);
   p.ntiles = ragged ? T * G / cols + R + 1 : R * p.tiles_per_req;
   const int64_t len = std::min(max_seq, reach + (cols + G - 1) / G + 16);
-  p.whole = len <= (p.wide ? kWideWhole * 32 : kWhole * 32 * p.waves);
+  p.whole = len <= (p.wide ? kWideWhole * 32 : kWhole * 32 * p.waves) &&
+            p.ntiles * c.heads < kMostThreads / (64 * p.waves);
   p.wgs = p.whole ? p.ntiles * c.heads : (p.wide ? 1 : 2) * (int64_t)device_shape().cus;
   return p;
 }
@@ -1264,7 +1265,8 @@ int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const K
   static_assert(kItem <= kMostItem && Wide<64>::ITEM <= kMostItem &&
                 Wide<128>::ITEM <= kMostItem && Wide<256>::ITEM <= kMostItem, "");
   const int64_t gr = p.wide ? 32 : 32 * p.waves;
-  if (p.wgs > INT32_MAX || p.ntiles > INT32_MAX / (x.max_seq / gr + 2 + kMostItem))
+  if (p.ntiles > INT32_MAX / (x.max_seq / gr + 2 + kMostItem) ||
+      (!p.whole && p.ntiles >= kMostThreads / 64))  // (kv4_tiles_kernel: a wave each)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   // (of scores times 0 the masked ones would be NaN)
   const double scale = std::max(std::fabs((double)x.sm_scale) * 1.4426950408889634, 1e-30);

@@ -61,6 +61,10 @@ constexpr int kEntry = 256;                // bytes of a table entry
 constexpr int kTable = 256 * kEntry;
 constexpr int kJoin = 8 * 16 * 8;          // maxima and sums of up to 8 waves
 
+// Threads of a launch stay below this; more workgroups of whole items than that
+// leaves room for become shares.
+constexpr int64_t kMostThreads = (int64_t)1 << 32;
+
 // 1 / l for a sum of weights, 0 where nothing was seen; NaN stays.
 __device__ inline float inverse(float l) { return l != 0.f ? 1.f / l : 0.f; }
 

@@ -341,6 +341,25 @@ def test_many_requests(kv4, ragged, long):
     _check(kv4, cache, tables, q, seq, nq, decode=not ragged, slopes=_slopes(2), window=1500)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=20.0), dict(window=7)], ids=str)
+def test_more_short_contexts_than_a_launch_has_workgroups(kv4, kw):
+    """65600 requests of 128 heads: a workgroup of 512 threads each would be 2^32
+    threads, so they go in shares.  An item's few tokens are one granule, which
+    no share cuts: the answer is that of fewer requests, bit for bit."""
+    H, D, R, few = 128, 64, 65600, 8
+    seq = [1, 16, 7, 0, 9, 16, 3, 12]
+    cache, tables, g = _setup(seq, 16, H, D, BF16, 3)
+    q = torch.randn(few, H, D, generator=g).to(BF16)
+    want = (_check(kv4, cache, tables, q, seq, [1] * few, decode=True, **kw) if kw else
+            kv4.attend(q.cuda(), kv4.Cache(*(t.cuda() for t in cache)), tables.cuda(), i32(seq)))
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    many = R // few
+    args = q.cuda().repeat(many, 1, 1), dev, tables.cuda().repeat(many, 1), i32(seq * many)
+    for cu in None, i32(list(range(R + 1))):
+        out = kv4.attend(*args, cu, **kw)
+        assert torch.equal(out.view(many, few, H, D), want.expand(many, few, H, D))
+
+
 @pytest.mark.parametrize("dtype,D,G", [(BF16, 128, 4), (F16, 64, 1), (F16, 256, 2)])
 def test_rows_of_no_request_beside_cut_ones(kv4, dtype, D, G):
     """Steps padded to many times their queries: those rows are 0."""

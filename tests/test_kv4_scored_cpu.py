@@ -76,6 +76,34 @@ def test_workspace(scores):
     assert rc == 2 and "aligned" in msg
 
 
+@pytest.mark.parametrize("scores", [dict(), dict(softcap=30.0), dict(slopes=FAKE, window=7)])
+@pytest.mark.parametrize("D,waves", [(64, 8), (128, 8), (256, 4)])
+def test_no_launch_of_2_32_threads(scores, D, waves):
+    """Short contexts go to a workgroup each while their threads are below 2^32,
+    and to equal shares (which need a workspace) from there on."""
+    from flash_kmeans_cuda import _lib
+    heads = 128
+    c, x = _cache(num_blocks=8, heads=heads, D=D), _scores(**scores)
+
+    def need(rows):
+        if scores:
+            return _lib.lib.fkc_kv4_attend_scored_workspace_bytes(
+                ctypes.addressof(c), heads, rows, rows, 16, 1, ctypes.addressof(x))
+        return _lib.lib.fkc_kv4_attend_workspace_bytes(ctypes.addressof(c), heads, rows, rows, 16)
+
+    # tiles of offsets that are not known yet: one per request and one per 16 rows
+    most = (2 ** 32 // (64 * waves * heads)) * 16 // 17 - 2
+    assert need(most) == 0 and need(most * 17 // 16 + 8) > 0
+
+
+def test_too_many_tiles():
+    c = _cache(num_blocks=8, heads=1)
+    for scores in dict(softcap=30.0), dict(window=5):
+        rc, msg = _attend(_scores(**scores), H=1, T=1 << 27, R=1 << 27, max_seq=16, cache=c,
+                          ws=FAKE, nbytes=1 << 50)
+        assert rc == 4 and "too many rows" in msg
+
+
 def test_reference_masks():
     """Written out by hand: four queries at positions 2 .. 5 of six tokens."""
     def rows(**kw):
