@@ -315,7 +315,9 @@ int fkc_free_blocks(const int32_t* tables, int64_t table_stride, int64_t max_blo
 
 size_t fkc_kv4_fork_workspace_bytes(const fkc_kv4_cache* cache, int64_t F) {
   clear_error();
-  if (cache_ok(cache, "kv4_fork_workspace_bytes")) return 0;
+  if (cache_ok(cache, "kv4_fork_workspace_bytes") ||
+      alike(*cache, *cache, "kv4_fork_workspace_bytes"))
+    return 0;
   if (F < 0 || F > kI32) {
     fail(FKC_ERR_INVALID, "kv4_fork_workspace_bytes: F out of range");
     return 0;

@@ -92,6 +92,21 @@ def test_compact_and_copy_refusals():
     assert _call("fkc_kv4_copy_blocks", [h, FAKE, h, FAKE, 3, None], 4, 1)[0] == 4
 
 
+def test_forks_of_blocks_past_31_bits_are_refused_by_name():
+    """Blocks whose 16-byte units 32 bits do not count: the workspace's size is 0
+    and says why, as the call itself does."""
+    from flash_kmeans_cuda import _lib
+    for kw in (dict(num_blocks=1, heads=16384, block_size=1 << 12, D=64),
+               dict(num_blocks=1, heads=16384, block_size=1 << 20, D=256),
+               dict(num_blocks=0, heads=8192, block_size=1 << 20, D=256)):
+        c = _cache(**kw)
+        ref = ctypes.addressof(c)
+        assert _lib.lib.fkc_kv4_fork_workspace_bytes(ref, 5) == 0
+        assert "2^31" in _lib.last_error()
+        ok = [ref, FAKE, 8, 8, FAKE, 3, FAKE, 5, FAKE, 6, FAKE, FAKE, FAKE, FAKE, 1 << 40, None]
+        assert _call("fkc_kv4_fork", ok, 7, 5)[0] == 4
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_reference_forks_leave_every_row_its_own_last_block(seed):
     """After a fork no row ends in a block that another row holds, and every
