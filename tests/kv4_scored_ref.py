@@ -24,9 +24,9 @@ def seen(n, m, causal=True, window=None, starts=None, prefix=None):
 
 
 def attend(q, cache, tables, seq, nq, causal=True, sm_scale=None, max_seq=None, softcap=None,
-           slopes=None, window=None, starts=None, prefix_lens=None):
+           slopes=None, window=None, starts=None, prefix_lens=None, pick=None):
     """-> (out, lse, and the largest errors that the kernel's arithmetic allows
-    of both), float64.
+    of both), float64; of the rows pick (ascending) alone where it is given.
 
     Errors of a token's score in fp32, as a factor of its weight e^(1 + e_t):
       D products and sums, the key's scale and the score's:  (D + 12) 2^-24 |q| |k|
@@ -60,6 +60,10 @@ def attend(q, cache, tables, seq, nq, causal=True, sm_scale=None, max_seq=None, 
         rows = slice(row, row + m)
         ok = seen(n, m, causal, window, None if starts is None else starts[rows].long(),
                   None if prefix_lens is None else int(prefix_lens[r]))
+        pos = torch.arange(n - m, n)
+        if pick is not None:
+            rows = torch.tensor([i for i in pick if row <= i < row + m], dtype=torch.long)
+            ok, pos = ok[rows - row], pos[rows - row]
         t = torch.arange(n)
         blk = tables[r, t // bs].long() if n else t
         ok &= ((blk >= 0) & (blk < num_blocks))[None, :]
@@ -68,7 +72,7 @@ def attend(q, cache, tables, seq, nq, causal=True, sm_scale=None, max_seq=None, 
             continue
         some = ok.any(0)
         t, blk, ok = t[some], blk[some], ok[:, some]
-        away = (torch.arange(n - m, n)[:, None] - t[None, :]).abs().double()
+        away = (pos[:, None] - t[None, :]).abs().double()
         alive = ok.any(1)
         for h in range(heads):
             k = ref.held(k_codes, k_scales, k_levels, blk, t % bs, h)
@@ -99,3 +103,56 @@ def attend(q, cache, tables, seq, nq, causal=True, sm_scale=None, max_seq=None, 
                 lse_tol[rows, g] = mean[:, 0] + 2.0 ** -21 + torch.where(
                     alive, top[:, 0].abs(), 0.0) * 2.0 ** -22
     return out, lse, tol, lse_tol
+
+
+# Prompts whose work per workgroup is many groups of 32 tokens and several items:
+# (dtype, D, heads, query heads per head, block size, tokens, queries).
+LONG_PROMPTS = [
+    (torch.bfloat16, 64, 7, 4, 32, [3100, 1500, 2700], [3100, 1500, 1100]),
+    (torch.float16, 128, 9, 3, 16, [2900, 1300, 3300], [2900, 1300, 900]),
+    (torch.bfloat16, 256, 7, 5, 48, [3000, 1100, 2300], [3000, 1100, 1000])]
+LONG_OPTIONS = [("cap",), ("slopes", "prefix"), ("window",), ("docs",),
+                ("cap", "slopes", "window", "docs", "prefix")]
+LONG_WINDOW, LONG_DOCUMENTS = 1700, 2000
+
+
+def replay(D, heads, G, seq, nq, cus, causal=True, window=None, starts=None, prefix_lens=None):
+    """The shares that the form for prompts cuts its work into, as lists of
+    (head, tile, first token, last token, whether the item goes on in the next
+    share): csrc/kv4_attend_scored.hip's walk over tiles of 16 rows a wave."""
+    cols, overhead = (192 if D == 256 else 256), (10 if D == 64 else 6)
+    tiles, row = [], 0
+    for r, (n, m) in enumerate(zip(seq, nq)):
+        p = torch.arange(n - m, n)
+        last = torch.full((m,), n) if not causal else (p + 1).clamp(
+            min=0 if prefix_lens is None else int(prefix_lens[r])).clamp(0, n)
+        first = torch.zeros(m, dtype=torch.long)
+        if window is not None:
+            first = (p - window + 1).clamp(min=0)
+        if starts is not None:
+            first = torch.maximum(first, starts[row:row + m].long())
+        for col in range(0, m * G, cols):
+            i = slice(col // G, (min(col + cols, m * G) - 1) // G + 1)
+            some = first[i] < last[i]
+            lo = int(first[i][some].min()) // 16 * 16 if bool(some.any()) else 0
+            hi = int(last[i][some].max()) if bool(some.any()) else 0
+            tiles.append((lo, hi, overhead + -(-(hi - lo) // 32) if hi > lo else 2))
+        row += m
+    items = [(h, t, *tile) for h in range(heads) for t, tile in enumerate(tiles)]
+    total = sum(x[4] for x in items)
+    share = max(-(-total // cus), 2)
+    shares, at, x = [], 0, 0
+    while x < len(items):
+        left, mine = share, []
+        while left and x < len(items):
+            h, t, lo, hi, n = items[x]
+            end = min(n, at + left)
+            token = [hi if a == n else min(lo + max(a - overhead, 0) * 32, hi) for a in (at, end)]
+            if token[0] < token[1] or (lo == hi and end == n):
+                mine.append((h, t, *token, token[1] < hi))
+            left -= end - at
+            at = end
+            if end == n:
+                x, at = x + 1, 0
+        shares.append(mine)
+    return shares

@@ -140,6 +140,39 @@ def test_prompts_in_shares(kv4, dtype, D, heads, G, bs, names):
     _check(kv4, cache, tables, q, seq, nq, **kw)
 
 
+@pytest.mark.parametrize("shape", sref.LONG_PROMPTS, ids=lambda s: str(s[1]))
+@pytest.mark.parametrize("names", sref.LONG_OPTIONS, ids=_id)
+def test_long_shares_of_prompts(kv4, shape, names):
+    """Workgroups whose shares are several items, of one head and of two, cut at
+    either end, and items of more than 1024 tokens; blocks missing all over them.
+    A sample of the rows, every head."""
+    dtype, D, heads, G, bs, seq, nq = shape
+    cache, tables, g = _setup(seq, bs, heads, D, dtype, D)
+    tables[0, 3] = -1
+    tables[0, 1100 // bs:1200 // bs] = -1
+    tables[0, 2100 // bs] = 2 ** 31 - 1
+    tables[2, 2000 // bs:2064 // bs] = cache[0].shape[0]
+    q = (1.5 * torch.randn(sum(nq), heads * G, D, generator=g)).to(dtype)
+    kw = _options(names, seq, nq, heads * G, D, window=sref.LONG_WINDOW,
+                  mean=sref.LONG_DOCUMENTS)
+    rng = random.Random(D)
+    first = np.concatenate([[0], np.cumsum(nq)]).tolist()
+    pick = sorted({x for a, b in zip(first, first[1:]) for x in (
+        a, a + 15, a + 16, b - 17, b - 1, *rng.sample(range(a, b), 25))})
+    want, want_lse, tol, lse_tol = (x[pick] for x in sref.attend(q, cache, tables, seq, nq,
+                                                                 pick=pick, **kw))
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    args = q.cuda(), dev, tables.cuda(), i32(seq), i32(first)
+    out = torch.full_like(args[0], math.nan)
+    _, lse = kv4.attend(*args, out=out, return_lse=True, **_gpu(kw))
+    assert bool(torch.isfinite(out).all())
+    err = (out.cpu().double()[pick] - want).abs()
+    assert bool((err <= tol).all()), f"out off by {float((err / tol.clamp(min=1e-30)).max()):.3g}"
+    err = (lse.cpu().double()[pick] - want_lse).abs()
+    assert bool((err <= lse_tol).all()), f"lse off by {float((err / lse_tol).max()):.3g}"
+    assert torch.equal(out, kv4.attend(*args, **_gpu(kw)))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("bs", [16, 48, 256])
 @pytest.mark.parametrize("names", OPTIONS, ids=_id)

@@ -126,3 +126,30 @@ def test_reference_is_plain_attention_with_nothing_set():
     a = ref.attend(q, cache, tables, [20, 31], [2, 4])
     b = sref.attend(q, cache, tables, [20, 31], [2, 4])
     assert torch.allclose(a[0], b[0], atol=1e-12) and torch.allclose(a[1], b[1], atol=1e-12)
+
+
+@pytest.mark.parametrize("shape", sref.LONG_PROMPTS, ids=lambda s: str(s[1]))
+@pytest.mark.parametrize("names", sref.LONG_OPTIONS, ids="+".join)
+def test_long_prompts_fill_their_shares(shape, names):
+    """What the test of long shares is for: at 256 compute units shares hold more
+    than one item, of two heads too, items of more than 1024 tokens, and cut
+    items behind whole ones."""
+    from test_gpu_kv4_scored import _options
+    dtype, D, heads, G, bs, seq, nq = shape
+    kw = _options(names, seq, nq, heads * G, D, window=sref.LONG_WINDOW, mean=sref.LONG_DOCUMENTS)
+    for unused in "softcap", "slopes":
+        kw.pop(unused, None)
+    shares = sref.replay(D, heads, G, seq, nq, 256, **kw)
+    with_tokens = [[x for x in s if x[2] < x[3]] for s in shares]
+    assert sum(len(s) > 1 for s in with_tokens) > 100
+    assert sum(len({x[0] for x in s}) > 1 for s in with_tokens) >= min(heads - 1, 5)
+    assert sum(any(x[3] - x[2] > 1024 for x in s) for s in with_tokens) > 20
+    assert sum(len(s) > 1 and s[-1][4] for s in with_tokens) > 50
+    # every item's tokens once
+    for h in range(heads):
+        covered = {}
+        for s in shares:
+            for head, tile, a, b, more in s:
+                if head == h:
+                    assert covered.get(tile, a) == a
+                    covered[tile] = b
