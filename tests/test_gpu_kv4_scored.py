@@ -550,6 +550,30 @@ def test_offsets_that_do_not_ascend_end(kv4):
             assert out.shape == q.shape
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(softcap=9.0), dict(window=50)], ids=str)
+def test_rows_that_one_request_names_are_its_own(kv4, kw):
+    """Offsets that do not ascend: rows that a single request names are its
+    answer, rows past the last offset are 0, and what nothing else is named by
+    is not left as it was."""
+    seq = [3000, 40, 900]
+    cache, tables, g = _setup(seq, 16, 1, 64, BF16, 4)
+    q = torch.randn(600, 4, 64, generator=g).to(BF16)
+    dev = kv4.Cache(*(t.cuda() for t in cache))
+    # rows 100 .. 499 belong to the first and the last request
+    want, want_lse, tol, lse_tol = sref.attend(q, cache, tables, seq, [500, 0, 100], **kw)
+    own = [*range(100), *range(500, 600)]
+    out = torch.full((600, 4, 64), math.nan, dtype=BF16, device="cuda")
+    _, lse = kv4.attend(q.cuda(), dev, tables.cuda(), i32(seq), i32([0, 500, 100, 600]), out=out,
+                        return_lse=True, **kw)
+    assert bool(((out.cpu().double() - want).abs() <= tol)[own].all())
+    assert bool(((lse.cpu().double() - want_lse).abs() <= lse_tol)[own].all())
+    assert bool(torch.isfinite(out).all())
+    out.fill_(math.nan)
+    _, lse = kv4.attend(q.cuda(), dev, tables.cuda(), i32(seq), i32([7, 7, 7, 7]), out=out,
+                        return_lse=True, **kw)
+    assert not bool(out[7:].any()) and bool((lse[7:] == -math.inf).all())
+
+
 def test_strided_queries_and_another_stream(kv4):
     seq, nq = [300, 90], [70, 90]
     cache, tables, g = _setup(seq, 16, 2, 64, F16, 7)
