@@ -1134,7 +1134,15 @@ kv4_masked_wide_kernel(const MArgs margs) {
   }
 }
 
-// As for kv4_attend.hip; a window bounds what a tile of a causal call sees.
+// Granules of a share at least, and up to how many granules a context is never
+// cut, as for kv4_attend.hip; a window bounds what a tile of a causal call sees.
+// (Capped, bf16, 8 heads of 4 query heads, us whole / cut.  One query of 1, 8 or
+// 64 requests: D = 128, 1536 tokens 16.9 / 16.8, 17.4 / 19.6, 27.0 / 30.4, 3000 tokens
+// 25.8 / 18.2, 26.7 / 23.4, 43.4 / 45.0; D = 256, 777 tokens 21.1 / 17.0, 21.2 / 19.1,
+// 28.5 / 30.9, 1536 tokens 29.8 / 20.0, 30.6 / 23.9, 41.0 / 42.3.  1, 4 or 16 prompts:
+// D = 128, 512 tokens 38 / 38, 43 / 65, 132 / 111, 1024 tokens 65 / 54, 120 / 115,
+// 376 / 349; D = 256, 1024 tokens 93 / 105, 211 / 221, 728 / 724, 2048 tokens 220 / 199,
+// 638 / 609, 2276 / 2220.)
 constexpr int kMinShare = 2, kWhole = 8, kWideWhole = 32;
 
 struct Plan {
@@ -1149,6 +1157,8 @@ struct Plan {
 };
 
 constexpr int wide_waves(int D) { return D == 256 ? 12 : 16; }
+// Columns of an average request up to which the split form is taken.
+constexpr int wide_from(int D) { return D == 64 ? 352 : D == 128 ? 448 : 288; }
 constexpr int waves_of(int D) { return D == 256 ? 4 : 8; }
 
 // reach: tokens that one query sees at most (max_seq, or the window).
@@ -1156,8 +1166,17 @@ Plan make_plan(const fkc_kv4_cache& c, int64_t H, int64_t T, int64_t R, int64_t 
                int64_t reach, bool ragged) {
   Plan p;
   const int64_t G = H / c.heads;
+  // By the columns of an average request.  Measured on 8 requests of 4096 tokens, 8
+  // heads of 4 query heads, bf16, capped, us with one tile per workgroup / with two /
+  // in the wide form, for so many columns each (slopes and masks the same within
+  // 10%, and better in the wide form by 5 to 20% at D = 64):
+  //   D =  64     64: 39 / 39 / 44     96: 47 / 42 / 52     256: 82 / 71 / 88
+  //              320: 106 / 95 / 106  384: 118 / 110 / 105  512: 153 / 130 / 106
+  //   D = 128     64: 48 / 48 / 64     96: 59 / 53 / 74     256: 106 / 88 / 115
+  //              384: 155 / 139 / 148 512: 203 / 160 / 147
+  //   D = 256     96: 94 / - / 144    256: 182 / - / 234    320: 247 / - / 236
   const int64_t avg = R > 0 ? T * G / R : 0;
-  p.wide = avg > (c.D == 256 ? 224 : 448);
+  p.wide = avg > wide_from((int)c.D);
   p.nt = p.wide ? 1 : c.D < 256 && avg > 64 ? 2 : 1;
   p.waves = p.wide ? wide_waves((int)c.D) : p.nt == 2 ? 4 : waves_of((int)c.D);
   const int64_t cols = p.cols();

@@ -128,6 +128,20 @@ def test_several_queries(kv4, dtype, D, heads, G, bs, causal, names):
     _check(kv4, cache, tables, q, seq, nq, causal=causal, **kw)
 
 
+@pytest.mark.parametrize("D,columns", [(64, 352), (128, 448), (256, 288)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("names", [("cap",), ("slopes", "window"), ("docs", "prefix")], ids=_id)
+def test_either_side_of_the_forms_border(kv4, dtype, D, columns, names):
+    """The most columns of the form for few of them, and the fewest of the one
+    for prompts; whole and in shares."""
+    for seq in [400, 500], [3000, 1500]:
+        for m in columns // 4, columns // 4 + 1:
+            cache, tables, g = _setup(seq, 32, 1, D, dtype, D + m)
+            q = torch.randn(2 * m, 4, D, generator=g).to(dtype)
+            _check(kv4, cache, tables, q, seq, [m, m],
+                   **_options(names, seq, [m, m], 4, D, window=200, mean=150))
+
+
 @pytest.mark.parametrize("dtype,D,heads,G,bs", [
     (BF16, 128, 1, 4, 32), (F16, 64, 2, 2, 48), (F16, 256, 1, 2, 64), (BF16, 256, 1, 3, 16)])
 @pytest.mark.parametrize("names", OPTIONS, ids=_id)

@@ -96,6 +96,23 @@ def test_no_launch_of_2_32_threads(scores, D, waves):
     assert need(most) == 0 and need(most * 17 // 16 + 8) > 0
 
 
+@pytest.mark.parametrize("D,columns", [(64, 352), (128, 448), (256, 288)])
+def test_the_forms_border(D, columns):
+    """Up to so many columns of an average request the form for few of them is
+    taken, whose parts are narrower: what the measurements beside the plan say."""
+    from flash_kmeans_cuda import _lib
+    c, x = _cache(num_blocks=1 << 12, D=D, heads=1), _scores(softcap=30.0)
+
+    def parts(m):
+        return _lib.lib.fkc_kv4_attend_scored_workspace_bytes(
+            ctypes.addressof(c), 4, 8 * m, 8, 40000, 1, ctypes.addressof(x))
+
+    # (the list of tiles grows with them, by less than a hundredth)
+    assert parts(columns // 4) < 1.01 * parts(columns // 5)
+    assert parts(columns // 4 + 1) > 3 * parts(columns // 4)
+    assert parts(columns // 2) < 1.01 * parts(columns // 4 + 1)
+
+
 def test_too_many_tiles():
     c = _cache(num_blocks=8, heads=1)
     for scores in dict(softcap=30.0), dict(window=5):
