@@ -10,10 +10,13 @@
 // last token is masked element by element.
 //
 // A tile's products are those of kv4_attend.hip.  The tanh is 1 - 2 / (1 + e^2x):
-// one exponential, one reciprocal, and nothing to tell apart for small or large x;
-// off by a few units in the last place of 1, which a cap of 50 makes 5e-5 of a
-// score at most (large caps: sharp_tanh).  Scores are in powers of two from there
-// on, so a weight is 2^(z - m).
+// one exponential, one reciprocal, and nothing to tell apart for small or large x.
+// It is off by units in the last place of 1, not of itself: with one unit (2^-23)
+// each of exponential and reciprocal and the sum rounded by half of one, by
+// 1.5 * 2^-22 at most, so a score by 2^-21 of the cap, however small the score
+// (measured: 2^-21.5; a cap of 50: 2.4e-5, where rounding a weight near 1 to fp16
+// is 4.9e-4; large caps: sharp_tanh).  Scores are in powers of two from there on,
+// so a weight is 2^(z - m).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -316,7 +319,7 @@ __device__ inline float exponent_of(float scale) {
 }
 
 // tanh x of e = 2 log2(e) x within 2^-18 of itself: for |x| < 0.35 the series, whose
-// first term left out is 2^-22 of it, and 1 - 2 / (1 + 2^e), off by 2^-20 of 1,
+// first term left out is 2^-22 of it, and 1 - 2 / (1 + 2^e), off by 2^-21 of 1,
 // beyond.
 __device__ inline float sharp_tanh(float e) {
   const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(e));
@@ -380,7 +383,8 @@ struct MState : State<DT, D, NT> {
 #pragma unroll
         for (int i = 0; i < 4; ++i) z[y][j][i] *= ks[j][i];
       // (WIDE: the wide form, where asking as it runs is the faster way: prefixes under
-      // slopes 699 us, without the question 737.  Drafts 93.4, with it 94.9.)
+      // slopes 702 us, without the question 737, registers being given out otherwise.
+      // Drafts 93.4, with it 94.9.)
       if (capped(MODE) || (WIDE && MODE == kBias && cap2 != 0.f)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -562,9 +566,9 @@ __device__ inline const MArgs& arguments() { return arguments_as<MArgs>(); }
 //
 // Bound by memory where contexts are long: one query of each of 64 ragged requests
 // that look back over 4096 tokens, 435 MB of bf16 cache (D = 256, 8 heads of 2
-// capped), takes 92 us, 4.7 TB/s, where a large copy moves 4.6 and reading alone
-// 6.4.  Drafts of 2 to 7 tokens under slopes (fp16, D = 128, 4 heads of 8, contexts of
-// 300 to 65536, 175 MB) take 76 us: tiles of 16 columns look the same codes up 2.75
+// capped), takes 97 us (89 at least), 4.5 TB/s, where a large copy moves 4.6 and
+// reading alone 6.4.  Drafts of 2 to 7 tokens under slopes (fp16, D = 128, 4 heads of 8,
+// contexts of 300 to 65536, 175 MB) take 77 us: tiles of 16 columns look the same codes up 2.75
 // times, 128 look-ups a tile of 32 tokens, beside ~230 vector and 16 matrix
 // operations.  (Two tiles a wave look up half as often with half the waves: the
 // same.)
@@ -814,17 +818,26 @@ kv4_masked_split_kernel(const MArgs margs) {
 // a SIMD 64 vector operations take 310 ns, 16 exponentials 233, 16 products 476, the
 // first two together 543, the first and the last 696, all 862.  A group's 256
 // capped columns (D = 128) are 16 products, 24 exponentials and reciprocals and
-// ~95 others a wave, 1.3 us by that sum, and take 1.6: ragged prompts of 900 to 5600
-// tokens, 32 heads of 128 columns, bf16, 650 us (0.59 PFLOP/s).  Prefixes with
-// slopes, D = 256, 2000 to 5000 tokens, 659 us (0.55 PFLOP/s); documents of 700
-// tokens in requests of 9000 and 16000, fp16, D = 64, 163 us, a third of it what an
+// ~95 others a wave, 1.3 us by that sum, and take 1.65: ragged prompts of 900 to 5600
+// tokens, 32 heads of 128 columns, bf16, 676 us (0.57 PFLOP/s).  Prefixes with
+// slopes, D = 256, 2000 to 5000 tokens, 662 us (0.55 PFLOP/s) with the vector unit 41%
+// and the matrix cores 24% busy: the waves wait 60% of their cycles.  Documents of 700
+// tokens in requests of 9000 and 16000, fp16, D = 64, 172 us, a third of it what an
 // item costs by itself, the rest waves whose columns see nothing of a stage beside
-// others' that do.  What was measured (us): two waves a SIMD of two tiles each with
-// the scores of one group beside the weights of the last 770 (capped), with three
-// and four waves a SIMD of one tile 751, without each wave converting the scales
-// and with one operation less a weight 673, items weighed right 650.  Steps of 64
-// tokens a wave are no faster (D = 64), or spill (D = 128); nor is an item's first
-// stage loaded and filled during the last one's.
+// others' that do.  What was measured while a maximum could lag behind, 5% less of
+// everything (us): two waves a SIMD of two tiles each with the scores of one group
+// beside the weights of the last 770 (capped), with three and four waves a SIMD of
+// one tile 751, without each wave converting the scales and with one operation less
+// a weight 673, items weighed right 650.  Nor is an item's first stage loaded and
+// filled during the last one's, no faster.
+//
+// Four waves a SIMD leave 128 registers (D = 256: three, 168), and the compiler
+// spills: of D = 64 none or two, of D = 128 14 to 18, with slopes 26 and 33, of
+// D = 256 30 to 40.  Most of them are stored and read once an item.  In the loop over
+// groups stand three (masks alone) or four reads of scratch memory at D = 256, and in
+// that over stages two at D = 128 with slopes, none without; such a read comes back
+// behind the codes that are on their way for the next stage.  Steps of 64 tokens a
+// wave are no faster at D = 64, and spill more at D = 128.
 //
 // Feature row n of fragment d of the second product is feature 32 (d / 2) + 2 n +
 // d % 2: the two codes of one byte go to two fragments, and 16 lanes read 16
@@ -835,8 +848,8 @@ struct Wide {
   static constexpr int COLS = 16 * WAVES, THREADS = WAVES * 64;
   static constexpr int KS = D / 32, ND = D / 16;
   static constexpr int G = 256 / D;           // groups of a stage
-  // Groups that an item costs by itself (us with 4 / 6 / 9: capped prompts 668 / 650 /
-  // 666, prefixes 693 / 690 / 692; documents with 7 / 10: 187 / 182).
+  // Groups that an item costs by itself (us with 4 / 6 / 9: capped prompts 713 / 690 /
+  // 696, prefixes 704 / 702 / 705; documents with 7 / 10 / 14: 191 / 188 / 188).
   static constexpr int ITEM = D == 64 ? 10 : 6;
   static constexpr int RUN = G * 32 * D * 2;  // bytes of a stage's keys or values
   static constexpr int BUF = 2 * RUN;         // keys, then values
@@ -1269,9 +1282,10 @@ size_t kv4_attend_scored_workspace_bytes(const fkc_kv4_cache& c, int64_t H, int6
   return p.whole ? 0 : Scratch(nullptr, c, p).bytes;
 }
 
-// Caps above this take kBoth, with slopes of 0: kCap's tanh is off by 2^-20 of the cap,
-// 2^-12 of a weight here, half of a step of fp16.  Prompts capped at 30 take 660 us
-// with kCap and 953 with the series, single tokens 13.4 and 14.6.
+// Caps above this take kBoth, with slopes of 0: kCap's tanh is off by 2^-21 of the cap,
+// 2^-13 of a weight here, a quarter of what rounding one to fp16 may cost.  Prompts
+// capped at 30 take 690 us with kCap and 951 with the series, single tokens 13.4 and
+// 14.6.
 constexpr float kSharp = 256.f;
 
 int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const Kv4Scores& sc,

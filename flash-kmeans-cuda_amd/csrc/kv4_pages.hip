@@ -124,6 +124,9 @@ names_small_kernel(const Rows t, uint32_t num_blocks, int32_t* __restrict__ list
 // the number of a held entry that names this block.  Bound by latency: 2048 rows of
 // up to 1024 entries over 470000 blocks take 5.4 + 5.0 + 3.4 us for marking,
 // counting and listing (a byte per block, cleared first, 2.2 + 4.6 + 2.4 + 4.5).
+// Every workgroup of the last adds up the counts of all, which grows with the square
+// of the blocks: a call over 2^20 / 2^22 / 2^24 / 2^26 of them takes 47 / 68 / 165 /
+// 1215 us, of which writing the list is 60 at most.
 __global__ void __launch_bounds__(PT)
 mark_kernel(const Rows t, uint32_t num_blocks, uint32_t* __restrict__ entry) {
   const int parts = (t.width + ENTRIES - 1) / ENTRIES;
@@ -520,7 +523,9 @@ fork_few_kernel(const Rows t, const int32_t* __restrict__ parents, int F, uint32
   if (b >= 0) data.store(store, (uint32_t)b, p);
 }
 
-// Any number of children: one workgroup finds them, with the lowest child that
+// Any number of children: one workgroup finds them (a call with 1024 children of 512
+// rows takes 21 us with the kernel above; 1025 / 4000 / 20000 / 200000 / 10^6 here
+// 26 / 43 / 139 / 1239 / 6430, ~6 ns a child), with the lowest child that
 // ends in a block in `first`.
 constexpr int FT = 1024;
 __global__ void __launch_bounds__(FT)

@@ -334,7 +334,9 @@ def attend(q: torch.Tensor, cache: Cache, tables: torch.Tensor, seq_lens: torch.
 
     Scores and masks of other models, any of them together, for a query at
     position p of its request and a token at t:
-      softcap      a score z becomes softcap * tanh(z / softcap), 1e-30 <= softcap <= 1e30;
+      softcap      a score z becomes softcap * tanh(z / softcap), 1e-30 <= softcap <= 1e30
+                   (off by up to 2^-21 of the cap; of caps above 256, and of any beside
+                   slopes, by 2^-18 of the score);
       slopes       (H,) float32: slopes[h] * |p - t| is taken off it, after the cap;
       window       no token more than window - 1 positions back is seen: t > p - window;
       starts       (T,) int32, no token before starts[row] is seen: the first token of

@@ -466,9 +466,11 @@ FKC_CAPI int fkc_kv4_attend(const fkc_kv4_cache* cache, const void* q,
  * softcap 0 or 1e-30 to 1e30; slopes (H) fp32, finite; window >= 0, below 2^31;
  * starts (T) and prefix_lens (R) int32 of any values.  A row whose first is not
  * below its last sees nothing.  Scores are fp32; the distance is exact below
- * 2^24 and rounded beyond.  With a softcap or slopes a key's scale times
- * 3 |sm_scale| / softcap or 1.5 |sm_scale| has to stay below 2^128; values whose
- * scale is not finite count where they have a weight above 0.
+ * 2^24 and rounded beyond; a capped score is off by up to 2^-21 of the cap, of caps
+ * above 256 and of any beside slopes by 2^-18 of the score.  With a softcap or
+ * slopes a key's scale times 3 |sm_scale| / softcap or 1.5 |sm_scale| has to stay
+ * below 2^128; values whose scale is not finite count where they have a weight
+ * above 0.
  */
 typedef struct fkc_kv4_scores {
   float softcap;
