@@ -444,10 +444,12 @@ def fork(cache: Cache, tables: torch.Tensor, seq_lens: torch.Tensor, parents: to
     child needs its own: the first child that ends in a block keeps it, unless
     another has it as a whole one, and every other child's becomes the next of
     free_blocks, with a copy of what the block holds.  taken (1) int32 counts
-    the copies; where free_blocks does not reach, a child's entry is -1.  Rows
-    that no child goes on from give their blocks back (`free_blocks` of the new
-    tables).  After a cut (a smaller length) into blocks that other rows hold
-    too, fork all rows onto themselves before anything is appended.
+    the copies; where free_blocks does not reach, a child's entry is -1.  It
+    names no block twice and none that a child goes on from: what such blocks
+    hold afterwards is not defined.  Rows that no child goes on from give their
+    blocks back (`free_blocks` of the new tables).  After a cut (a smaller
+    length) into blocks that other rows hold too, fork all rows onto themselves
+    before anything is appended.
     """
     dev = cache.device
     seq_lens = _i32("seq_lens", seq_lens, 1, dev)

@@ -521,6 +521,8 @@ FKC_CAPI int fkc_free_blocks(const int32_t* tables, int64_t table_stride,
  * block, codes and scales.  taken (1): such copies; where free_blocks does not
  * reach, or names no block, the child's entry is -1.  tables and seq_lens are
  * not written.  What rows that are no child's parent hold is not looked at.
+ * free_blocks names no block twice and none that a child goes on from: what such
+ * blocks hold afterwards is not defined.
  */
 FKC_CAPI size_t fkc_kv4_fork_workspace_bytes(const fkc_kv4_cache* cache, int64_t F);
 FKC_CAPI int fkc_kv4_fork(const fkc_kv4_cache* cache, const int32_t* tables,
