@@ -1299,7 +1299,7 @@ int launch_kv4_attend_scored(const fkc_kv4_cache& c, const Kv4Attend& x, const K
                 Wide<128>::ITEM <= kMostItem && Wide<256>::ITEM <= kMostItem, "");
   const int64_t gr = p.wide ? 32 : 32 * p.waves;
   if (p.ntiles > INT32_MAX / (x.max_seq / gr + 2 + kMostItem) ||
-      (!p.whole && p.ntiles >= kMostThreads / 64))  // (kv4_tiles_kernel: a wave each)
+      (!p.whole && p.ntiles + 3 >= kMostThreads / 64))  // (kv4_tiles_kernel: a wave each)
     return fail(FKC_ERR_UNSUPPORTED, "kv4_attend: too many rows times tokens");
   // (of scores times 0 the masked ones would be NaN)
   const double scale = std::max(std::fabs((double)x.sm_scale) * 1.4426950408889634, 1e-30);

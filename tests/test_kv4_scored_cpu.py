@@ -113,6 +113,20 @@ def test_the_forms_border(D, columns):
     assert parts(columns // 2) < 1.01 * parts(columns // 4 + 1)
 
 
+@pytest.mark.parametrize("requests", [(1 << 26) - 4, (1 << 27) - 1])
+def test_a_launch_that_weighs_tiles_has_a_wave_for_each(requests):
+    """Of 64 threads, four to a workgroup: 2^26 - 4 tiles fill 2^24 workgroups of
+    256, one launch too many."""
+    c = _cache(num_blocks=8, heads=1)
+    for scores in dict(softcap=30.0), dict(window=5):
+        rc, msg = _attend(_scores(**scores), H=1, T=requests * 0, R=requests, cu=FAKE, max_seq=16,
+                          cache=c, ws=FAKE, nbytes=1 << 50)
+        assert rc == 0  # nothing to do
+        rc, msg = _attend(_scores(**scores), H=1, T=1, R=requests, cu=FAKE, max_seq=16,
+                          cache=c, ws=FAKE, nbytes=1 << 50)
+        assert rc == 4 and "too many rows" in msg
+
+
 def test_too_many_tiles():
     c = _cache(num_blocks=8, heads=1)
     for scores in dict(softcap=30.0), dict(window=5):
