@@ -669,6 +669,46 @@ def test_lloyd_iteration_captures_into_a_graph():
         state = e_c
 
 
+def test_lloyd_iterations_captured_and_ordered():
+    """As above, the stream waiting for what the default one writes before each
+    call (the streams are not ordered by themselves: a copy into the centroids
+    may otherwise land behind the iteration), over three iterations."""
+    from flash_kmeans_cuda import _lib, synth
+    L = _lib.lib
+    cfg = synth.CONFIGS["c2"]
+    x_np, init_np = synth.make(cfg, N=16384)
+    x, state = synth.to_torch(x_np, "f16"), synth.to_torch(init_np, "f16")
+    B, N, K, D = 1, 16384, cfg.K, cfg.D
+    dt = _lib.dtype_code(x.dtype)
+    ws = _lib.workspace(L.fkc_kmeans_workspace_bytes(B, N, K, D, dt, 3), x.device)
+    cents, ids = state.clone(), torch.empty((B, N), dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+
+    def three():
+        _lib.check(L.fkc_kmeans_lloyd(x.data_ptr(), cents.data_ptr(), ids.data_ptr(), B, N, K,
+                                      D, dt, 3, 0.0, ws.data_ptr(), ws.numel(),
+                                      s.cuda_stream, None, None), "kmeans_lloyd")
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        three()
+    for rep in range(4):
+        got = []
+        for run in three, g.replay:
+            cents.copy_(state)
+            ids.fill_(-1)
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                run()
+            torch.cuda.current_stream().wait_stream(s)
+            got.append((cents.clone(), ids.clone()))
+        assert torch.equal(got[0][0], got[1][0]), f"replay {rep}: centroids"
+        assert torch.equal(got[0][1], got[1][1]), f"replay {rep}: labels"
+        assert rep > 0 or not torch.equal(got[0][0], state)  # (later ones may have converged)
+        state = got[0][0]
+
+
 _FIRST_CALL_CAPTURED = r'''
 import sys, torch
 sys.path.insert(0, sys.argv[1])
