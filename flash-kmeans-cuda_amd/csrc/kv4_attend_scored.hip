@@ -828,8 +828,8 @@ kv4_masked_split_kernel(const MArgs margs) {
 // everything (us): two waves a SIMD of two tiles each with the scores of one group
 // beside the weights of the last 770 (capped), with three and four waves a SIMD of
 // one tile 751, without each wave converting the scales and with one operation less
-// a weight 673, items weighed right 650.  Nor is an item's first stage loaded and
-// filled during the last one's, no faster.
+// a weight 673, items weighed right 650; an item's first stage loaded and filled
+// during the last one's no faster.
 //
 // Four waves a SIMD leave 128 registers (D = 256: three, 168), and the compiler
 // spills: of D = 64 none or two, of D = 128 14 to 18, with slopes 26 and 33, of
